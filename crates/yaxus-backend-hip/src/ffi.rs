@@ -33,6 +33,13 @@ pub const YX_DTYPE_F32: c_int = 0;
 pub const YX_DTYPE_F16: c_int = 1;
 pub const YX_K: c_int = 0;
 pub const YX_V: c_int = 1;
+pub const YX_ACT_NONE: c_int = 0;
+pub const YX_ACT_RELU: c_int = 1;
+pub const YX_ACT_SILU: c_int = 2;
+pub const YX_ACT_GELU: c_int = 3;
+pub const YX_ACT_GELU_TANH: c_int = 4;
+pub const YX_MAX_TOP: c_int = 32;
+pub const YX_NO_TOKEN: u32 = 0xffff_ffff;
 pub const YX_KERNEL_ATTENTION: c_int = 0;
 pub const YX_KERNEL_APPEND: c_int = 1;
 pub const YX_KERNEL_COPY: c_int = 2;
@@ -96,6 +103,17 @@ unsafe extern "C" {
                               k: usize, n: usize) -> c_int;
     pub fn yx_argmax_rows_dev(ctx: *mut yx_ctx, logits: *const f32, rows: usize, cols: usize,
                               out: *mut u32) -> c_int;
+    pub fn yx_linear_bf16_dev(ctx: *mut yx_ctx, x: *const f32, w: *const u16, bias: *const f32,
+                              act: c_int, gated: c_int, residual: *const f32, out: *mut f32,
+                              t: usize, k: usize, n: usize) -> c_int;
+    pub fn yx_add_norm_rows_dev(ctx: *mut yx_ctx, x: *const f32, post_w: *const f32,
+                                post_offset: f32, h: *const f32, h_out: *mut f32, w: *const f32,
+                                offset: f32, out: *mut f32, eps: f32, rows: usize,
+                                cols: usize) -> c_int;
+    pub fn yx_logprobs_rows_dev(ctx: *mut yx_ctx, logits: *const f32, rows: usize, cols: usize,
+                                ld: usize, tokens: *const u32, given: usize, top: usize,
+                                logprob: *mut f32, entropy: *mut f32, top_ids: *mut u32,
+                                top_logprobs: *mut f32) -> c_int;
 
     pub fn yx_dev_alloc(ctx: *mut yx_ctx, bytes: usize, out: *mut *mut c_void) -> c_int;
     pub fn yx_dev_free(ctx: *mut yx_ctx, p: *mut c_void) -> c_int;

@@ -38,6 +38,11 @@ typedef struct yx_kv yx_kv;
 
 enum { YX_DTYPE_F32 = 0, YX_DTYPE_F16 = 1 };
 enum { YX_K = 0, YX_V = 1 };
+/* Activations of yx_linear_bf16_dev; gelu with the error function, or its tanh form. */
+enum { YX_ACT_NONE = 0, YX_ACT_RELU = 1, YX_ACT_SILU = 2, YX_ACT_GELU = 3, YX_ACT_GELU_TANH = 4 };
+/* Most alternatives of yx_logprobs_rows_dev, and the id where a row has fewer. */
+enum { YX_MAX_TOP = 32 };
+#define YX_NO_TOKEN 0xffffffffu
 /* Kernels whose launches yx_profile_read reports. */
 enum { YX_KERNEL_ATTENTION = 0, YX_KERNEL_APPEND = 1, YX_KERNEL_COPY = 2, YX_KERNEL_QK_ROPE = 3 };
 
@@ -213,6 +218,43 @@ int yx_matmul_bf16_dev(yx_ctx* ctx, const float* x, const uint16_t* w, float* ou
  * never chosen, and a row with nothing above -inf gives 0. out is a device array of
  * `rows` u32. */
 int yx_argmax_rows_dev(yx_ctx* ctx, const float* logits, size_t rows, size_t cols, uint32_t* out);
+
+/* yx_matmul_bf16_dev with the operations that follow a product in a model's block, in the
+ * product's epilogue (no counterpart in the reference, whose backends run them one by one):
+ *   y = x w^T + bias;  out = act(y) + residual                        (gated 0: w `[n][k]`)
+ *   out = act(y_gate) * y_up + residual    (gated 1: w `[2n][k]`, the n gate rows first)
+ * bias `[n]` (`[2n]` gated) and residual `[t][n]` are f32 and may be null; residual may be
+ * out itself (rows added to in place), otherwise out overlaps no input. act is a YX_ACT_*
+ * value. Sums, activation, gate and residual are f32 (an activation is within 2^-21 of its
+ * argument, gelu 2^-19); -inf gives NaN in silu and the gelus. k a
+ * multiple of 8, x and w 16-byte aligned, the others 4-byte aligned (16-byte accesses where
+ * all are 16-byte aligned and n is a multiple of 4). matmul_k_split applies as above, and
+ * the statistics matmul_kernel and matmul_k_parts report these calls too. */
+int yx_linear_bf16_dev(yx_ctx* ctx, const float* x, const uint16_t* w, const float* bias, int act,
+                       int gated, const float* residual, float* out, size_t t, size_t k, size_t n);
+/* The seam between two blocks (f32, `[rows][cols]`): with norm(v; w, o)_i =
+ * v_i / sqrt(mean v^2 + eps) * (o + w_i),
+ *   u = norm(x; post_w, post_offset), or x where post_w is null
+ *   h' = h + u, or u where h is null; stored to h_out unless that is null
+ *   out = norm(h'; w, offset)  (w and out both, or neither)
+ * So x, w and out alone are a plain RMSNorm. h_out and out may each be x or h itself,
+ * otherwise they overlap no input and never each other. */
+int yx_add_norm_rows_dev(yx_ctx* ctx, const float* x, const float* post_w, float post_offset,
+                         const float* h, float* h_out, const float* w, float offset, float* out,
+                         float eps, size_t rows, size_t cols);
+/* Of each row of logits (f32, `rows` rows of `cols` values, `ld` values apart): the log
+ * probabilities logprob `[rows][given]` of tokens `[rows][given]`, the entropy `[rows]` in
+ * nats (null: not computed), and the `top` (at most YX_MAX_TOP) most probable tokens, top_ids
+ * and top_logprobs `[rows][top]`, larger logit first, of equal ones the lower id first.
+ * Logits of -inf are masked tokens: probability 0, never an alternative; a row with fewer
+ * than `top` others ends in YX_NO_TOKEN and -inf. A row with nothing above -inf has no
+ * distribution: log probabilities -inf, entropy 0, no alternatives. NaN or +inf in a row
+ * makes its log probabilities and entropy NaN; NaN is never an alternative. A given token of
+ * `cols` or more (YX_NO_TOKEN for a row that has none) gets -inf (NaN in a NaN row). The same
+ * bits every time. Outputs overlap neither the inputs nor each other. */
+int yx_logprobs_rows_dev(yx_ctx* ctx, const float* logits, size_t rows, size_t cols, size_t ld,
+                         const uint32_t* tokens, size_t given, size_t top, float* logprob,
+                         float* entropy, uint32_t* top_ids, float* top_logprobs);
 
 /* Device memory and copies on the context's stream (h2d/d2h are synchronous). */
 int yx_dev_alloc(yx_ctx* ctx, size_t bytes, void** out);

@@ -23,6 +23,13 @@ YX_DTYPE_F32 = 0
 YX_DTYPE_F16 = 1
 YX_K = 0
 YX_V = 1
+YX_ACT_NONE = 0
+YX_ACT_RELU = 1
+YX_ACT_SILU = 2
+YX_ACT_GELU = 3
+YX_ACT_GELU_TANH = 4
+YX_MAX_TOP = 32
+YX_NO_TOKEN = 0xFFFFFFFF
 YX_KERNEL_ATTENTION = 0
 YX_KERNEL_APPEND = 1
 YX_KERNEL_COPY = 2
@@ -100,6 +107,9 @@ HIP_SYMBOLS = {
     "yx_ctx_get_stat": (I, [P, ctypes.c_char_p, P]),
     "yx_matmul_bf16_dev": (I, [P, P, P, P, S, S, S]),
     "yx_argmax_rows_dev": (I, [P, P, S, S, P]),
+    "yx_linear_bf16_dev": (I, [P, P, P, P, I, I, P, P, S, S, S]),
+    "yx_add_norm_rows_dev": (I, [P, P, P, F, P, P, P, F, P, F, S, S]),
+    "yx_logprobs_rows_dev": (I, [P, P, S, S, S, P, S, S, P, P, P, P]),
     "yx_fill_normal": (I, [P, P, S, I, U64, U64]),
     "yx_graph_begin": (I, [P]),
     "yx_graph_end": (I, [P]),

@@ -15,6 +15,7 @@ that cannot open a gfx950 device, raises: nothing here computes on the host.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import numpy as np
 
@@ -27,6 +28,21 @@ def _need(t, nbytes, what):
     pointers, so a short buffer would be read or written past its end."""
     if t.nbytes < nbytes:
         raise ValueError(f"{what}: device tensor of {t.nbytes} bytes, {nbytes} needed")
+
+
+# The activations of HipBackend.linear_bf16.
+ACTIVATIONS = {"none": _lib.YX_ACT_NONE, "relu": _lib.YX_ACT_RELU, "silu": _lib.YX_ACT_SILU,
+               "gelu": _lib.YX_ACT_GELU, "gelu_tanh": _lib.YX_ACT_GELU_TANH}
+
+
+class LogProbs(NamedTuple):
+    """HipBackend.logprobs_rows' device tensors: logprob `[rows][given]`, entropy `[rows]`,
+    top_ids and top_logprobs `[rows][top]`."""
+
+    logprob: object
+    entropy: object
+    top_ids: object
+    top_logprobs: object
 
 
 class DeviceTensor:
@@ -308,6 +324,87 @@ class HipBackend:
         out = out if out is not None else self.tensor((rows,), np.uint32)
         _need(out, rows * 4, "out")
         check_hip(self.L.yx_argmax_rows_dev(self.ctx, logits.ptr, rows, cols, out.ptr))
+        return out
+
+    def linear_bf16(self, x, w, bias=None, act="none", gated=False, residual=None, out=None):
+        """act(x w^T + bias) + residual in one launch (yx_linear_bf16_dev): x `[t][k]` f32, w
+        `[n][k]` bf16 bits, bias `[n]` and residual `[t][n]` f32 device tensors; ``gated``: w
+        `[2n][k]` and bias `[2n]` hold the gate's rows, then the up projection's, and the
+        result is act(gate) * up + residual. act: one of ``ACTIVATIONS``. ``out`` may be the
+        residual itself. Returns `[t][n]` f32."""
+        t, k = x.shape
+        n = w.shape[0]
+        if w.shape[1] != k:
+            raise ValueError("x and w disagree on k")
+        if gated:
+            if n % 2:
+                raise ValueError("a gated w has as many gate rows as up rows")
+            n //= 2
+        if act not in ACTIVATIONS:
+            raise ValueError(f"act must be one of {', '.join(ACTIVATIONS)}")
+        _need(x, t * k * 4, "x")
+        _need(w, w.shape[0] * k * 2, "w")
+        if bias is not None:
+            _need(bias, w.shape[0] * 4, "bias")
+        if residual is not None:
+            _need(residual, t * n * 4, "residual")
+        out = out if out is not None else self.tensor((t, n))
+        _need(out, t * n * 4, "out")
+        check_hip(self.L.yx_linear_bf16_dev(self.ctx, x.ptr, w.ptr, bias and bias.ptr,
+                                            ACTIVATIONS[act], 1 if gated else 0,
+                                            residual and residual.ptr, out.ptr, t, k, n))
+        return out
+
+    def add_norm(self, x, w=None, eps=1e-6, offset=1.0, post_w=None, post_offset=1.0, h=None,
+                 h_out=None, out=None):
+        """The seam between two blocks in one launch (yx_add_norm_rows_dev): u = norm(x) with
+        post_w where given, else x; h' = h + u where h is given, else u; out = norm(h') with w
+        where given. norm(v) = v / sqrt(mean(v^2) + eps) * (offset + weight). x and h
+        `[rows][cols]`, weights `[cols]`, f32. ``h_out`` (h' stored) and ``out`` may each be x or
+        h itself. Returns (h_out, out); h_out is made where h or post_w is given and it is not,
+        out where w is."""
+        rows, cols = x.shape
+        b = rows * cols * 4
+        if w is not None and out is None:
+            out = self.tensor((rows, cols))
+        if w is None and out is not None:
+            raise ValueError("out needs the norm's weight w")
+        if h_out is None and (w is None or h is not None or post_w is not None):
+            h_out = self.tensor((rows, cols))
+        for v, need, what in ((x, b, "x"), (h, b, "h"), (h_out, b, "h_out"), (out, b, "out"),
+                              (w, cols * 4, "w"), (post_w, cols * 4, "post_w")):
+            if v is not None:
+                _need(v, need, what)
+        check_hip(self.L.yx_add_norm_rows_dev(self.ctx, x.ptr, post_w and post_w.ptr, post_offset,
+                                              h and h.ptr, h_out and h_out.ptr, w and w.ptr, offset,
+                                              out and out.ptr, eps, rows, cols))
+        return h_out, out
+
+    def logprobs_rows(self, logits, tokens=None, top=0, cols=None, out=None):
+        """Log probabilities, entropy and top alternatives of rows of logits
+        (yx_logprobs_rows_dev). logits `[rows][ld]` f32, of each row the first ``cols`` (default:
+        all) are the vocabulary; tokens `[rows][given]` (or `[rows]`) uint32. Returns
+        ``LogProbs``; ``out`` is four device tensors to use instead of new ones."""
+        rows, ld = logits.shape
+        cols = ld if cols is None else cols
+        given = 0 if tokens is None else tokens.shape[1] if len(tokens.shape) > 1 else 1
+        if tokens is not None and tokens.shape[0] != rows:
+            raise ValueError("tokens and logits disagree on the rows")
+        if out is None:
+            out = LogProbs(self.tensor((rows, given)), self.tensor((rows,)),
+                           self.tensor((rows, top), np.uint32), self.tensor((rows, top)))
+        lp, entropy, ids, tlp = out
+        _need(logits, rows * ld * 4, "logits")
+        if given:
+            _need(tokens, rows * given * 4, "tokens")
+            _need(lp, rows * given * 4, "logprob")
+        _need(entropy, rows * 4, "entropy")
+        if top:
+            _need(ids, rows * top * 4, "top_ids")
+            _need(tlp, rows * top * 4, "top_logprobs")
+        check_hip(self.L.yx_logprobs_rows_dev(self.ctx, logits.ptr, rows, cols, ld,
+                                              tokens.ptr if given else None, given, top, lp.ptr,
+                                              entropy.ptr, ids.ptr, tlp.ptr))
         return out
 
     def stat(self, key):

@@ -15,11 +15,11 @@
 #include <type_traits>
 
 #include "attn_decode.hpp"
+#include "epilogue.hpp"
 
 namespace yx {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 // The bf16 parts of two f32 values, packed: h, m, l hold (value 1 << 16 | value 0). An
@@ -39,19 +39,6 @@ __device__ __forceinline__ void split_bf16x3(float f0, float f1, uint32_t& h, ui
   h = __builtin_amdgcn_perm(hb[1], hb[0], 0x07060302);  // the upper halves of both
   m = __builtin_amdgcn_perm(mb[1], mb[0], 0x07060302);
   l = __builtin_amdgcn_perm(lb[1], lb[0], 0x07060302);
-}
-
-// A lane's four outputs of a 16 x 16 tile: columns col .. col + 3 of one row.
-__device__ __forceinline__ void store_out4(float* out, uint32_t row, uint32_t col, uint32_t n, bool wide,
-                                           const f32x4& v) {
-  float* o = out + static_cast<size_t>(row) * n + col;
-  if (wide) {  // n a multiple of 4, out 16-byte aligned
-    if (col < n) *reinterpret_cast<f32x4*>(o) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < n) o[i] = v[i];
-  }
 }
 
 // ---- many rows -------------------------------------------------------------------
@@ -332,13 +319,14 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
         for (int b = 0; b < MT; ++b)
           sum[a][b] = sum[a][b] + __builtin_bit_cast(f32x4, ld4_coherent(rp, (base + q * kTile + (a * MT + b) * 64) * 16));
   }
-  const bool wide = (n & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const bool wide = wide_out(NoEpilogue{}, out, n);
 #pragma unroll
   for (int b = 0; b < MT; ++b) {
     const uint32_t row = t0 + (wm * MT + b) * 16 + c;
     if (row >= t) continue;
 #pragma unroll
-    for (int a = 0; a < NT; ++a) store_out4(out, row, n0 + (wn * NT + a) * 16 + 4 * g, n, wide, sum[a][b]);
+    for (int a = 0; a < NT; ++a)
+      store_out4(NoEpilogue{}, out, row, n0 + (wn * NT + a) * 16 + 4 * g, n, wide, sum[a][b], sum[a][b]);
   }
 }
 
@@ -397,7 +385,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void matmul_bf16_stream(
     for (int u = 0; u < S; ++u)
       r[u] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(rw, voff + u * 64, 0, 0));
   };
-  const bool wide = (n & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const bool wide = wide_out(NoEpilogue{}, out, n);
   u16x8 wv[2][S];
   uint32_t b = blockIdx.x, j = 0, half = 0;  // this tile: the j-th of batch b
   uint32_t lb = b, lj = 0;                   // the next one to load
@@ -428,7 +416,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void matmul_bf16_stream(
         f32x4 s = part[half][wave][0][lane];
 #pragma unroll
         for (int q = 1; q < kStreamWaves; ++q) s = s + part[half][wave][q][lane];
-        if (static_cast<uint32_t>(c) < t) store_out4(out, c, tile * 16 + 4 * g, n, wide, s);
+        if (static_cast<uint32_t>(c) < t) store_out4(NoEpilogue{}, out, c, tile * 16 + 4 * g, n, wide, s, s);
       }
       half ^= 1;
       j = 0;

@@ -15,11 +15,13 @@
 #include <vector>
 
 #include "../../include/yaxus_hip.h"
+#include "add_norm.hpp"
 #include "attn_decode.hpp"
 #include "attn_prefill.hpp"
 #include "attn_prefill_f32.hpp"
 #include "deal.hpp"
 #include "kv_kernels.hpp"
+#include "logprobs.hpp"
 #include "qk_rope.hpp"
 #include "step_after.hpp"
 
@@ -1534,6 +1536,21 @@ int matmul_scratch(yx_ctx* c, size_t tiles, size_t ks) {
   return c->mm_counters.ensure(cnt, c->stream, true);
 }
 
+template <class E>
+int matmul_rows(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
+                size_t ks, const E& epi) {
+  const uint32_t ntn = (n + 15) / 16, ntt = (t + 15) / 16;
+  c->mm_kernel = 1;
+  c->mm_k_parts = ks;
+  if (ks > 1)
+    if (int rc = matmul_scratch(c, static_cast<size_t>(ntn) * ntt * (E::kGated ? 2 : 1), ks)) return rc;
+  hipLaunchKernelGGL(yx::matmul_bf16_rows<E>, dim3(ntn, ntt, static_cast<unsigned>(ks)), dim3(64 * yx::kMmWaves), 0,
+                     c->stream, x, w, out, t, k, n, static_cast<yx::f32x4*>(c->mm_part.p),
+                     static_cast<uint32_t>(c->mm_part.cap), static_cast<uint32_t*>(c->mm_counters.p), epi);
+  YX_HIP(hipGetLastError());
+  return YX_OK;
+}
+
 // At most 16 rows against many weight rows: the streaming kernel, for the k it is built
 // for (false: another one). From two 16-row tiles per CU on, where matmul_bf16_rows does
 // not split k (so the bits are the same): n 8192, k 2048 14.9 -> 10.5 us; at n 4096 8.9
@@ -1636,6 +1653,39 @@ bool matmul_rows_faster(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n, double ti
   const double passes = std::ceil(steps / (yx::kMmWaves * yx::kMmSteps)), x_mb = 4e-6 * t * k;
   const double rows_us = 2.65 + per_cu * (steps / 16 - 0.5) + std::ceil(per_cu) * passes + 0.043 * x_mb * std::min(8.0, nt);
   return rows_us < 1.05 * tiles_us - 1.5 + (n % 4 ? 0.9 : 0.0);
+}
+
+// Workgroups per output tile of matmul_bf16_rows along k: about two workgroups per CU in
+// all, each wave at least one pass of its loop (kMmSteps steps of 32).
+size_t matmul_rows_split(const yx_ctx* c, size_t tiles, size_t steps) {
+  if (c->matmul_k_split > 0) return std::min<size_t>(static_cast<size_t>(c->matmul_k_split), steps);
+  return std::max<size_t>(1, std::min<size_t>({(2 * static_cast<size_t>(c->cus) + tiles - 1) / tiles,
+                                               steps / (yx::kMmWaves * yx::kMmSteps), 64}));
+}
+
+int matmul_check(const void* x, const void* w, size_t t, size_t k, size_t n) {
+  if (k == 0 || k % 8) return fail(YX_ERR_UNSUPPORTED, "k must be a positive multiple of 8");
+  if (t > 0xffffffffu || k > 0xffffffffu || n > 0xffffffffu || (n + 15) / 16 > 0x7fffffff ||
+      (t + 15) / 16 > 0xffff)
+    return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
+  if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(w) % 16)
+    return fail(YX_ERR_INVALID, "x and w must be 16-byte aligned");
+  return YX_OK;
+}
+
+// Whether two buffers share a byte (null: none).
+bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + bn && y < x + an;
+}
+
+// yx_linear_bf16_dev, its arguments checked.
+template <class E>
+int linear_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
+                const E& epi) {
+  const size_t steps = (static_cast<size_t>(k) + 31) / 32;
+  const size_t tiles16 = static_cast<size_t>((n + 15) / 16) * ((t + 15) / 16);
+  return matmul_rows(c, x, w, out, t, k, n, matmul_rows_split(c, tiles16, steps), epi);
 }
 
 int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
@@ -2362,14 +2412,8 @@ int yx_matmul_bf16_dev(yx_ctx* c, const float* x, const uint16_t* w, float* out,
   if (!c) return fail(YX_ERR_INVALID, "null context");
   if (t == 0 || n == 0) return YX_OK;
   if (!x || !w || !out) return fail(YX_ERR_INVALID, "null x, w or out");
-  if (k == 0 || k % 8) return fail(YX_ERR_UNSUPPORTED, "k must be a positive multiple of 8");
-  if (t > 0xffffffffu || k > 0xffffffffu || n > 0xffffffffu || (n + 15) / 16 > 0x7fffffff ||
-      (t + 15) / 16 > 0xffff)
-    return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
-  if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(w) % 16)
-    return fail(YX_ERR_INVALID, "x and w must be 16-byte aligned");
-  int rc = c->set_device();
-  if (rc) return rc;
+  int rc = matmul_check(x, w, t, k, n);
+  if (rc || (rc = c->set_device())) return rc;
   const size_t steps = (k + 31) / 32;
   const auto T = static_cast<uint32_t>(t), K = static_cast<uint32_t>(k), N = static_cast<uint32_t>(n);
   const size_t tiles16 = ((n + 15) / 16) * ((t + 15) / 16);
@@ -2385,21 +2429,58 @@ int yx_matmul_bf16_dev(yx_ctx* c, const float* x, const uint16_t* w, float* out,
       if (!matmul_rows_faster(c, T, K, N, split.us)) return matmul_tiled(c, x, w, out, T, K, N, split);
     }
   }
-  // Workgroups per output tile along k: about two workgroups per CU in all, each wave
-  // at least one pass of its loop (kMmSteps steps of 32).
-  const size_t tiles = tiles16;
-  size_t ks = std::max<size_t>(1, std::min<size_t>({(2 * slots + tiles - 1) / tiles,
-                                                     steps / (yx::kMmWaves * yx::kMmSteps), 64}));
-  if (c->matmul_k_split > 0) ks = std::min<size_t>(static_cast<size_t>(c->matmul_k_split), steps);
-  c->mm_kernel = 1;
-  c->mm_k_parts = ks;
-  if (ks > 1 && (rc = matmul_scratch(c, tiles, ks))) return rc;
-  hipLaunchKernelGGL(yx::matmul_bf16_rows,
-                     dim3(static_cast<unsigned>((n + 15) / 16), static_cast<unsigned>((t + 15) / 16),
-                          static_cast<unsigned>(ks)),
-                     dim3(64 * yx::kMmWaves), 0, c->stream, x, w, out, T, K, N,
-                     static_cast<yx::f32x4*>(c->mm_part.p), static_cast<uint32_t>(c->mm_part.cap),
-                     static_cast<uint32_t*>(c->mm_counters.p));
+  return matmul_rows(c, x, w, out, T, K, N, matmul_rows_split(c, tiles16, steps), yx::NoEpilogue{});
+}
+
+int yx_linear_bf16_dev(yx_ctx* c, const float* x, const uint16_t* w, const float* bias, int act, int gated,
+                       const float* residual, float* out, size_t t, size_t k, size_t n) {
+  if (!c) return fail(YX_ERR_INVALID, "null context");
+  if (act < YX_ACT_NONE || act > YX_ACT_GELU_TANH) return fail(YX_ERR_INVALID, "unknown activation");
+  if (gated != 0 && gated != 1) return fail(YX_ERR_INVALID, "gated is 0 or 1");
+  if (t == 0 || n == 0) return YX_OK;
+  if (!x || !w || !out) return fail(YX_ERR_INVALID, "null x, w or out");
+  const size_t m = gated ? 2 : 1;
+  if (n > 0x7fffffffu) return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
+  int rc = matmul_check(x, w, t, k, m * n);
+  if (rc) return rc;
+  for (const void* p : {static_cast<const void*>(out), static_cast<const void*>(bias), static_cast<const void*>(residual)})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(YX_ERR_INVALID, "bias, residual and out must be 4-byte aligned");
+  const size_t ob = t * n * 4;
+  if (overlap(out, ob, x, t * k * 4) || overlap(out, ob, w, m * n * k * 2) || overlap(out, ob, bias, m * n * 4) ||
+      (residual != out && overlap(out, ob, residual, ob)))
+    return fail(YX_ERR_INVALID, "out overlaps an input (the residual may be out itself)");
+  if ((rc = c->set_device())) return rc;
+  const auto T = static_cast<uint32_t>(t), K = static_cast<uint32_t>(k), N = static_cast<uint32_t>(n);
+  if (gated) return linear_impl(c, x, w, out, T, K, N, yx::Epilogue<true>{bias, residual, static_cast<uint32_t>(act)});
+  return linear_impl(c, x, w, out, T, K, N, yx::Epilogue<false>{bias, residual, static_cast<uint32_t>(act)});
+}
+
+int yx_add_norm_rows_dev(yx_ctx* c, const float* x, const float* post_w, float post_offset, const float* h,
+                         float* h_out, const float* w, float offset, float* out, float eps, size_t rows,
+                         size_t cols) {
+  if (!c) return fail(YX_ERR_INVALID, "null context");
+  if ((w == nullptr) != (out == nullptr)) return fail(YX_ERR_INVALID, "w and out go together");
+  if (!h_out && !out) return fail(YX_ERR_INVALID, "nothing to compute: no h_out and no out");
+  if (!(eps >= 0.0f)) return fail(YX_ERR_INVALID, "eps must not be negative");
+  if (rows == 0 || cols == 0) return YX_OK;
+  if (!x) return fail(YX_ERR_INVALID, "null x");
+  if (rows > 0x7fffffffu || cols > 0x7fffffffu) return fail(YX_ERR_UNSUPPORTED, "add_norm dimensions too large");
+  if (rows > (size_t{1} << 48) / cols) return fail(YX_ERR_UNSUPPORTED, "add_norm dimensions too large");
+  const size_t b = rows * cols * 4, wb = cols * 4;
+  for (const void* p : {static_cast<const void*>(x), static_cast<const void*>(post_w), static_cast<const void*>(h),
+                        static_cast<const void*>(h_out), static_cast<const void*>(w), static_cast<const void*>(out)})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(YX_ERR_INVALID, "add_norm buffers must be 4-byte aligned");
+  if (overlap(h_out, b, out, b)) return fail(YX_ERR_INVALID, "h_out and out overlap");
+  for (const float* o : {h_out, out}) {
+    if ((o != x && overlap(o, b, x, b)) || (o != h && overlap(o, b, h, b)))
+      return fail(YX_ERR_INVALID, "an output overlaps x or h without being it");
+    if (overlap(o, b, post_w, wb) || overlap(o, b, w, wb)) return fail(YX_ERR_INVALID, "an output overlaps a weight");
+  }
+  int rc = c->set_device();
+  if (rc) return rc;
+  const yx::AddNorm a{x, post_w, h, h_out, w, out, post_offset, offset, eps};
+  hipLaunchKernelGGL(yx::add_norm_rows, dim3(static_cast<unsigned>(rows)), dim3(yx::kNormThreads), 0, c->stream, a,
+                     static_cast<uint32_t>(cols));
   YX_HIP(hipGetLastError());
   return YX_OK;
 }
@@ -2424,6 +2505,46 @@ int yx_argmax_rows_dev(yx_ctx* c, const float* logits, size_t rows, size_t cols,
   hipLaunchKernelGGL(yx::argmax_rows, dim3(static_cast<unsigned>(nsl), static_cast<unsigned>(rows)),
                      dim3(yx::kArgmaxThreads), 0, c->stream, logits, static_cast<uint32_t>(cols), out,
                      static_cast<unsigned long long*>(c->am_keys.p), static_cast<uint32_t*>(c->am_counters.p));
+  YX_HIP(hipGetLastError());
+  return YX_OK;
+}
+
+int yx_logprobs_rows_dev(yx_ctx* c, const float* logits, size_t rows, size_t cols, size_t ld,
+                         const uint32_t* tokens, size_t given, size_t top, float* logprob, float* entropy,
+                         uint32_t* top_ids, float* top_logprobs) {
+  if (!c) return fail(YX_ERR_INVALID, "null context");
+  if (top > YX_MAX_TOP) return fail(YX_ERR_UNSUPPORTED, "more alternatives than YX_MAX_TOP");
+  if (rows == 0) return YX_OK;
+  if (!logits) return fail(YX_ERR_INVALID, "null logits");
+  if (cols == 0) return fail(YX_ERR_INVALID, "empty rows");
+  if (ld < cols) return fail(YX_ERR_INVALID, "the row stride is below the row's length");
+  if (given && (!tokens || !logprob)) return fail(YX_ERR_INVALID, "null tokens or logprob");
+  if (top && (!top_ids || !top_logprobs)) return fail(YX_ERR_INVALID, "null top_ids or top_logprobs");
+  if (!given && !top && !entropy) return fail(YX_ERR_INVALID, "nothing to compute");
+  constexpr size_t kMost = size_t{1} << 48;  // values of one buffer
+  if (rows > 0x7fffffffu || cols > 0x7fffffffu || given > 0x7fffffffu || ld > kMost / rows || given > kMost / rows)
+    return fail(YX_ERR_UNSUPPORTED, "logprobs dimensions too large");
+  if (!given) logprob = nullptr;
+  const size_t lb = ((rows - 1) * ld + cols) * 4;
+  const struct {
+    const void* p;
+    size_t bytes;
+  } outs[] = {{logprob, rows * given * 4}, {entropy, rows * 4}, {top ? top_ids : nullptr, rows * top * 4},
+              {top ? top_logprobs : nullptr, rows * top * 4}};
+  for (const auto& o : outs) {
+    if (reinterpret_cast<uintptr_t>(o.p) % 4) return fail(YX_ERR_INVALID, "logprobs buffers must be 4-byte aligned");
+    if (overlap(o.p, o.bytes, logits, lb) || (given && overlap(o.p, o.bytes, tokens, rows * given * 4)))
+      return fail(YX_ERR_INVALID, "an output overlaps an input");
+    for (const auto& q : outs)
+      if (&q != &o && overlap(o.p, o.bytes, q.p, q.bytes)) return fail(YX_ERR_INVALID, "two outputs overlap");
+  }
+  if (reinterpret_cast<uintptr_t>(logits) % 4 || reinterpret_cast<uintptr_t>(tokens) % 4)
+    return fail(YX_ERR_INVALID, "logprobs buffers must be 4-byte aligned");
+  int rc = c->set_device();
+  if (rc) return rc;
+  hipLaunchKernelGGL(yx::logprobs_rows, dim3(static_cast<unsigned>(rows)), dim3(yx::kLpThreads), 0, c->stream, logits,
+                     static_cast<uint32_t>(cols), ld, tokens, static_cast<uint32_t>(given),
+                     static_cast<uint32_t>(top), yx::LogprobsOut{logprob, entropy, top_ids, top_logprobs});
   YX_HIP(hipGetLastError());
   return YX_OK;
 }

@@ -16,6 +16,8 @@
 //   A (weight): lane (c, g) holds w[n0 + c][k + 8g .. k + 8g + 7]
 //   B (x part): lane (c, g) holds x[t0 + c][k + 8g .. k + 8g + 7]
 //   D: lane (c, g) holds out[t0 + c][n0 + 4g + i], i = 0..3
+// A gated epilogue's workgroup owns 16 columns of the output, so 16 gate rows and 16 up rows
+// of the weight: x is cut up once for both, and a lane holds both sums of its outputs.
 //
 // argmax_rows: per row the first index of the largest value; NaN is never chosen and a
 // row with nothing above -inf gives 0, as the CPU loop does (best starts at (0, -inf),
@@ -35,20 +37,20 @@ namespace yx {
 static constexpr int kMmWaves = 8;
 static constexpr int kMmSteps = 4;  // 32-wide k steps per wave and pass of its loop
 
-// t rows of x [t][k] f32, w [n][k] bf16 bits, out [t][n] f32. Grid: (ceil(n / 16),
+// t rows of x [t][k] f32, w [n][k] bf16 bits ([2n][k] gated), out [t][n] f32. Grid: (ceil(n / 16),
 // ceil(t / 16), ks): the ks workgroups of an output tile take consecutive parts of k
 // (whole 32-wide steps), their 8 waves eighths of those; k a multiple of 8
 // (host-checked), n and t any. With ks > 1 each workgroup's tile goes to part (write-
 // through) and the tile's last workgroup to arrive (counters, left at zero) adds the
 // parts in k order.
+template <class E>
 __global__ __launch_bounds__(64 * kMmWaves) void matmul_bf16_rows(const float* __restrict__ x,
-                                                                  const uint16_t* __restrict__ w,
-                                                                  float* __restrict__ out, uint32_t t,
-                                                                  uint32_t k, uint32_t n,
-                                                                  f32x4* __restrict__ part,
-                                                                  uint32_t part_bytes,
-                                                                  uint32_t* __restrict__ counters) {
-  __shared__ f32x4 wpart[kMmWaves][64];
+                                                                  const uint16_t* __restrict__ w, float* out,
+                                                                  uint32_t t, uint32_t k, uint32_t n,
+                                                                  f32x4* __restrict__ part, uint32_t part_bytes,
+                                                                  uint32_t* __restrict__ counters, E epi) {
+  constexpr int W = E::kGated ? 2 : 1;  // weight rows per output column
+  __shared__ f32x4 wpart[kMmWaves][W][64];
   __shared__ uint32_t last;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -62,17 +64,22 @@ __global__ __launch_bounds__(64 * kMmWaves) void matmul_bf16_rows(const float* _
   const uint32_t p0 = steps * kp / ks, p1 = steps * (kp + 1) / ks;
   const uint32_t s0 = p0 + (p1 - p0) * wave / kMmWaves, s1 = p0 + (p1 - p0) * (wave + 1) / kMmWaves;
   const uint16_t* wp = w + static_cast<size_t>(wrow ? wn : 0) * k;
+  const size_t up = static_cast<size_t>(n) * k;  // gated: from a gate row to its up row
   const float* xp = x + static_cast<size_t>(xrow ? xt : 0) * k;
-  f32x4 acc = {0, 0, 0, 0};
+  f32x4 acc[W];
+#pragma unroll
+  for (int j = 0; j < W; ++j) acc[j] = f32x4{0, 0, 0, 0};
   for (uint32_t s = s0; s < s1; s += kMmSteps) {
-    u16x8 wv[kMmSteps];
+    u16x8 wv[kMmSteps][W];
     f32x4 xa[kMmSteps], xb[kMmSteps];
 #pragma unroll
     for (int u = 0; u < kMmSteps; ++u) {
       const uint32_t kk = (s + u) * 32 + 8 * g;
       const bool ok = (s + u < s1) & (kk < k);
-      wv[u] = (ok & wrow) ? __builtin_nontemporal_load(reinterpret_cast<const u16x8*>(wp + kk))
-                          : u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        wv[u][j] = (ok & wrow) ? __builtin_nontemporal_load(reinterpret_cast<const u16x8*>(wp + j * up + kk))
+                               : u16x8{0, 0, 0, 0, 0, 0, 0, 0};
       xa[u] = (ok & xrow) ? *reinterpret_cast<const f32x4*>(xp + kk) : f32x4{0, 0, 0, 0};
       xb[u] = (ok & xrow) ? *reinterpret_cast<const f32x4*>(xp + kk + 4) : f32x4{0, 0, 0, 0};
     }
@@ -93,26 +100,33 @@ __global__ __launch_bounds__(64 * kMmWaves) void matmul_bf16_rows(const float* _
         mid[e] = static_cast<__bf16>(xm);
         lo[e] = static_cast<__bf16>(r1 - xm);
       }
-      const bf16x8 a = __builtin_bit_cast(bf16x8, wv[u]);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, hi, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, mid, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, lo, acc, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const bf16x8 a = __builtin_bit_cast(bf16x8, wv[u][j]);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, hi, acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, mid, acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, lo, acc[j], 0, 0, 0);
+      }
     }
   }
-  wpart[wave][lane] = acc;
+#pragma unroll
+  for (int j = 0; j < W; ++j) wpart[wave][j][lane] = acc[j];
   __syncthreads();
   const size_t tile = static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x;
-  f32x4 sum = {0, 0, 0, 0};
+  const auto at = [&](uint32_t q, int j) { return static_cast<uint32_t>((((tile * ks + q) * W + j) * 64 + lane) * 16); };
+  f32x4 sum[W];
   if (wave == 0) {
-    sum = wpart[0][lane];
 #pragma unroll
-    for (int wv = 1; wv < kMmWaves; ++wv) {
-      const f32x4 q = wpart[wv][lane];
-      sum = f32x4{sum.x + q.x, sum.y + q.y, sum.z + q.z, sum.w + q.w};
+    for (int j = 0; j < W; ++j) {
+      sum[j] = wpart[0][j][lane];
+#pragma unroll
+      for (int wv = 1; wv < kMmWaves; ++wv) {
+        const f32x4 q = wpart[wv][j][lane];
+        sum[j] = f32x4{sum[j].x + q.x, sum[j].y + q.y, sum[j].z + q.z, sum[j].w + q.w};
+      }
+      if (ks > 1)  // to memory all XCDs share (write-through) before the arrival
+        st4_coherent(make_rsrc(part, part_bytes), at(kp, j), __builtin_bit_cast(float4, sum[j]));
     }
-    if (ks > 1)  // to memory all XCDs share (write-through) before the arrival
-      st4_coherent(make_rsrc(part, part_bytes), static_cast<uint32_t>(((tile * ks + kp) * 64 + lane) * 16),
-                   __builtin_bit_cast(float4, sum));
   }
   if (ks > 1) {
     __builtin_amdgcn_s_waitcnt(0);
@@ -126,20 +140,27 @@ __global__ __launch_bounds__(64 * kMmWaves) void matmul_bf16_rows(const float* _
     }
     __syncthreads();
     if (!last || wave != 0) return;
-    sum = f32x4{0, 0, 0, 0};
     const __amdgpu_buffer_rsrc_t rp = make_rsrc(part, part_bytes);
+#pragma unroll
+    for (int j = 0; j < W; ++j) sum[j] = f32x4{0, 0, 0, 0};
     for (uint32_t q = 0; q < ks; ++q) {  // the parts in k order
-      const f32x4 v = __builtin_bit_cast(f32x4, ld4_coherent(rp, static_cast<uint32_t>(((tile * ks + q) * 64 + lane) * 16)));
-      sum = q == 0 ? v : f32x4{sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w};
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const f32x4 v = __builtin_bit_cast(f32x4, ld4_coherent(rp, at(q, j)));
+        sum[j] = q == 0 ? v : f32x4{sum[j].x + v.x, sum[j].y + v.y, sum[j].z + v.z, sum[j].w + v.w};
+      }
     }
   } else if (wave != 0) {
     return;
   }
-  if (xrow) {
+  if (!xrow) return;
+  if constexpr (E::kFused) {
+    store_out4(epi, out, xt, n0 + 4 * g, n, wide_out(epi, out, n), sum[0], sum[W - 1]);
+  } else {
     float* o = out + static_cast<size_t>(xt) * n + n0 + 4 * g;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (n0 + 4 * g + i < n) o[i] = sum[i];
+      if (n0 + 4 * g + i < n) o[i] = sum[0][i];
   }
 }
 
