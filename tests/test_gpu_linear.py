@@ -145,7 +145,7 @@ def test_epilogues(hip, t, k, n, act, gated, bias, residual, skip):
         np.testing.assert_array_equal(run(hip, x, w, b, act, gated, r, in_place=True, skip=skip), got)
 
 
-@pytest.mark.parametrize("t,k,n", [(1, 2048, 2048), (16, 2048, 8192), (40, 2048, 250)])
+@pytest.mark.parametrize("t,k,n", [(1, 2048, 2048), (16, 2048, 8192), (40, 2048, 250), (333, 1536, 1501), (600, 2048, 2048)])
 def test_without_an_epilogue_it_is_the_matmul(hip, t, k, n):
     x, w, _, _ = inputs(t, k, n, False)
     dx, dw = hip.tensor(x.shape).upload(x), hip.tensor(w.shape, np.uint16).upload(w)

@@ -64,6 +64,9 @@ __device__ __forceinline__ void split_bf16x3(float f0, float f1, uint32_t& h, ui
 // Accuracy: sums of at most an eighth of k (and at least two stages) are added to the
 // result in f32, as matmul_bf16_rows adds its waves' eighths; one chain over k = 2048
 // was 4.8e-7 off 64 bits (2-norm), this is 1.8e-7, as that kernel.
+// A gated epilogue's tile has TN / 2 output columns: 16 gate rows of the weight, the 16 up
+// rows that belong to them, the next 16 gate rows, so that a lane ends up with both sums of its
+// outputs; a wave's loads are from one of the two parts (8 or 16 consecutive rows).
 // With ks > 1 (grid y) the ks workgroups of a tile take consecutive stages and hand
 // their tiles over as matmul_bf16_rows does.
 // Measured (k = n = 2048): t 4096 702 -> 81 us (128 x 256 tiles, 425 TFLOP/s, 3x that in
@@ -78,15 +81,17 @@ using MatmulTileA = MatmulTile<128, 256, 4, 2, 1, 2>;
 using MatmulTileB = MatmulTile<128, 128, 4, 2, 1, 2>;
 using MatmulTileC = MatmulTile<64, 128, 2, 4, 2, 2>;
 using MatmulTileD = MatmulTile<64, 64, 2, 4, 2, 4>;
+using MatmulTileDGated = MatmulTile<64, 64, 4, 2, 2, 4>;  // two weight tiles per wave
 
-template <class T>
+template <class T, class E>
 __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_tiles(
-    const float* __restrict__ x, const uint16_t* __restrict__ w, float* __restrict__ out, uint32_t t,
-    uint32_t k, uint32_t n, f32x4* __restrict__ part, uint32_t part_bytes,
-    uint32_t* __restrict__ counters) {
+    const float* __restrict__ x, const uint16_t* __restrict__ w, float* out, uint32_t t, uint32_t k,
+    uint32_t n, f32x4* __restrict__ part, uint32_t part_bytes, uint32_t* __restrict__ counters, E epi) {
   constexpr int TM = T::TM, TN = T::TN, KU = T::KU, KT = T::KT, TH = kMatmulThreads;
   static_assert(T::WM * T::WN * 64 == TH, "8 waves");
   constexpr int MT = TM / T::WM / 16, NT = TN / T::WN / 16;  // 16 x 16 tiles per wave
+  constexpr int TC = E::kGated ? TN / 2 : TN;                // output columns
+  static_assert(!E::kGated || NT % 2 == 0, "a wave holds gate and up rows of its columns");
   // Chunks of 8 k per thread and stage.
   constexpr int XC = TM * KT / 8 / TH, WC = TN * KT / 8 / TH;
   static_assert(TM * KT / 8 == XC * TH && TN * KT / 8 == WC * TH, "whole rounds of chunks");
@@ -99,10 +104,10 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
   const int wm = wave / T::WN, wn = wave % T::WN;
   // Tiles so that those running on one XCD (workgroups are dealt to the 8 XCDs in turn)
   // are consecutive, the operand with fewer tiles fastest: they share operands in its L2.
-  const uint32_t ntn = (n + TN - 1) / TN, ntt = (t + TM - 1) / TM, tiles = ntn * ntt;
+  const uint32_t ntn = (n + TC - 1) / TC, ntt = (t + TM - 1) / TM, tiles = ntn * ntt;
   const uint32_t xcd = blockIdx.x & 7;
   const uint32_t tile = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (blockIdx.x >> 3);
-  const uint32_t n0 = (ntn <= ntt ? tile % ntn : tile / ntt) * TN;
+  const uint32_t n0 = (ntn <= ntt ? tile % ntn : tile / ntt) * TC;
   const uint32_t t0 = (ntn <= ntt ? tile / ntn : tile % ntt) * TM;
   const uint32_t ks = gridDim.y, kp = blockIdx.y;
   const uint32_t stages = (k + KT - 1) / KT;
@@ -123,13 +128,19 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
   for (int i = 0; i < WC; ++i) {
     const int id = i * TH + tid, row = id / (4 * KU), kc = id % (4 * KU);
     wk[i] = kc * 8;
-    wo[i] = (row * static_cast<int>(k) + kc * 8) * 2;
+    const int col = E::kGated ? row / 32 * 16 + row % 16 : row;
+    wo[i] = (col * static_cast<int>(k) + kc * 8) * 2;
     wd[i] = (kc / 4) * TN * 4 + row * 4 + ((kc & 3) ^ ((row >> 1) & 3));
   }
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(const_cast<float*>(x + static_cast<size_t>(t0) * k),
                                               min(t - t0, static_cast<uint32_t>(TM)) * k * 4);
-  const __amdgpu_buffer_rsrc_t rw = make_rsrc(const_cast<uint16_t*>(w + static_cast<size_t>(n0) * k),
-                                              min(n - n0, static_cast<uint32_t>(TN)) * k * 2);
+  // Of the weight rows of this wave's i-th chunks: gated, every second 16 rows of the tile are
+  // up rows.
+  const auto rw = [&](int i) {
+    const bool up = E::kGated && (((i * TH + wave * 64) / (4 * KU)) & 16);
+    return make_rsrc(const_cast<uint16_t*>(w + (static_cast<size_t>(up ? n : 0) + n0) * k),
+                     min(n - n0, static_cast<uint32_t>(TC)) * k * 2);
+  };
   struct XRegs {
     f32x4 a[XC], b[XC];
   };
@@ -156,7 +167,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
 #pragma unroll
     for (int i = 0; i < WC; ++i) {
       const int o = tail && kb + wk[i] >= k ? kOutside : wo[i];
-      r.v[i] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(rw, o, kb * 2, 0));
+      r.v[i] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(rw(i), o, kb * 2, 0));
     }
   };
   float big = 0.0f;  // the largest |x| this thread has cut up
@@ -319,14 +330,15 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
         for (int b = 0; b < MT; ++b)
           sum[a][b] = sum[a][b] + __builtin_bit_cast(f32x4, ld4_coherent(rp, (base + q * kTile + (a * MT + b) * 64) * 16));
   }
-  const bool wide = wide_out(NoEpilogue{}, out, n);
+  const bool wide = wide_out(epi, out, n);
+  constexpr int W = E::kGated ? 2 : 1;
 #pragma unroll
   for (int b = 0; b < MT; ++b) {
     const uint32_t row = t0 + (wm * MT + b) * 16 + c;
     if (row >= t) continue;
 #pragma unroll
-    for (int a = 0; a < NT; ++a)
-      store_out4(NoEpilogue{}, out, row, n0 + (wn * NT + a) * 16 + 4 * g, n, wide, sum[a][b], sum[a][b]);
+    for (int a = 0; a < NT; a += W)
+      store_out4(epi, out, row, n0 + (wn * NT + a) / W * 16 + 4 * g, n, wide, sum[a][b], sum[a + W - 1][b]);
   }
 }
 
@@ -338,22 +350,23 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
 // every tile (twice w's bytes from L2 and ~60 vector instructions per KiB of w). The waves'
 // partial tiles meet in LDS, nb tiles at a time in one of two halves (so one barrier per
 // nb tiles), and are added in wave order: the bits of matmul_bf16_rows without a split
-// of k. Grid: at most one workgroup per CU; workgroup i takes batches i, i + grid, ...
+// of k. With a gated epilogue the tiles alternate between 16 gate rows and the 16 up rows that
+// belong to them; nb is even, so both meet in one batch. Grid: at most one workgroup per CU; workgroup i takes batches i, i + grid, ...
 // Measured (k 2048): 16 x 151936 222 -> 120 us (5.2 TB/s of w), 1 x 151936 128 -> 104,
 // 16 x 16384 27 -> 15, 16 x 8192 14.9 -> 10.5; a third tile in flight or nontemporal
 // loads are 2-30% slower.
 static constexpr int kStreamWaves = 8;
 static constexpr int kStreamMaxBatch = 8;  // one tile per wave to add up
 
-template <int S>
+template <int S, class E>
 __global__ __launch_bounds__(64 * kStreamWaves, 2) void matmul_bf16_stream(
-    const float* __restrict__ x, const uint16_t* __restrict__ w, float* __restrict__ out, uint32_t t,
-    uint32_t n, uint32_t nb) {
-  constexpr uint32_t k = S * 32 * kStreamWaves;
+    const float* __restrict__ x, const uint16_t* __restrict__ w, float* out, uint32_t t, uint32_t n,
+    uint32_t nb, E epi) {
+  constexpr uint32_t k = S * 32 * kStreamWaves, W = E::kGated ? 2 : 1;
   __shared__ f32x4 part[2][kStreamMaxBatch][kStreamWaves][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 15, g = lane >> 4;
-  const uint32_t tiles = (n + 15) / 16, batches = (tiles + nb - 1) / nb;
+  const uint32_t tiles = (n + 15) / 16 * W, batches = (tiles + nb - 1) / nb;
   bf16x8 xf[S][3];
   {
     // Rows past t repeat the last one; their outputs are not stored.
@@ -378,14 +391,16 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void matmul_bf16_stream(
   }
   const int voff = (c * static_cast<int>(k) + wave * S * 32 + 8 * g) * 2;
   const auto load = [&](u16x8 (&r)[S], uint32_t tile) {  // past the end: the last tile again, unused
-    const uint32_t n0 = min(tile, tiles - 1) * 16;
+    tile = min(tile, tiles - 1);
+    const uint32_t n0 = tile / W * 16;
+    const size_t first = (E::kGated && (tile & 1) ? static_cast<size_t>(n) : 0) + n0;
     const __amdgpu_buffer_rsrc_t rw =
-        make_rsrc(const_cast<uint16_t*>(w + static_cast<size_t>(n0) * k), min(n - n0, 16u) * k * 2);
+        make_rsrc(const_cast<uint16_t*>(w + first * k), min(n - n0, 16u) * k * 2);
 #pragma unroll
     for (int u = 0; u < S; ++u)
       r[u] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(rw, voff + u * 64, 0, 0));
   };
-  const bool wide = wide_out(NoEpilogue{}, out, n);
+  const bool wide = wide_out(epi, out, n);
   u16x8 wv[2][S];
   uint32_t b = blockIdx.x, j = 0, half = 0;  // this tile: the j-th of batch b
   uint32_t lb = b, lj = 0;                   // the next one to load
@@ -411,12 +426,16 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void matmul_bf16_stream(
       part[half][j][wave][lane] = acc;
       if (++j < nb) continue;
       lds_barrier();  // the next tile's loads stay in flight
-      const uint32_t tile = b * nb + wave;
-      if (static_cast<uint32_t>(wave) < nb && tile < tiles) {
-        f32x4 s = part[half][wave][0][lane];
+      const uint32_t tile = b * nb + wave * W;
+      if (wave * W < nb && tile < tiles) {
+        f32x4 s[W];
 #pragma unroll
-        for (int q = 1; q < kStreamWaves; ++q) s = s + part[half][wave][q][lane];
-        if (static_cast<uint32_t>(c) < t) store_out4(NoEpilogue{}, out, c, tile * 16 + 4 * g, n, wide, s, s);
+        for (uint32_t i = 0; i < W; ++i) {
+          s[i] = part[half][wave * W + i][0][lane];
+#pragma unroll
+          for (int q = 1; q < kStreamWaves; ++q) s[i] = s[i] + part[half][wave * W + i][q][lane];
+        }
+        if (static_cast<uint32_t>(c) < t) store_out4(epi, out, c, tile / W * 16 + 4 * g, n, wide, s[0], s[W - 1]);
       }
       half ^= 1;
       j = 0;

@@ -1559,13 +1559,14 @@ int matmul_rows(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32
 // Tiles per batch: the count that leaves the busiest workgroup the fewest tiles, the
 // larger of equals (fewer barriers): n 151936 118 us with 2, 122 with 4, 128 with 8; n
 // 16384 15.0 with 4, 16.7 with 2.
-bool matmul_stream(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n) {
+template <class E>
+bool matmul_stream(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
+                   const E& epi) {
   if (k % 256) return false;
-  c->mm_kernel = 2;
-  c->mm_k_parts = 1;
-  const uint32_t tiles = (n + 15) / 16, cus = static_cast<uint32_t>(c->cus);
-  uint32_t nb = 1, least = UINT32_MAX;
-  for (uint32_t b = 1; b <= static_cast<uint32_t>(yx::kStreamMaxBatch); b *= 2) {
+  constexpr uint32_t W = E::kGated ? 2 : 1;
+  const uint32_t tiles = (n + 15) / 16 * W, cus = static_cast<uint32_t>(c->cus);
+  uint32_t nb = W, least = UINT32_MAX;
+  for (uint32_t b = W; b <= static_cast<uint32_t>(yx::kStreamMaxBatch); b *= 2) {
     const uint32_t batches = (tiles + b - 1) / b, busiest = (batches + cus - 1) / cus * b;
     if (busiest <= least) {
       least = busiest;
@@ -1574,14 +1575,16 @@ bool matmul_stream(yx_ctx* c, const float* x, const uint16_t* w, float* out, uin
   }
   const dim3 grid(std::min(cus, (tiles + nb - 1) / nb));
   const auto go = [&](auto* kern) {
-    hipLaunchKernelGGL(kern, grid, dim3(64 * yx::kStreamWaves), 0, c->stream, x, w, out, t, n, nb);
+    c->mm_kernel = 2;
+    c->mm_k_parts = 1;
+    hipLaunchKernelGGL(kern, grid, dim3(64 * yx::kStreamWaves), 0, c->stream, x, w, out, t, n, nb, epi);
     return true;
   };
   switch (k / 256) {
-    case 4: return go(yx::matmul_bf16_stream<4>);
-    case 6: return go(yx::matmul_bf16_stream<6>);
-    case 8: return go(yx::matmul_bf16_stream<8>);
-    case 10: return go(yx::matmul_bf16_stream<10>);
+    case 4: return go(yx::matmul_bf16_stream<4, E>);
+    case 6: return go(yx::matmul_bf16_stream<6, E>);
+    case 8: return go(yx::matmul_bf16_stream<8, E>);
+    case 10: return go(yx::matmul_bf16_stream<10, E>);
     default: return false;
   }
 }
@@ -1679,35 +1682,52 @@ bool overlap(const void* a, size_t an, const void* b, size_t bn) {
   return a && b && x < y + bn && y < x + an;
 }
 
-// yx_linear_bf16_dev, its arguments checked.
 template <class E>
-int linear_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
-                const E& epi) {
-  const size_t steps = (static_cast<size_t>(k) + 31) / 32;
-  const size_t tiles16 = static_cast<size_t>((n + 15) / 16) * ((t + 15) / 16);
-  return matmul_rows(c, x, w, out, t, k, n, matmul_rows_split(c, tiles16, steps), epi);
-}
-
 int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
-                 const MatmulSplit& split) {
+                 const MatmulSplit& split, const E& epi) {
   const MatmulShape& sh = kMatmulShapes[split.shape];
   c->mm_kernel = 3 + static_cast<uint64_t>(split.shape);
   c->mm_k_parts = split.ks;
-  const size_t tiles = static_cast<size_t>((t + sh.tm - 1) / sh.tm) * ((n + sh.tn - 1) / sh.tn);
+  const size_t cols = E::kGated ? sh.tn / 2 : sh.tn;
+  const size_t tiles = ((t + sh.tm - 1) / sh.tm) * ((n + cols - 1) / cols);
   if (tiles > 0x7fffffff) return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
   const auto go = [&](auto* kern) {
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles), split.ks), dim3(yx::kMatmulThreads), 0, c->stream, x,
                        w, out, t, k, n, static_cast<yx::f32x4*>(c->mt_part.p),
-                       static_cast<uint32_t>(c->mt_part.cap), static_cast<uint32_t*>(c->mt_counters.p));
+                       static_cast<uint32_t>(c->mt_part.cap), static_cast<uint32_t*>(c->mt_counters.p), epi);
   };
+  using D = std::conditional_t<E::kGated, yx::MatmulTileDGated, yx::MatmulTileD>;
   switch (split.shape) {
-    case 0: go(yx::matmul_bf16_tiles<yx::MatmulTileA>); break;
-    case 1: go(yx::matmul_bf16_tiles<yx::MatmulTileB>); break;
-    case 2: go(yx::matmul_bf16_tiles<yx::MatmulTileC>); break;
-    default: go(yx::matmul_bf16_tiles<yx::MatmulTileD>); break;
+    case 0: go(yx::matmul_bf16_tiles<yx::MatmulTileA, E>); break;
+    case 1: go(yx::matmul_bf16_tiles<yx::MatmulTileB, E>); break;
+    case 2: go(yx::matmul_bf16_tiles<yx::MatmulTileC, E>); break;
+    default: go(yx::matmul_bf16_tiles<D, E>); break;
   }
   YX_HIP(hipGetLastError());
   return YX_OK;
+}
+
+// A product whose arguments are checked: the kernel for its sizes. What decides are the weight's
+// rows (two per output column where the epilogue is gated).
+template <class E>
+int matmul_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
+                const E& epi) {
+  constexpr uint32_t W = E::kGated ? 2 : 1;
+  const size_t steps = (static_cast<size_t>(k) + 31) / 32;
+  const size_t tiles16 = static_cast<size_t>((n + 15) / 16) * ((t + 15) / 16);
+  const size_t slots = static_cast<size_t>(c->cus);
+  if (c->matmul_k_split == 0 && W * tiles16 >= 2 * slots) {
+    if (t <= 16) {
+      if (matmul_stream(c, x, w, out, t, k, n, epi)) {
+        YX_HIP(hipGetLastError());
+        return YX_OK;
+      }
+    } else if (k <= (size_t{1} << 20)) {  // a tile's rows within a buffer resource
+      const MatmulSplit split = matmul_tile_split(c, t, k, W * n);
+      if (!matmul_rows_faster(c, t, k, W * n, split.us)) return matmul_tiled(c, x, w, out, t, k, n, split, epi);
+    }
+  }
+  return matmul_rows(c, x, w, out, t, k, n, matmul_rows_split(c, tiles16, steps), epi);
 }
 
 }  // namespace
@@ -2414,22 +2434,8 @@ int yx_matmul_bf16_dev(yx_ctx* c, const float* x, const uint16_t* w, float* out,
   if (!x || !w || !out) return fail(YX_ERR_INVALID, "null x, w or out");
   int rc = matmul_check(x, w, t, k, n);
   if (rc || (rc = c->set_device())) return rc;
-  const size_t steps = (k + 31) / 32;
-  const auto T = static_cast<uint32_t>(t), K = static_cast<uint32_t>(k), N = static_cast<uint32_t>(n);
-  const size_t tiles16 = ((n + 15) / 16) * ((t + 15) / 16);
-  const size_t slots = static_cast<size_t>(c->cus);
-  if (c->matmul_k_split == 0 && tiles16 >= 2 * slots) {
-    if (t <= 16) {
-      if (matmul_stream(c, x, w, out, T, K, N)) {
-        YX_HIP(hipGetLastError());
-        return YX_OK;
-      }
-    } else if (k <= (size_t{1} << 20)) {  // a tile's rows within a buffer resource
-      const MatmulSplit split = matmul_tile_split(c, T, K, N);
-      if (!matmul_rows_faster(c, T, K, N, split.us)) return matmul_tiled(c, x, w, out, T, K, N, split);
-    }
-  }
-  return matmul_rows(c, x, w, out, T, K, N, matmul_rows_split(c, tiles16, steps), yx::NoEpilogue{});
+  return matmul_impl(c, x, w, out, static_cast<uint32_t>(t), static_cast<uint32_t>(k), static_cast<uint32_t>(n),
+                     yx::NoEpilogue{});
 }
 
 int yx_linear_bf16_dev(yx_ctx* c, const float* x, const uint16_t* w, const float* bias, int act, int gated,
@@ -2451,8 +2457,8 @@ int yx_linear_bf16_dev(yx_ctx* c, const float* x, const uint16_t* w, const float
     return fail(YX_ERR_INVALID, "out overlaps an input (the residual may be out itself)");
   if ((rc = c->set_device())) return rc;
   const auto T = static_cast<uint32_t>(t), K = static_cast<uint32_t>(k), N = static_cast<uint32_t>(n);
-  if (gated) return linear_impl(c, x, w, out, T, K, N, yx::Epilogue<true>{bias, residual, static_cast<uint32_t>(act)});
-  return linear_impl(c, x, w, out, T, K, N, yx::Epilogue<false>{bias, residual, static_cast<uint32_t>(act)});
+  if (gated) return matmul_impl(c, x, w, out, T, K, N, yx::Epilogue<true>{bias, residual, static_cast<uint32_t>(act)});
+  return matmul_impl(c, x, w, out, T, K, N, yx::Epilogue<false>{bias, residual, static_cast<uint32_t>(act)});
 }
 
 int yx_add_norm_rows_dev(yx_ctx* c, const float* x, const float* post_w, float post_offset, const float* h,
