@@ -22,6 +22,7 @@
 #include "deal.hpp"
 #include "kv_kernels.hpp"
 #include "logprobs.hpp"
+#include "matmul_few.hpp"
 #include "qk_rope.hpp"
 #include "step_after.hpp"
 
@@ -357,6 +358,9 @@ struct yx_ctx {
   // its calls need no earlier one to be captured, and (unlike the buffers counted in
   // buffer_gens) leave captured graphs valid.
   DevBuf mt_part, mt_counters;
+  // Rows of logits read in slices: the slices' sums and keys and the rows' arrival counters,
+  // for kLogprobsParts slices in all, allocated with the context too.
+  DevBuf lp_keys, lp_parts, lp_counters;
   uint64_t mm_kernel = 0, mm_k_parts = 0;  // what the latest matmul ran (tests)
   // options
   long target_waves = 0;  // 0: one work item per CU
@@ -1658,6 +1662,14 @@ bool matmul_rows_faster(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n, double ti
   return rows_us < 1.05 * tiles_us - 1.5 + (n % 4 ? 0.9 : 0.0);
 }
 
+constexpr size_t kLogprobsParts = 4096;  // slices of a call that has rows in several
+int logprobs_scratch(yx_ctx* c) {
+  int rc;
+  if ((rc = c->lp_keys.ensure(kLogprobsParts * YX_MAX_TOP * 8, c->stream))) return rc;
+  if ((rc = c->lp_parts.ensure(kLogprobsParts * 16, c->stream))) return rc;
+  return c->lp_counters.ensure(kLogprobsParts / 2 * 4 * yx::kCounterStride, c->stream, true);
+}
+
 // Workgroups per output tile of matmul_bf16_rows along k: about two workgroups per CU in
 // all, each wave at least one pass of its loop (kMmSteps steps of 32).
 size_t matmul_rows_split(const yx_ctx* c, size_t tiles, size_t steps) {
@@ -1707,6 +1719,32 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
   return YX_OK;
 }
 
+// Few rows with an epilogue. The workgroups of a column group share k so that all of them
+// make up at most one per CU (two run no faster together, and their hand-off's parts are twice as
+// many: 16 x 2048 x 8192 gated in 1, 2, 4 and 8 parts 39, 23.6, 17.8 and 23.5 us; 16 x 8192 x
+// 2048 in 8, 16 and 32 parts 13.8, 13.1 and 18.0).
+template <class E>
+int matmul_few(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
+               const E& epi) {
+  constexpr int N = E::kGated ? 2 : 1;
+  constexpr uint32_t cols = 128;
+  const uint32_t groups = (n + cols - 1) / cols;
+  const auto go = [&](auto* kern, uint32_t kc) {
+    const uint32_t ks = std::max(1u, std::min(static_cast<uint32_t>(c->cus) / groups, (k + kc - 1) / kc));
+    c->mm_kernel = 7;
+    c->mm_k_parts = ks;
+    hipLaunchKernelGGL(kern, dim3(groups, ks), dim3(yx::kFewThreads), 0, c->stream, x, w, out, t, k, n,
+                       static_cast<yx::f32x4*>(c->mt_part.p), static_cast<uint32_t>(c->mt_part.cap),
+                       static_cast<uint32_t*>(c->mt_counters.p), epi);
+  };
+  if (t <= 16)
+    go(yx::matmul_bf16_few<1, N, E>, yx::few_chunk<1>());
+  else
+    go(yx::matmul_bf16_few<2, N, E>, yx::few_chunk<2>());
+  YX_HIP(hipGetLastError());
+  return YX_OK;
+}
+
 // A product whose arguments are checked: the kernel for its sizes. What decides are the weight's
 // rows (two per output column where the epilogue is gated).
 template <class E>
@@ -1716,6 +1754,8 @@ int matmul_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32
   const size_t steps = (static_cast<size_t>(k) + 31) / 32;
   const size_t tiles16 = static_cast<size_t>((n + 15) / 16) * ((t + 15) / 16);
   const size_t slots = static_cast<size_t>(c->cus);
+  if constexpr (E::kFused)
+    if (c->matmul_k_split == 0 && t <= 32 && k <= (size_t{1} << 20)) return matmul_few(c, x, w, out, t, k, n, epi);
   if (c->matmul_k_split == 0 && W * tiles16 >= 2 * slots) {
     if (t <= 16) {
       if (matmul_stream(c, x, w, out, t, k, n, epi)) {
@@ -1770,6 +1810,7 @@ int yx_ctx_create(int device, yx_ctx** out) {
   }
   int rc = scratch_init(device, c->stream);
   if (!rc) rc = matmul_tiles_scratch(c);
+  if (!rc) rc = logprobs_scratch(c);
   if (rc) {
     yx_ctx_destroy(c);
     return rc;
@@ -1795,7 +1836,7 @@ int yx_ctx_destroy(yx_ctx* c) {
   for (DevBuf& b : c->spare) b.release();
   c->spare.clear();
   for (DevBuf* b : {&c->d_meta, &c->d_pages, &c->am_keys, &c->am_counters, &c->mm_part, &c->mm_counters,
-                    &c->mt_part, &c->mt_counters,
+                    &c->mt_part, &c->mt_counters, &c->lp_keys, &c->lp_parts, &c->lp_counters,
                     &c->part_o, &c->part_ml, &c->counters,
                     &c->io_a, &c->io_b, &c->io_c, &c->io_q})
     b->release();
@@ -2457,6 +2498,8 @@ int yx_linear_bf16_dev(yx_ctx* c, const float* x, const uint16_t* w, const float
     return fail(YX_ERR_INVALID, "out overlaps an input (the residual may be out itself)");
   if ((rc = c->set_device())) return rc;
   const auto T = static_cast<uint32_t>(t), K = static_cast<uint32_t>(k), N = static_cast<uint32_t>(n);
+  if (!gated && act == YX_ACT_NONE && !bias && !residual)  // yx_matmul_bf16_dev's call, and its bits
+    return matmul_impl(c, x, w, out, T, K, N, yx::NoEpilogue{});
   if (gated) return matmul_impl(c, x, w, out, T, K, N, yx::Epilogue<true>{bias, residual, static_cast<uint32_t>(act)});
   return matmul_impl(c, x, w, out, T, K, N, yx::Epilogue<false>{bias, residual, static_cast<uint32_t>(act)});
 }
@@ -2548,9 +2591,20 @@ int yx_logprobs_rows_dev(yx_ctx* c, const float* logits, size_t rows, size_t col
     return fail(YX_ERR_INVALID, "logprobs buffers must be 4-byte aligned");
   int rc = c->set_device();
   if (rc) return rc;
-  hipLaunchKernelGGL(yx::logprobs_rows, dim3(static_cast<unsigned>(rows)), dim3(yx::kLpThreads), 0, c->stream, logits,
-                     static_cast<uint32_t>(cols), ld, tokens, static_cast<uint32_t>(given),
-                     static_cast<uint32_t>(top), yx::LogprobsOut{logprob, entropy, top_ids, top_logprobs});
+  size_t want = 1024, least = 256;
+  if (getenv("YX_LP")) sscanf(getenv("YX_LP"), "%zu,%zu", &want, &least);
+  const size_t quads = (cols + 3) / 4;
+  size_t nsl = std::min({(want + rows - 1) / rows, (quads + least - 1) / least, static_cast<size_t>(yx::kLpMaxSlices),
+                         kLogprobsParts / rows});
+  nsl = std::max<size_t>(nsl, 1);
+  const size_t per = (quads + nsl - 1) / nsl;
+  nsl = (quads + per - 1) / per;
+  hipLaunchKernelGGL(yx::logprobs_rows, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(nsl)),
+                     dim3(yx::kLpThreads), 0, c->stream, logits, static_cast<uint32_t>(cols), ld, tokens,
+                     static_cast<uint32_t>(given), static_cast<uint32_t>(top),
+                     yx::LogprobsOut{logprob, entropy, top_ids, top_logprobs}, static_cast<uint32_t>(per),
+                     static_cast<unsigned long long*>(c->lp_keys.p), static_cast<float*>(c->lp_parts.p),
+                     static_cast<uint32_t*>(c->lp_counters.p));
   YX_HIP(hipGetLastError());
   return YX_OK;
 }
