@@ -1,11 +1,16 @@
 // The seam between two blocks of a model: residual addition and RMSNorms of rows, on MI355X:
 //   u = norm(x; post_w, post_offset) or x,  h' = h + u or u,  out = norm(h'; w, offset),
 //   norm(v; w, o)_i = v_i / sqrt(mean v^2 + eps) * (o + w_i)
-// (all f32). h_out and out may each be x or h itself: a thread writes only columns that it
-// alone reads.
+// (all f32; sums of squares f32 in a fixed order). Bound by reading x and h and writing h' and out
+// once: rows of up to 8192 columns stay in a workgroup's registers between the sums and the
+// stores; with few rows by the chain load, sum, sum, store, so the weights' loads go out with the
+// rows'. h_out and out may each be x or h itself: a thread writes only columns that it alone
+// reads, after it has read them.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include "epilogue.hpp"
 
 namespace yx {
 
@@ -31,8 +36,69 @@ __device__ __forceinline__ float norm_sum(float v, float* ws) {
   return (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
-// One workgroup per row.
+// Columns 4q .. 4q + 3 of a row whose length and address may be any.
+__device__ __forceinline__ f32x4 norm_load(const float* p, uint32_t q, uint32_t cols) {
+  if (4 * q + 4 <= cols) return reinterpret_cast<const f32x4_any*>(p)[q];
+  f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (4 * q + j < cols) v[j] = p[4 * q + j];
+  return v;
+}
+__device__ __forceinline__ void norm_store(float* p, uint32_t q, uint32_t cols, const f32x4& v) {
+  if (4 * q + 4 <= cols) {
+    reinterpret_cast<f32x4_any*>(p)[q] = v;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (4 * q + j < cols) p[4 * q + j] = v[j];
+}
+
+// One workgroup per row, V pieces of four columns per thread: at most 1024 V columns.
+template <int V>
 __global__ __launch_bounds__(kNormThreads) void add_norm_rows(AddNorm a, uint32_t cols) {
+  __shared__ float ws[2][kNormThreads / 64];
+  const size_t base = static_cast<size_t>(blockIdx.x) * cols;
+  f32x4 x[V], h[V], pw[V], w[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t q = i * kNormThreads + threadIdx.x;
+    x[i] = h[i] = pw[i] = w[i] = f32x4{0, 0, 0, 0};
+    if (4 * q >= cols) continue;
+    x[i] = norm_load(a.x + base, q, cols);
+    if (a.h) h[i] = norm_load(a.h + base, q, cols);
+    if (a.post_w) pw[i] = norm_load(a.post_w, q, cols);
+    if (a.w) w[i] = norm_load(a.w, q, cols);
+  }
+  const auto rms = [&](const f32x4 (&v)[V], float* s) {  // 1 / sqrt(mean v^2 + eps)
+    f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum = sum + v[i] * v[i];
+    return 1.0f / sqrtf(norm_sum((sum.x + sum.y) + (sum.z + sum.w), s) / static_cast<float>(cols) + a.eps);
+  };
+  if (a.post_w) {
+    const float r = rms(x, ws[0]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = x[i] * r * (a.post_offset + pw[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t q = i * kNormThreads + threadIdx.x;
+    if (a.h) x[i] = h[i] + x[i];
+    if (a.h_out && 4 * q < cols) norm_store(a.h_out + base, q, cols, x[i]);
+  }
+  if (!a.w) return;
+  const float r = rms(x, ws[1]);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t q = i * kNormThreads + threadIdx.x;
+    if (4 * q < cols) norm_store(a.out + base, q, cols, x[i] * r * (a.offset + w[i]));
+  }
+}
+
+// The same for rows of any length, which are read again after each sum.
+__global__ __launch_bounds__(kNormThreads) void add_norm_long_rows(AddNorm a, uint32_t cols) {
   __shared__ float ws[kNormThreads / 64];
   const size_t base = static_cast<size_t>(blockIdx.x) * cols;
   float ru = 1.0f, sum = 0.0f;

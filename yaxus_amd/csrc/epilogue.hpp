@@ -15,6 +15,8 @@
 namespace yx {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+// Four floats at any float's address: the hardware takes 16-byte accesses there.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // Four values at once (one branch on act, which is uniform). NaN stays NaN in every one of
 // them; -inf gives NaN where the formula is -inf * 0 (all but none and relu).

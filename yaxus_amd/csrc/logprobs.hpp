@@ -49,9 +49,6 @@ __device__ __forceinline__ float ord_value(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
 }
 
-// Rows are only 4-byte aligned (any stride); the hardware takes 16-byte loads there.
-typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-
 // Sums of e^(x - m) and (x - m) log2(e) e^(x - m) over some logits and their maximum m.
 struct LpSums {
   float m, s, u;

@@ -359,7 +359,7 @@ struct yx_ctx {
   // buffer_gens) leave captured graphs valid.
   DevBuf mt_part, mt_counters;
   // Rows of logits read in slices: the slices' sums and keys and the rows' arrival counters,
-  // for kLogprobsParts slices in all, allocated with the context too.
+  // for logprobs_slots slices in all, allocated with the context too.
   DevBuf lp_keys, lp_parts, lp_counters;
   uint64_t mm_kernel = 0, mm_k_parts = 0;  // what the latest matmul ran (tests)
   // options
@@ -1662,12 +1662,25 @@ bool matmul_rows_faster(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n, double ti
   return rows_us < 1.05 * tiles_us - 1.5 + (n % 4 ? 0.9 : 0.0);
 }
 
-constexpr size_t kLogprobsParts = 4096;  // slices of a call that has rows in several
+// Workgroups of logprobs_rows that run at once (four per CU).
+size_t logprobs_slots(const yx_ctx* c) { return 4 * static_cast<size_t>(c->cus); }
+
 int logprobs_scratch(yx_ctx* c) {
+  const size_t n = logprobs_slots(c);
   int rc;
-  if ((rc = c->lp_keys.ensure(kLogprobsParts * YX_MAX_TOP * 8, c->stream))) return rc;
-  if ((rc = c->lp_parts.ensure(kLogprobsParts * 16, c->stream))) return rc;
-  return c->lp_counters.ensure(kLogprobsParts / 2 * 4 * yx::kCounterStride, c->stream, true);
+  if ((rc = c->lp_keys.ensure(n * YX_MAX_TOP * 8, c->stream))) return rc;
+  if ((rc = c->lp_parts.ensure(n * 16, c->stream))) return rc;
+  return c->lp_counters.ensure(n / 2 * 4 * yx::kCounterStride, c->stream, true);
+}
+
+// Slices of a row (quads: its 16-byte pieces): as many as run at once over all rows, each at
+// least one round of a workgroup's loads. More rounds of workgroups, or fuller ones, are no
+// faster: rows of 151936, 1 / 2 / 4 / 8 slices: 100 rows 47 / 33 / 23 / 21 us, 300 rows 54 / 41 /
+// 46 / 44, 600 rows 66 / 76 / 71 / 71.
+size_t logprobs_slices(const yx_ctx* c, size_t rows, size_t quads) {
+  const size_t least = yx::kLpThreads;
+  return std::max<size_t>(1, std::min({logprobs_slots(c) / rows, (quads + least - 1) / least,
+                                       static_cast<size_t>(yx::kLpMaxSlices)}));
 }
 
 // Workgroups per output tile of matmul_bf16_rows along k: about two workgroups per CU in
@@ -2528,8 +2541,16 @@ int yx_add_norm_rows_dev(yx_ctx* c, const float* x, const float* post_w, float p
   int rc = c->set_device();
   if (rc) return rc;
   const yx::AddNorm a{x, post_w, h, h_out, w, out, post_offset, offset, eps};
-  hipLaunchKernelGGL(yx::add_norm_rows, dim3(static_cast<unsigned>(rows)), dim3(yx::kNormThreads), 0, c->stream, a,
-                     static_cast<uint32_t>(cols));
+  const auto go = [&](auto* kern) {
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(rows)), dim3(yx::kNormThreads), 0, c->stream, a,
+                       static_cast<uint32_t>(cols));
+  };
+  const size_t per = (cols + 4 * yx::kNormThreads - 1) / (4 * yx::kNormThreads);  // pieces of a thread
+  if (per <= 1) go(yx::add_norm_rows<1>);
+  else if (per <= 2) go(yx::add_norm_rows<2>);
+  else if (per <= 4) go(yx::add_norm_rows<4>);
+  else if (per <= 8) go(yx::add_norm_rows<8>);
+  else go(yx::add_norm_long_rows);
   YX_HIP(hipGetLastError());
   return YX_OK;
 }
@@ -2591,14 +2612,10 @@ int yx_logprobs_rows_dev(yx_ctx* c, const float* logits, size_t rows, size_t col
     return fail(YX_ERR_INVALID, "logprobs buffers must be 4-byte aligned");
   int rc = c->set_device();
   if (rc) return rc;
-  size_t want = 1024, least = 256;
-  if (getenv("YX_LP")) sscanf(getenv("YX_LP"), "%zu,%zu", &want, &least);
   const size_t quads = (cols + 3) / 4;
-  size_t nsl = std::min({(want + rows - 1) / rows, (quads + least - 1) / least, static_cast<size_t>(yx::kLpMaxSlices),
-                         kLogprobsParts / rows});
-  nsl = std::max<size_t>(nsl, 1);
+  size_t nsl = logprobs_slices(c, rows, quads);
   const size_t per = (quads + nsl - 1) / nsl;
-  nsl = (quads + per - 1) / per;
+  nsl = (quads + per - 1) / per;  // none of them empty
   hipLaunchKernelGGL(yx::logprobs_rows, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(nsl)),
                      dim3(yx::kLpThreads), 0, c->stream, logits, static_cast<uint32_t>(cols), ld, tokens,
                      static_cast<uint32_t>(given), static_cast<uint32_t>(top),
