@@ -115,8 +115,8 @@ CASES = [
     (1, 8, 1), (5, 72, 40), (16, 8, 16), (17, 264, 33), (3, 4096, 1000), (1, 2048, 2048), (40, 2048, 250),
     # the streaming kernel (k a multiple of 256), whole and ragged batches of tiles
     (16, 2048, 8192), (1, 1024, 8200), (7, 1536, 16390), (16, 2560, 8207),
-    # at most 16 rows, k it is not built for
-    (16, 4096, 8192), (9, 1000, 9000), (16, 8192, 2048),
+    # few rows against much weight, in two and more chunks of k, the last of them partial
+    (16, 4096, 8192), (9, 1000, 9000), (16, 8192, 2048), (32, 2048, 4100), (17, 1048, 12000), (2, 776, 16001),
     # LDS tiles of each shape, k ending inside a stage, n no multiple of 4
     (80, 2048, 2752), (64, 1536, 6001), (333, 1536, 1501), (1000, 1000, 1030), (300, 2048, 5512), (2048, 520, 2056),
 ]

@@ -61,15 +61,15 @@ struct Epilogue {
 };
 
 // A lane's outputs at columns col .. col + 3 of one row; y holds the sums (of the gate rows),
-// up those of the up rows (gated only). wide: n a multiple of 4, every pointer 16-byte
-// aligned.
+// up those of the up rows (gated only). wide (without an epilogue): wide_out.
 template <class E>
 __device__ __forceinline__ void store_out4(const E& e, float* out, uint32_t row, uint32_t col, uint32_t n,
                                            bool wide, const f32x4& y, const f32x4& up) {
+  if (col >= n) return;
   float* o = out + static_cast<size_t>(row) * n + col;
   if constexpr (!E::kFused) {
     if (wide) {
-      if (col < n) *reinterpret_cast<f32x4*>(o) = y;
+      *reinterpret_cast<f32x4*>(o) = y;
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -78,16 +78,16 @@ __device__ __forceinline__ void store_out4(const E& e, float* out, uint32_t row,
   } else {
     f32x4 v = y, u = up, a = {0, 0, 0, 0};
     const float* r = e.residual + static_cast<size_t>(row) * n + col;
-    if (wide) {
-      if (col >= n) return;
-      if (e.residual) a = *reinterpret_cast<const f32x4*>(r);
+    const bool whole = col + 4 <= n;  // 16-byte accesses, at any float's address
+    if (whole) {
+      if (e.residual) a = *reinterpret_cast<const f32x4_any*>(r);
       if (e.bias) {
-        v = v + *reinterpret_cast<const f32x4*>(e.bias + col);
-        if (E::kGated) u = u + *reinterpret_cast<const f32x4*>(e.bias + n + col);
+        v = v + *reinterpret_cast<const f32x4_any*>(e.bias + col);
+        if (E::kGated) u = u + *reinterpret_cast<const f32x4_any*>(e.bias + static_cast<size_t>(n) + col);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 3; ++i) {
         if (col + i >= n) continue;
         if (e.residual) a[i] = r[i];
         if (e.bias) {
@@ -99,22 +99,19 @@ __device__ __forceinline__ void store_out4(const E& e, float* out, uint32_t row,
     v = activate(v, e.act);
     if (E::kGated) v = v * u;
     if (e.residual) v = v + a;
-    if (wide) {
-      *reinterpret_cast<f32x4*>(o) = v;
+    if (whole) {
+      *reinterpret_cast<f32x4_any*>(o) = v;
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 3; ++i)
         if (col + i < n) o[i] = v[i];
     }
   }
 }
 
-// Whether store_out4 may use 16-byte accesses.
-template <class E>
-__device__ __forceinline__ bool wide_out(const E& e, const float* out, uint32_t n) {
-  uintptr_t p = reinterpret_cast<uintptr_t>(out);
-  if constexpr (E::kFused) p |= reinterpret_cast<uintptr_t>(e.bias) | reinterpret_cast<uintptr_t>(e.residual);
-  return (n & 3) == 0 && (p & 15) == 0;
+// Whether store_out4 may use 16-byte accesses without an epilogue.
+__device__ __forceinline__ bool wide_out(const float* out, uint32_t n) {
+  return (n & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 }
 
 }  // namespace yx

@@ -214,8 +214,10 @@ __global__ __launch_bounds__(kLpThreads, 4) void logprobs_rows(const float* __re
       floor = max(1ull, static_cast<unsigned long long>(lp_reach(o, top)) << 32);
     }
     uint32_t* count = &sh.count[turn];
-    const uint32_t fo = static_cast<uint32_t>(floor >> 32);  // below -inf's: any number
-    const float reach = fo > 0x007fffffu ? ord_value(fo) : -INFINITY;
+    // (-3.4e38: any number. -inf would let in every masked logit, 32 turns of the loop below for
+    // each thread of a masked row.)
+    const uint32_t fo = static_cast<uint32_t>(floor >> 32);
+    const float reach = fo > 0x00800000u ? ord_value(fo) : -3.402823466e38f;
     if (m >= reach) {
       uint32_t hits = 0;  // bit 4 i + j: v[i][j]
 #pragma unroll

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
         for (int b = 0; b < MT; ++b)
           sum[a][b] = sum[a][b] + __builtin_bit_cast(f32x4, ld4_coherent(rp, (base + q * kTile + (a * MT + b) * 64) * 16));
   }
-  const bool wide = wide_out(epi, out, n);
+  const bool wide = wide_out(out, n);
   constexpr int W = E::kGated ? 2 : 1;
 #pragma unroll
   for (int b = 0; b < MT; ++b) {
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, 2) void matmul_bf16_stream(
     for (int u = 0; u < S; ++u)
       r[u] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(rw, voff + u * 64, 0, 0));
   };
-  const bool wide = wide_out(epi, out, n);
+  const bool wide = wide_out(out, n);
   u16x8 wv[2][S];
   uint32_t b = blockIdx.x, j = 0, half = 0;  // this tile: the j-th of batch b
   uint32_t lb = b, lj = 0;                   // the next one to load

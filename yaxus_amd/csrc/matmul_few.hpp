@@ -1,17 +1,23 @@
-// Products of few rows (up to 96) with an epilogue: bound by reading the weight once.
+// Products of at most 32 rows with an epilogue: bound by reading the weight once.
 // out[t][n] = x[t][:] . w[n][:] as in matmul_bf16.hpp (x in three bf16 parts, every product
 // exact, f32 sums), then the epilogue.
 //
-// A workgroup's 8 waves own NT tiles of 16 weight rows each (128 NT rows; gated: 16 gate and
-// their 16 up rows per wave) against all R tiles of 16 rows of x. x is cut up once per
-// workgroup, KC of k at a time, into LDS (two slots, one barrier per KC), in the order in which
-// lanes read it; the weight goes straight from memory to the registers of the wave that
-// multiplies it, a whole chunk of KC ahead (8 KiB per wave and weight tile at KC 256), so that
-// nothing waits for it but its own product. No sums meet between waves.
-// Layouts as in step_after.hpp (A: 16 weight rows, B: 16 rows of a part of x). A chunk's
+// A workgroup's 8 waves own NT tiles of 16 weight rows each (gated: 16 gate rows and their 16 up
+// rows) against all R tiles of 16 rows of x. x is cut up once per workgroup, KC of k at a time,
+// into LDS (two slots, one barrier per KC), in the order in which lanes read it; the weight goes
+// straight from memory to the registers of the wave that multiplies it, a whole chunk of KC
+// ahead, so that nothing waits for it but its own product. No sums meet between waves; a chunk's
 // products are added to the result in f32, so chains stay short.
+// Workgroups start at different chunks and go round: rows are 2 k bytes apart, and workgroups in
+// step would ask the same memory channels for their rows' same columns (k 8192, 262 MB 61 -> 52
+// us, 524 MB 126 -> 104; k 2048 28.4 -> 27.9).
+// Layouts as in step_after.hpp (A: 16 weight rows, B: 16 rows of a part of x).
 // With ks > 1 (grid y) the workgroups of a column group take consecutive chunks of k and hand
 // their tiles over as matmul_bf16_rows does.
+// Measured, 16 rows: k 2048, n 8192 gated (67 MB) 17.7 us, k 8192, n 2048 13.1 (33.5 MB), k 4096,
+// n 14336 gated 51 (4.6 TB/s), k 8192, n 16000 gated 104 (5.1 TB/s). Tried: a wave streaming
+// tiles past x in registers (16 rows of 2 KiB at a time, no LDS) 100 us for the last, but 18-29%
+// slower up to 34 MB, where each part of x is cut up for too few tiles.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -22,7 +28,6 @@
 namespace yx {
 
 static constexpr int kFewThreads = 512;
-static constexpr int kFewMaxRowTiles = 6;
 
 template <int R>
 constexpr int few_chunk() {
@@ -30,11 +35,12 @@ constexpr int few_chunk() {
 }
 
 template <int R, int NT, class E>
-__global__ __launch_bounds__(kFewThreads, R <= 3 ? 4 : 2) void matmul_bf16_few(
+__global__ __launch_bounds__(kFewThreads, 4) void matmul_bf16_few(
     const float* __restrict__ x, const uint16_t* __restrict__ w, float* out, uint32_t t, uint32_t k,
     uint32_t n, f32x4* __restrict__ part, uint32_t part_bytes, uint32_t* __restrict__ counters, E epi) {
   constexpr int KC = few_chunk<R>(), STEPS = KC / 32, TH = kFewThreads;
-  constexpr int XN = R * 16 * KC / 8, XC = (XN + TH - 1) / TH;  // x in pieces of 8 k
+  constexpr int XC = R * 16 * KC / 8 / TH;  // pieces of 8 k of x per thread
+  static_assert(XC * TH == R * 16 * KC / 8, "whole rounds of pieces");
   constexpr uint32_t COLS = E::kGated ? 128 : 128 * NT;
   constexpr int kOutside = 0x7ffffff0;  // beyond every resource: reads zeros
   static_assert(!E::kGated || NT == 2, "a gate and an up tile");
@@ -45,6 +51,8 @@ __global__ __launch_bounds__(kFewThreads, R <= 3 ? 4 : 2) void matmul_bf16_few(
   const uint32_t n0 = blockIdx.x * COLS, ks = gridDim.y, kp = blockIdx.y;
   const uint32_t chunks = (k + KC - 1) / KC, c0 = chunks * kp / ks, c1 = chunks * (kp + 1) / ks;
 
+  const uint32_t len = c1 - c0, rot = blockIdx.x % len;
+  const auto chunk = [&](uint32_t i) { return i < len ? c0 + (i + rot >= len ? i + rot - len : i + rot) : c1; };
   const uint32_t wbytes = min(n - n0, COLS) * k * 2;
   const __amdgpu_buffer_rsrc_t rw = make_rsrc(const_cast<uint16_t*>(w + static_cast<size_t>(n0) * k), wbytes);
   const __amdgpu_buffer_rsrc_t ru =
@@ -80,7 +88,7 @@ __global__ __launch_bounds__(kFewThreads, R <= 3 ? 4 : 2) void matmul_bf16_few(
     const uint32_t kb = ch * KC;
 #pragma unroll
     for (int i = 0; i < XC; ++i) {
-      const bool ok = (ch < c1) & (kb + xk[i] < k) & (i * TH + tid < XN);
+      const bool ok = (ch < c1) & (kb + xk[i] < k);
       const int o = ok ? xo[i] : kOutside;
       r.a[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, o, kb * 4, 0));
       r.b[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, o, kb * 4 + 16, 0));
@@ -90,7 +98,6 @@ __global__ __launch_bounds__(kFewThreads, R <= 3 ? 4 : 2) void matmul_bf16_few(
     u16x8* d = &xs[slot][0][0][0][0];
 #pragma unroll
     for (int i = 0; i < XC; ++i) {
-      if (XN % TH && i * TH + tid >= XN) break;
       const float v[8] = {r.a[i].x, r.a[i].y, r.a[i].z, r.a[i].w, r.b[i].x, r.b[i].y, r.b[i].z, r.b[i].w};
       u32x4 p[3];
 #pragma unroll
@@ -116,20 +123,21 @@ __global__ __launch_bounds__(kFewThreads, R <= 3 ? 4 : 2) void matmul_bf16_few(
   XRegs xr;
   {
     XRegs first;
-    load_x(first, c0);
-    load_x(xr, c0 + 1);
+    load_x(first, chunk(0));
+    load_x(xr, chunk(1));
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) load_w(s, c0);
+    for (int s = 0; s < STEPS; ++s) load_w(s, chunk(0));
     __builtin_amdgcn_sched_barrier(0);
     write_x(first, 0);
   }
   lds_barrier();
   int slot = 0;
-  for (uint32_t ch = c0; ch < c1; ++ch, slot ^= 1) {
+  for (uint32_t i = 0; i < len; ++i, slot ^= 1) {
+    const uint32_t next = chunk(i + 1);
     // The other slot was last read before the barrier that ended the previous chunk.
     write_x(xr, slot ^ 1);
-    load_x(xr, ch + 2);
+    load_x(xr, chunk(i + 2));
     __builtin_amdgcn_sched_barrier(0);
     f32x4 acc[NT][R];
     bf16x8 xf[2][R][3];
@@ -139,13 +147,10 @@ __global__ __launch_bounds__(kFewThreads, R <= 3 ? 4 : 2) void matmul_bf16_few(
 #pragma unroll
         for (int q = 0; q < 3; ++q) xf[s & 1][b][q] = __builtin_bit_cast(bf16x8, xs[slot][s][b][q][sw]);
     };
-    if (R <= 2) read_x(0);
+    read_x(0);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      if (R > 2)
-        read_x(s);
-      else if (s + 1 < STEPS)
-        read_x(s + 1);
+      if (s + 1 < STEPS) read_x(s + 1);
 #pragma unroll
       for (int b = 0; b < R; ++b)
 #pragma unroll
@@ -154,7 +159,7 @@ __global__ __launch_bounds__(kFewThreads, R <= 3 ? 4 : 2) void matmul_bf16_few(
           for (int a = 0; a < NT; ++a)
             acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[s][a]), xf[s & 1][b][q],
                                                                 s == 0 && q == 0 ? f32x4{0, 0, 0, 0} : acc[a][b], 0, 0, 0);
-      load_w(s, ch + 1);
+      load_w(s, next);
       __builtin_amdgcn_sched_barrier(0);  // this step's registers are filled again here, not at the chunk's end
     }
 #pragma unroll
@@ -194,7 +199,7 @@ __global__ __launch_bounds__(kFewThreads, R <= 3 ? 4 : 2) void matmul_bf16_few(
         for (int b = 0; b < R; ++b)
           sum[a][b] = sum[a][b] + __builtin_bit_cast(f32x4, ld4_coherent(rp, (base + q * kTile + (a * R + b) * 64) * 16));
   }
-  const bool wide = wide_out(epi, out, n);
+  const bool wide = wide_out(out, n);
 #pragma unroll
   for (int b = 0; b < R; ++b) {
     const uint32_t row = b * 16 + c;

@@ -1732,10 +1732,24 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
   return YX_OK;
 }
 
+// Whether matmul_bf16_few takes a product of at most 32 rows: much weight in many rows. On the
+// other side matmul_bf16_rows starts sooner and hands over less (us, 16 rows, that / few: k 2048,
+// n 2048 7.3 / 7.4, n 4096 11.1 / 8.0; k 8192, n 1024 11.8 / 14.0, n 2048 17.4 / 13.1; gated k
+// 2048, n 2048 8.7 / 10.2, n 4096 13.9 / 11.9; k 512, n 8192 7.9 / 8.4, n 16000 13.3 / 11.0), and
+// matmul_bf16_stream is faster where a row's k is short (gated, k 1024, n 8192 8.4 / 10.8; k 2048
+// 19.4 / 17.7). The number of rows does not decide up to 16: a row's bits stay the same.
+template <class E>
+bool matmul_few_faster(uint32_t t, uint32_t k, uint32_t n) {
+  constexpr uint32_t W = E::kGated ? 2 : 1;
+  if (t <= 16 && k < 2048 && k % 256 == 0 && k >= 1024) return false;
+  return t <= 32 && k <= (1u << 20) && n >= 2048 * W && static_cast<uint64_t>(W) * n * k * 2 >= 12000000ull * W;
+}
+
 // Few rows with an epilogue. The workgroups of a column group share k so that all of them
 // make up at most one per CU (two run no faster together, and their hand-off's parts are twice as
-// many: 16 x 2048 x 8192 gated in 1, 2, 4 and 8 parts 39, 23.6, 17.8 and 23.5 us; 16 x 8192 x
-// 2048 in 8, 16 and 32 parts 13.8, 13.1 and 18.0).
+// many: 16 x 2048 x 8192 gated in 1, 2, 4 and 8 parts 39, 23.6, 17.8 and 23.5 us), more than 8 of
+// them only with 512 k each (16 x 4096 x 2048 in 8 and 16 parts 9.3 and 10.0, 16 x 8192 x 2048
+// 13.8 and 13.1).
 template <class E>
 int matmul_few(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
                const E& epi) {
@@ -1743,7 +1757,7 @@ int matmul_few(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_
   constexpr uint32_t cols = 128;
   const uint32_t groups = (n + cols - 1) / cols;
   const auto go = [&](auto* kern, uint32_t kc) {
-    const uint32_t ks = std::max(1u, std::min(static_cast<uint32_t>(c->cus) / groups, (k + kc - 1) / kc));
+    const uint32_t ks = std::max(1u, std::min({static_cast<uint32_t>(c->cus) / groups, (k + kc - 1) / kc, std::max(8u, k / 512)}));
     c->mm_kernel = 7;
     c->mm_k_parts = ks;
     hipLaunchKernelGGL(kern, dim3(groups, ks), dim3(yx::kFewThreads), 0, c->stream, x, w, out, t, k, n,
@@ -1768,7 +1782,7 @@ int matmul_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32
   const size_t tiles16 = static_cast<size_t>((n + 15) / 16) * ((t + 15) / 16);
   const size_t slots = static_cast<size_t>(c->cus);
   if constexpr (E::kFused)
-    if (c->matmul_k_split == 0 && t <= 32 && k <= (size_t{1} << 20)) return matmul_few(c, x, w, out, t, k, n, epi);
+    if (c->matmul_k_split == 0 && matmul_few_faster<E>(t, k, n)) return matmul_few(c, x, w, out, t, k, n, epi);
   if (c->matmul_k_split == 0 && W * tiles16 >= 2 * slots) {
     if (t <= 16) {
       if (matmul_stream(c, x, w, out, t, k, n, epi)) {

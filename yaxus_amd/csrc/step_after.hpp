@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * kMmWaves) void matmul_bf16_rows(const float* _
   }
   if (!xrow) return;
   if constexpr (E::kFused) {
-    store_out4(epi, out, xt, n0 + 4 * g, n, wide_out(epi, out, n), sum[0], sum[W - 1]);
+    store_out4(epi, out, xt, n0 + 4 * g, n, wide_out(out, n), sum[0], sum[W - 1]);
   } else {
     float* o = out + static_cast<size_t>(xt) * n + n0 + 4 * g;
 #pragma unroll
