@@ -119,6 +119,7 @@ CASES = [
     (16, 4096, 8192), (9, 1000, 9000), (16, 8192, 2048), (32, 2048, 4100), (17, 1048, 12000), (2, 776, 16001),
     # LDS tiles of each shape, k ending inside a stage, n no multiple of 4
     (80, 2048, 2752), (64, 1536, 6001), (333, 1536, 1501), (1000, 1000, 1030), (300, 2048, 5512), (2048, 520, 2056),
+    (130, 1048, 9000), (700, 4096, 4100), (33, 9000, 2100), (1100, 1000, 3000),
 ]
 
 
@@ -175,7 +176,7 @@ def test_activations_over_the_range(hip, act):
     assert got[2] == {"none": -np.inf, "relu": 0.0}.get(act) if act in ("none", "relu") else np.isnan(got[2])
 
 
-@pytest.mark.parametrize("t,k,n", [(5, 256, 64), (16, 2048, 8192), (100, 512, 2048)])
+@pytest.mark.parametrize("t,k,n", [(5, 256, 64), (16, 2048, 8192), (100, 512, 2048), (700, 1000, 4100)])
 @pytest.mark.parametrize("gated", [False, True])
 def test_nonfinite_rows_stay_in_their_rows(hip, t, k, n, gated):
     x, w, b, r = inputs(t, k, n, gated, 9)

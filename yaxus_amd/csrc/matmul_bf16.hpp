@@ -69,6 +69,14 @@ __device__ __forceinline__ void split_bf16x3(float f0, float f1, uint32_t& h, ui
 // outputs; a wave's loads are from one of the two parts (8 or 16 consecutive rows).
 // With ks > 1 (grid y) the ks workgroups of a tile take consecutive stages and hand
 // their tiles over as matmul_bf16_rows does.
+// kRuns: workgroups are not tied to tiles. The stages of all tiles, one tile's after the other's,
+// are dealt out in runs of `per`, so few tiles, or a few more than fill the GPU once, load all CUs
+// alike (1000 x 2048 x 12000 144 -> 131 us, 3000 x 1000 x 3000 86 -> 72, 333 x 4096 x 11008 118 ->
+// 96). A run may end one tile, do whole ones and begin another; a tile of several workgroups is
+// joined in k order by the last of them to arrive, which adds its own part from its registers. At
+// most the first and the last tile of a run are shared, so scratch is two tiles per workgroup, and
+// a shared tile's counter is that of its first workgroup. Where every workgroup has one tile
+// the loop around it costs 2-7% (registers), so those are not runs.
 // Measured (k = n = 2048): t 4096 702 -> 81 us (128 x 256 tiles, 425 TFLOP/s, 3x that in
 // matrix instructions), t 2048 350 -> 54, t 512 90 -> 22, t 80 19.4 -> 12.0.
 template <int TM_, int TN_, int WM_, int WN_, int KU_, int kWaves_>
@@ -83,10 +91,11 @@ using MatmulTileC = MatmulTile<64, 128, 2, 4, 2, 2>;
 using MatmulTileD = MatmulTile<64, 64, 2, 4, 2, 4>;
 using MatmulTileDGated = MatmulTile<64, 64, 4, 2, 2, 4>;  // two weight tiles per wave
 
-template <class T, class E>
+template <class T, class E, bool kRuns>
 __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_tiles(
     const float* __restrict__ x, const uint16_t* __restrict__ w, float* out, uint32_t t, uint32_t k,
-    uint32_t n, f32x4* __restrict__ part, uint32_t part_bytes, uint32_t* __restrict__ counters, E epi) {
+    uint32_t n, uint32_t per, f32x4* __restrict__ part, uint32_t part_bytes, uint32_t* __restrict__ counters,
+    E epi) {
   constexpr int TM = T::TM, TN = T::TN, KU = T::KU, KT = T::KT, TH = kMatmulThreads;
   static_assert(T::WM * T::WN * 64 == TH, "8 waves");
   constexpr int MT = TM / T::WM / 16, NT = TN / T::WN / 16;  // 16 x 16 tiles per wave
@@ -104,15 +113,17 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
   const int wm = wave / T::WN, wn = wave % T::WN;
   // Tiles so that those running on one XCD (workgroups are dealt to the 8 XCDs in turn)
   // are consecutive, the operand with fewer tiles fastest: they share operands in its L2.
-  const uint32_t ntn = (n + TC - 1) / TC, ntt = (t + TM - 1) / TM, tiles = ntn * ntt;
+  const uint32_t ntn = (n + TC - 1) / TC, ntt = (t + TM - 1) / TM;
   const uint32_t xcd = blockIdx.x & 7;
-  const uint32_t tile = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (blockIdx.x >> 3);
-  const uint32_t n0 = (ntn <= ntt ? tile % ntn : tile / ntt) * TC;
-  const uint32_t t0 = (ntn <= ntt ? tile / ntn : tile % ntt) * TM;
-  const uint32_t ks = gridDim.y, kp = blockIdx.y;
+  const uint32_t place = xcd * (gridDim.x >> 3) + min(xcd, gridDim.x & 7) + (blockIdx.x >> 3);
   const uint32_t stages = (k + KT - 1) / KT;
-  const uint32_t s0 = static_cast<uint32_t>(static_cast<uint64_t>(stages) * kp / ks);
-  const uint32_t s1 = static_cast<uint32_t>(static_cast<uint64_t>(stages) * (kp + 1) / ks);
+  const uint32_t ks = gridDim.y, kp = blockIdx.y;
+  uint32_t tile, n0, t0, s0, s1;  // the tile at work, its stages
+  const auto start = [&](uint32_t at) {
+    tile = at;
+    n0 = (ntn <= ntt ? tile % ntn : tile / ntt) * TC;
+    t0 = (ntn <= ntt ? tile / ntn : tile % ntt) * TM;
+  };
   const uint32_t seg = max(2u, (stages >> 3) & ~1u);  // stages per partial sum (even: the slots alternate)
 
   int xd[XC], wd[WC], xo[XC], wo[WC];  // LDS chunk, global byte offset in the tile's rows
@@ -132,8 +143,9 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
     wo[i] = (col * static_cast<int>(k) + kc * 8) * 2;
     wd[i] = (kc / 4) * TN * 4 + row * 4 + ((kc & 3) ^ ((row >> 1) & 3));
   }
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(const_cast<float*>(x + static_cast<size_t>(t0) * k),
-                                              min(t - t0, static_cast<uint32_t>(TM)) * k * 4);
+  const auto rx = [&]() {
+    return make_rsrc(const_cast<float*>(x + static_cast<size_t>(t0) * k), min(t - t0, static_cast<uint32_t>(TM)) * k * 4);
+  };
   // Of the weight rows of this wave's i-th chunks: gated, every second 16 rows of the tile are
   // up rows.
   const auto rw = [&](int i) {
@@ -151,17 +163,17 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
     u32x4 p[XC][3];
   };
   // Stage s (the last one again past the end, which nothing uses).
-  const auto load_x = [&](XRegs& r, uint32_t s) {
+  const auto load_x = [&](XRegs& r, uint32_t s) __attribute__((always_inline)) {
     const uint32_t kb = min(s, s1 - 1) * KT;
     const bool tail = kb + KT > k;  // uniform
 #pragma unroll
     for (int i = 0; i < XC; ++i) {
       const int o = tail && kb + xk[i] >= k ? kOutside : xo[i];
-      r.a[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, o, kb * 4, 0));
-      r.b[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, o, kb * 4 + 16, 0));
+      r.a[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx(), o, kb * 4, 0));
+      r.b[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx(), o, kb * 4 + 16, 0));
     }
   };
-  const auto load_w = [&](WRegs& r, uint32_t s) {
+  const auto load_w = [&](WRegs& r, uint32_t s) __attribute__((always_inline)) {
     const uint32_t kb = min(s, s1 - 1) * KT;
     const bool tail = kb + KT > k;
 #pragma unroll
@@ -171,7 +183,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
     }
   };
   float big = 0.0f;  // the largest |x| this thread has cut up
-  const auto split = [&](XParts& o, const XRegs& r, auto inf) {
+  const auto split = [&](XParts& o, const XRegs& r, auto inf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < XC; ++i) {
       const float v[8] = {r.a[i].x, r.a[i].y, r.a[i].z, r.a[i].w, r.b[i].x, r.b[i].y, r.b[i].z, r.b[i].w};
@@ -191,7 +203,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
       }
     }
   };
-  const auto write = [&](const XParts& xp, const WRegs& wr, int slot) {
+  const auto write = [&](const XParts& xp, const WRegs& wr, int slot) __attribute__((always_inline)) {
     u16x8* xb = &xs[slot][0][0][0];
     u16x8* wb = &ws[slot][0][0];
 #pragma unroll
@@ -203,7 +215,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
     for (int i = 0; i < WC; ++i) wb[wd[i]] = wr.v[i];
   };
   bf16x8 wf[KU][NT], xf[KU][MT][3];
-  const auto read_operands = [&](int slot) {
+  const auto read_operands = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < KU; ++u) {
 #pragma unroll
@@ -217,7 +229,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
     }
   };
   f32x4 acc[NT][MT], sum[NT][MT];
-  const auto multiply = [&](auto first) {  // first: a new partial sum
+  const auto multiply = [&](auto first) __attribute__((always_inline)) {  // first: a new partial sum
 #pragma unroll
     for (int u = 0; u < KU; ++u)
 #pragma unroll
@@ -243,7 +255,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
   XRegs xr[2];
   WRegs wr[2];
   XParts xp;
-  const auto run = [&](auto inf) {
+  const auto run = [&](auto inf) __attribute__((always_inline)) {
 #pragma unroll
     for (int a = 0; a < NT; ++a)
 #pragma unroll
@@ -260,7 +272,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
     load_x(xr[1], s0 + 3);
     barrier();
     if (late) barrier();
-    const auto stage = [&](uint32_t s, auto parity, auto first) {
+    const auto stage = [&](uint32_t s, auto parity, auto first) __attribute__((always_inline)) {
       constexpr int P = decltype(parity)::value;
       write(xp, wr[P ^ 1], P ^ 1);
       load_w(wr[P ^ 1], s + 3);
@@ -297,48 +309,108 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
     }
     if (!late) barrier();
   };
-  run(std::false_type{});
-  if (__builtin_expect(__syncthreads_or(big == INFINITY), 0)) run(std::true_type{});
-
-  if (ks > 1) {  // as matmul_bf16_rows: write-through partial tiles, an arrival count
-    const __amdgpu_buffer_rsrc_t rp = make_rsrc(part, part_bytes);
-    constexpr uint32_t kTile = TM * TN / 4;  // in f32x4
-    const uint32_t base = tile * ks * kTile + wave * MT * NT * 64 + lane;
+  const auto products = [&]() __attribute__((always_inline)) {
+    big = 0.0f;
+    run(std::false_type{});
+    if (__builtin_expect(__syncthreads_or(big == INFINITY), 0)) run(std::true_type{});
+  };
+  const __amdgpu_buffer_rsrc_t rp = make_rsrc(part, part_bytes);
+  constexpr uint32_t kTile = TM * TN / 4;  // in f32x4
+  const uint32_t mine = wave * MT * NT * 64 + lane;
+  // The tile in `sum` to a slot of the scratch (write-through), and an arrival: whether it was the
+  // last of `all` at the counter.
+  const auto hand_over = [&](uint32_t slot, uint32_t counter, uint32_t all) __attribute__((always_inline)) {
 #pragma unroll
     for (int a = 0; a < NT; ++a)
 #pragma unroll
       for (int b = 0; b < MT; ++b)
-        st4_coherent(rp, (base + kp * kTile + (a * MT + b) * 64) * 16, __builtin_bit_cast(float4, sum[a][b]));
+        st4_coherent(rp, (slot * kTile + mine + (a * MT + b) * 64) * 16, __builtin_bit_cast(float4, sum[a][b]));
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (tid == 0) {
-      uint32_t* cnt = counters + static_cast<size_t>(tile) * kCounterStride;
+      uint32_t* cnt = counters + static_cast<size_t>(counter) * kCounterStride;
       const uint32_t arrived = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      last = arrived == ks - 1;
+      last = arrived == all - 1;
       if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (!last) return;
+    return last != 0;
+  };
+  const auto store = [&]() __attribute__((always_inline)) {
+    const bool wide = wide_out(out, n);
+    constexpr int W = E::kGated ? 2 : 1;
 #pragma unroll
-    for (int a = 0; a < NT; ++a)
+    for (int b = 0; b < MT; ++b) {
+      const uint32_t row = t0 + (wm * MT + b) * 16 + c;
+      if (row >= t) continue;
 #pragma unroll
-      for (int b = 0; b < MT; ++b) sum[a][b] = f32x4{0, 0, 0, 0};
-    for (uint32_t q = 0; q < ks; ++q)  // the parts in k order
+      for (int a = 0; a < NT; a += W)
+        store_out4(epi, out, row, n0 + (wn * NT + a) / W * 16 + 4 * g, n, wide, sum[a][b], sum[a + W - 1][b]);
+    }
+  };
+  if constexpr (kRuns) {
+    const uint64_t units = static_cast<uint64_t>(ntn) * ntt * stages;
+    const uint64_t begin = static_cast<uint64_t>(place) * per, end = min(units, begin + per);
+    uint64_t at = begin;
+    for (uint32_t next = static_cast<uint32_t>(begin / stages); at < end; ++next) {
+      if (at != begin) __syncthreads();  // LDS was read by every wave
+      const uint64_t t_first = static_cast<uint64_t>(next) * stages;
+      const uint32_t until = static_cast<uint32_t>(min(static_cast<uint64_t>(stages), end - t_first));
+      start(next);
+      s0 = static_cast<uint32_t>(at - t_first);
+      s1 = until;
+      at = t_first + until;
+      products();
+      if (s0 != 0 || until != stages) {
+        // Workgroups r0 .. r1 share the tile; all but r0 begin in it.
+        const uint32_t r0 = static_cast<uint32_t>(t_first / per), r1 = static_cast<uint32_t>((t_first + stages - 1) / per);
+        const auto slot = [&](uint32_t r) { return 2 * r + (static_cast<uint64_t>(r) * per < t_first ? 1 : 0); };
+        if (!hand_over(slot(place), r0, r1 - r0 + 1)) continue;
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+          for (int b = 0; b < MT; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
+        for (uint32_t r = r0; r <= r1; ++r) {
+          if (r == place) {
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+              for (int b = 0; b < MT; ++b) acc[a][b] = acc[a][b] + sum[a][b];
+          } else {
+            const uint32_t from = slot(r) * kTile + mine;
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+              for (int b = 0; b < MT; ++b)
+                acc[a][b] = acc[a][b] + __builtin_bit_cast(f32x4, ld4_coherent(rp, (from + (a * MT + b) * 64) * 16));
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < NT; ++a)
+#pragma unroll
+          for (int b = 0; b < MT; ++b) sum[a][b] = acc[a][b];
+      }
+      store();
+    }
+  } else {
+    start(place);
+    s0 = static_cast<uint32_t>(static_cast<uint64_t>(stages) * kp / ks);
+    s1 = static_cast<uint32_t>(static_cast<uint64_t>(stages) * (kp + 1) / ks);
+    products();
+    if (ks > 1) {  // as matmul_bf16_rows: write-through partial tiles, an arrival count
+      if (!hand_over(tile * ks + kp, tile, ks)) return;
 #pragma unroll
       for (int a = 0; a < NT; ++a)
 #pragma unroll
-        for (int b = 0; b < MT; ++b)
-          sum[a][b] = sum[a][b] + __builtin_bit_cast(f32x4, ld4_coherent(rp, (base + q * kTile + (a * MT + b) * 64) * 16));
-  }
-  const bool wide = wide_out(out, n);
-  constexpr int W = E::kGated ? 2 : 1;
+        for (int b = 0; b < MT; ++b) sum[a][b] = f32x4{0, 0, 0, 0};
+      for (uint32_t q = 0; q < ks; ++q)  // the parts in k order
 #pragma unroll
-  for (int b = 0; b < MT; ++b) {
-    const uint32_t row = t0 + (wm * MT + b) * 16 + c;
-    if (row >= t) continue;
+        for (int a = 0; a < NT; ++a)
 #pragma unroll
-    for (int a = 0; a < NT; a += W)
-      store_out4(epi, out, row, n0 + (wn * NT + a) / W * 16 + 4 * g, n, wide, sum[a][b], sum[a + W - 1][b]);
+          for (int b = 0; b < MT; ++b)
+            sum[a][b] = sum[a][b] + __builtin_bit_cast(f32x4, ld4_coherent(rp, ((tile * ks + q) * kTile + mine + (a * MT + b) * 64) * 16));
+    }
+    store();
   }
 }
 

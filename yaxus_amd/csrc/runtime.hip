@@ -1597,15 +1597,17 @@ bool matmul_stream(yx_ctx* c, const float* x, const uint16_t* w, float* out, uin
 struct MatmulShape {
   uint32_t tm, tn, per_cu;  // workgroups per CU
   double stage_us;          // per 32 k, with per_cu workgroups on a CU
+  uint32_t kt;              // k of a stage
 };
-constexpr MatmulShape kMatmulShapes[] = {{128, 256, 1, 1.22}, {128, 128, 1, 0.75}, {64, 128, 1, 0.46}, {64, 64, 2, 0.56}};
+constexpr MatmulShape kMatmulShapes[] = {
+    {128, 256, 1, 1.22, 32}, {128, 128, 1, 0.75, 32}, {64, 128, 1, 0.46, 64}, {64, 64, 2, 0.56, 64}};
 
-// Its scratch, for splits of at most one round of workgroups (32 MiB on 256 CUs).
+// Its scratch, two tiles for each of one round of workgroups (64 MiB on 256 CUs).
 int matmul_tiles_scratch(yx_ctx* c) {
   size_t part = 0, slots = 0;
   for (const MatmulShape& sh : kMatmulShapes) {
     slots = std::max(slots, static_cast<size_t>(sh.per_cu) * c->cus);
-    part = std::max(part, static_cast<size_t>(sh.per_cu) * c->cus * sh.tm * sh.tn * 4);
+    part = std::max(part, 2 * static_cast<size_t>(sh.per_cu) * c->cus * sh.tm * sh.tn * 4);
   }
   if (int rc = c->mt_part.ensure(part, c->stream)) return rc;
   return c->mt_counters.ensure(slots * 4 * yx::kCounterStride, c->stream, true);
@@ -1623,6 +1625,7 @@ struct MatmulSplit {
   int shape;
   uint32_t ks;
   double us;  // estimated
+  uint32_t per = 0;  // not 0: runs of this many stages
 };
 MatmulSplit matmul_tile_split(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
   const uint32_t steps = (k + 31) / 32;
@@ -1640,6 +1643,36 @@ MatmulSplit matmul_tile_split(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
                         (ks > 1 ? 1.0 + ks * (sh.tm * sh.tn) / 12500.0 : 0.0);
       if (us < best.us) best = {s, ks, us};
     }
+  }
+  return best;
+}
+
+// The same with an epilogue, where a tile's parts may be any number up to 8, and, where that leaves
+// CUs idle in a round, all stages may be dealt out evenly in runs. Then up to two tiles of a
+// workgroup are shared, and each costs writing it through (about 20 GB/s a CU) and 2 us, and its
+// last workgroup reading the others' parts. (us, estimated and measured, whole tiles or parts / runs:
+// 333 x 1536 x 6001 34 and 37 / 39 and 35, 1000 x 2048 x 12000 164 and 144 / 142 and 131, 3000 x
+// 1000 x 3000 85 and 86 / 72 and 72; 64 x 2048 x 11024 23 and 21 / 25 and 23.)
+MatmulSplit matmul_tile_runs(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
+  MatmulSplit best{0, 1, 1e30};
+  for (int s = 0; s < 4; ++s) {
+    const MatmulShape& sh = kMatmulShapes[s];
+    const uint32_t stages = (k + sh.kt - 1) / sh.kt;
+    const uint64_t tiles = static_cast<uint64_t>((t + sh.tm - 1) / sh.tm) * ((n + sh.tn - 1) / sh.tn);
+    const uint64_t slots = static_cast<uint64_t>(sh.per_cu) * c->cus;
+    const double stage = sh.stage_us * (sh.kt / 32), tile_kb = sh.tm * sh.tn / 256.0;
+    for (uint32_t ks = 1; ks <= 8 && (ks == 1 || (stages / ks * (sh.kt / 32) >= 8 && tiles * ks <= slots)); ++ks) {
+      const uint64_t rounds = (tiles * ks + slots - 1) / slots;
+      // A CU with one workgroup where two fit runs it faster.
+      const double one = sh.per_cu > 1 && tiles * ks * sh.per_cu <= slots ? 0.6 * stage : stage;
+      const double us = 5.0 + rounds * (one * stages / ks + 1.0) + (ks > 1 ? 1.0 + ks * tile_kb / 48.0 : 0.0);
+      if (us < best.us) best = {s, ks, us, 0};
+    }
+    const uint64_t even = (tiles * stages + slots - 1) / slots;
+    if (even < 4 || even > 0x7fffffff || even % stages == 0 || stages % even == 0) continue;  // too short; as above
+    const double parts = static_cast<double>(stages) / even;  // of a tile
+    const double us = 8.0 + stage * even + std::min(2.0, 1.0 + 1.0 / parts) * (tile_kb / 20.0 + 2.0) + parts * tile_kb / 48.0;
+    if (us < best.us) best = {s, static_cast<uint32_t>(std::ceil(parts)), us, static_cast<uint32_t>(even)};
   }
   return best;
 }
@@ -1716,17 +1749,29 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
   const size_t cols = E::kGated ? sh.tn / 2 : sh.tn;
   const size_t tiles = ((t + sh.tm - 1) / sh.tm) * ((n + cols - 1) / cols);
   if (tiles > 0x7fffffff) return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
+  const size_t stages = (k + sh.kt - 1) / sh.kt, grid = split.per ? (tiles * stages + split.per - 1) / split.per : tiles;
   const auto go = [&](auto* kern) {
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(tiles), split.ks), dim3(yx::kMatmulThreads), 0, c->stream, x,
-                       w, out, t, k, n, static_cast<yx::f32x4*>(c->mt_part.p),
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(grid), split.per ? 1 : split.ks), dim3(yx::kMatmulThreads), 0,
+                       c->stream, x, w, out, t, k, n, split.per, static_cast<yx::f32x4*>(c->mt_part.p),
                        static_cast<uint32_t>(c->mt_part.cap), static_cast<uint32_t*>(c->mt_counters.p), epi);
   };
-  using D = std::conditional_t<E::kGated, yx::MatmulTileDGated, yx::MatmulTileD>;
-  switch (split.shape) {
-    case 0: go(yx::matmul_bf16_tiles<yx::MatmulTileA, E>); break;
-    case 1: go(yx::matmul_bf16_tiles<yx::MatmulTileB, E>); break;
-    case 2: go(yx::matmul_bf16_tiles<yx::MatmulTileC, E>); break;
-    default: go(yx::matmul_bf16_tiles<D, E>); break;
+  const auto shape = [&](auto runs) {
+    constexpr bool kRuns = decltype(runs)::value;
+    using D = std::conditional_t<E::kGated, yx::MatmulTileDGated, yx::MatmulTileD>;
+    switch (split.shape) {
+      case 0: go(yx::matmul_bf16_tiles<yx::MatmulTileA, E, kRuns>); break;
+      case 1: go(yx::matmul_bf16_tiles<yx::MatmulTileB, E, kRuns>); break;
+      case 2: go(yx::matmul_bf16_tiles<yx::MatmulTileC, E, kRuns>); break;
+      default: go(yx::matmul_bf16_tiles<D, E, kRuns>); break;
+    }
+  };
+  if constexpr (E::kFused) {
+    if (split.per)
+      shape(std::true_type{});
+    else
+      shape(std::false_type{});
+  } else {
+    shape(std::false_type{});
   }
   YX_HIP(hipGetLastError());
   return YX_OK;
@@ -1790,7 +1835,7 @@ int matmul_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32
         return YX_OK;
       }
     } else if (k <= (size_t{1} << 20)) {  // a tile's rows within a buffer resource
-      const MatmulSplit split = matmul_tile_split(c, t, k, W * n);
+      const MatmulSplit split = E::kFused ? matmul_tile_runs(c, t, k, W * n) : matmul_tile_split(c, t, k, W * n);
       if (!matmul_rows_faster(c, t, k, W * n, split.us)) return matmul_tiled(c, x, w, out, t, k, n, split, epi);
     }
   }
