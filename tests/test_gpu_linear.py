@@ -242,3 +242,48 @@ def test_graph_replays_match_eager(hip, t, k, n):
     finally:
         for d in (dx, dw, db, out):
             d.free()
+
+
+def part(hip, t, first, n, dtype=np.float32):
+    """Values first .. first + n of a device tensor."""
+    from yaxus_amd._lib import check_hip, ptr
+
+    a = np.empty(n, dtype)
+    check_hip(hip.L.yx_memcpy_d2h(hip.ctx, ptr(a), ctypes.c_void_p(t.ptr.value + first * a.itemsize), a.nbytes))
+    return a
+
+
+def test_output_beyond_32_bits(hip):
+    """More than 2^32 outputs: the last rows of a product with a short k."""
+    t, k, n = 66000, 8, 66000
+    x, w = normal(t * k, 31, 3).reshape(t, k), bf16_bits(normal(n * k, 32, 3).reshape(n, k))
+    dx, dw, out = hip.tensor(x.shape).upload(x), hip.tensor(w.shape, np.uint16).upload(w), hip.tensor((t, n))
+    try:
+        hip.linear_bf16(dx, dw, act="relu", out=out)
+        for rows in (slice(0, 2), slice(t - 3, t)):
+            got = part(hip, out, rows.start * n, (rows.stop - rows.start) * n).reshape(-1, n)
+            want, bound = linear64(x[rows], w, None, "relu", False, None)
+            assert np.all(np.abs(got - want) <= bound)
+    finally:
+        for d in (dx, dw, out):
+            d.free()
+
+
+@pytest.mark.parametrize("t,k,n", [(2, 8192, 140000), (40, 8192, 140000), (3, 7992, 140000)])
+def test_weight_beyond_32_bits(hip, t, k, n):
+    """A gated weight of more than 4 GiB (the up rows begin beyond 2 GiB): the first and last
+    columns."""
+    x = normal(t * k, 31, 7).reshape(t, k)
+    dx, dw, out = hip.tensor(x.shape).upload(x), hip.tensor((2 * n, k), np.uint16), hip.tensor((t, n))
+    try:
+        # binary16 bits of a normal read as bf16: finite values from 2^-126 to 2^-6.
+        hip.fill_normal(dw.ptr, 2 * n * k, True, 77)
+        hip.linear_bf16(dx, dw, act="silu", gated=True, out=out)
+        got = out.numpy()
+        for c in (0, n - 300):
+            w = np.concatenate([part(hip, dw, (half * n + c) * k, 300 * k, np.uint16).reshape(300, k) for half in (0, 1)])
+            want, bound = linear64(x, w, None, "silu", True, None)
+            assert np.all(np.abs(got[:, c:c + 300] - want) <= bound)
+    finally:
+        for d in (dx, dw, out):
+            d.free()

@@ -303,3 +303,26 @@ def test_two_contexts_at_once():
     finally:
         for h in hips:
             h.close()
+
+
+@pytest.mark.parametrize("rows,ld,cols", [(33000, 131072, 130003), (3, 1 << 31, 40000)])
+def test_offsets_beyond_32_bits(hip, rows, ld, cols):
+    """More than 2^32 logits (17 and 25 GB), and rows that lie 8 GiB apart: the first and last rows."""
+    x, t = hip.tensor((rows, ld)), some(rows, cols)
+    dt = hip.tensor(t.shape, np.uint32).upload(t.astype(np.uint32))
+    out = None
+    try:
+        hip.fill_normal(x.ptr, rows * ld, False, 5)
+        out = hip.logprobs_rows(x, tokens=dt, top=6, cols=cols)
+        got = [o.numpy() for o in out]
+        for r in (0, rows - 1):
+            a = np.empty((1, cols), np.float32)
+            _lib.check_hip(hip.L.yx_memcpy_d2h(hip.ctx, _lib.ptr(a), ctypes.c_void_p(x.ptr.value + 4 * r * ld), a.nbytes))
+            wl, dl, we, de, wi, wt, dtt = oracle(a, t[r:r + 1], 6)
+            np.testing.assert_array_equal(got[2][r:r + 1], wi)
+            near(got[0][r:r + 1], wl, dl)
+            near(got[1][r:r + 1], we, de)
+            near(got[3][r:r + 1], wt, dtt)
+    finally:
+        for d in (x, dt, *(out or ())):
+            d.free()
