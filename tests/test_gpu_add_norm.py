@@ -82,7 +82,7 @@ def inputs(rows, cols, seed=0):
 
 
 SIZES = [(1, 1), (3, 2), (2, 63), (5, 64), (1, 255), (4, 257), (16, 2048), (7, 2047), (1, 4096), (3, 8192),
-         (2, 8196), (2, 10001), (1, 40000), (700, 1000), (4096, 260)]
+         (2, 8196), (2, 10001), (3, 16384), (2, 16385), (1, 40000), (300, 5000), (700, 1000), (4096, 260)]
 
 
 @pytest.mark.parametrize("post,add,norm", [(0, 0, 1), (0, 1, 1), (1, 1, 1), (1, 1, 0), (0, 1, 0), (1, 0, 0), (1, 0, 1)])

@@ -208,7 +208,8 @@ def test_nan_and_infinity(hip, rows, cols):
     x[4, :] = np.nan
     x[7, [3, cols - 2]] = np.inf
     x[9, ::3] = np.nan
-    x[9, 1] = -np.inf
+    x.view(np.uint32)[9, 1::7] = 0x7F800001  # signalling ones
+    x[9, 4] = -np.inf
     lp, ent, ids, tlp = run(hip, x, t, 6)
     bad = [1, 4, 7, 9]
     good = [i for i in range(rows) if i not in bad]

@@ -203,9 +203,15 @@ __global__ __launch_bounds__(kLpThreads, 4) void logprobs_rows(const float* __re
         u[j] = fmaf(fmaxf(d, -300.0f), e, u[j]);
       }
     }
-    a.s += (s[0] + s[1]) + (s[2] + s[3]);
+    const float chunk_s = (s[0] + s[1]) + (s[2] + s[3]);
+    a.s += chunk_s;
     a.u += (u[0] + u[1]) + (u[2] + u[3]);
     if (top == 0) return;
+    if (chunk_s != chunk_s) {  // a signalling NaN may have cost v_max3 the maximum so far
+      m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4 * kLpQuads; ++i) m = v[i / 4][i % 4] > m ? v[i / 4][i % 4] : m;
+    }
 
     if (floor == 1ull) {  // fewer than `top` so far: a value that `top` logits reach, if that many are
       sh.ord[tid] = static_cast<uint32_t>(top_key(m, 0) >> 32);

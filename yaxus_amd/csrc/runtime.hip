@@ -2600,16 +2600,15 @@ int yx_add_norm_rows_dev(yx_ctx* c, const float* x, const float* post_w, float p
   int rc = c->set_device();
   if (rc) return rc;
   const yx::AddNorm a{x, post_w, h, h_out, w, out, post_offset, offset, eps};
-  const auto go = [&](auto* kern) {
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(rows)), dim3(yx::kNormThreads), 0, c->stream, a,
-                       static_cast<uint32_t>(cols));
+  const auto go = [&](auto* kern, int threads) {
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, c->stream, a, static_cast<uint32_t>(cols));
   };
-  const size_t per = (cols + 4 * yx::kNormThreads - 1) / (4 * yx::kNormThreads);  // pieces of a thread
-  if (per <= 1) go(yx::add_norm_rows<1>);
-  else if (per <= 2) go(yx::add_norm_rows<2>);
-  else if (per <= 4) go(yx::add_norm_rows<4>);
-  else if (per <= 8) go(yx::add_norm_rows<8>);
-  else go(yx::add_norm_long_rows);
+  if (cols <= 1024) go(yx::add_norm_rows<256, 1>, 256);
+  else if (cols <= 2048) go(yx::add_norm_rows<256, 2>, 256);
+  else if (cols <= 4096) go(yx::add_norm_rows<256, 4>, 256);
+  else if (cols <= 8192) go(yx::add_norm_rows<512, 4>, 512);
+  else if (cols <= 16384) go(yx::add_norm_rows<1024, 4>, 1024);
+  else go(yx::add_norm_long_rows, yx::kNormLongThreads);
   YX_HIP(hipGetLastError());
   return YX_OK;
 }
