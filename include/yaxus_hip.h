@@ -94,9 +94,10 @@ int yx_ctx_set_option(yx_ctx* ctx, const char* key, long value);
  * "prefill_split_tiles" (prefill tiles split along keys in the work lists built) and
  * "prefill_plans" (work lists built as prefill tiles rather than decode items); "decode_items",
  * the items, of all heads, of the latest list of decode items. And of its
- * latest yx_matmul_bf16_dev: "matmul_kernel" (0 none yet, 1 the kernel of 16 x 16 tiles, 2 the
- * one that streams the weight, 3 to 6 LDS tiles of 128 x 256, 128 x 128, 64 x 128, 64 x 64) and
- * "matmul_k_parts" (the workgroups of a tile along k).
+ * latest yx_matmul_bf16_dev or yx_linear_bf16_dev: "matmul_kernel" (0 none yet, 1 the kernel of 16 x 16 tiles, 2 the
+ * one that streams the weight, 3 to 6 LDS tiles of 128 x 256, 128 x 128, 64 x 128, 64 x 64; of
+ * yx_linear_bf16_dev also 7, tiles of 96 x 128, and 8, the kernel of few rows) and "matmul_k_parts"
+ * (the workgroups of a tile along k, at most).
  * A pass whose groups keep their order and fit the device regions of the previous pass
  * sends only the entries that changed. */
 int yx_ctx_get_stat(yx_ctx* ctx, const char* key, uint64_t* out);
@@ -227,9 +228,10 @@ int yx_argmax_rows_dev(yx_ctx* ctx, const float* logits, size_t rows, size_t col
  * out itself (rows added to in place), otherwise out overlaps no input. act is a YX_ACT_*
  * value. Sums, activation, gate and residual are f32 (an activation is within 2^-21 of its
  * argument, gelu 2^-19); -inf gives NaN in silu and the gelus. k a
- * multiple of 8, x and w 16-byte aligned, the others 4-byte aligned (16-byte accesses where
- * all are 16-byte aligned and n is a multiple of 4). matmul_k_split applies as above, and
- * the statistics matmul_kernel and matmul_k_parts report these calls too. */
+ * multiple of 8, x and w 16-byte aligned, the others 4-byte aligned. With matmul_k_split set,
+ * the kernel of 16 x 16 tiles takes every size. As yx_matmul_bf16_dev, a row's bits do not depend on the others of
+ * a pass of up to 16, and a call that needs more scratch than any before (few tiles, split along
+ * k) is refused under capture; without bias, activation, gate and residual it is that call. */
 int yx_linear_bf16_dev(yx_ctx* ctx, const float* x, const uint16_t* w, const float* bias, int act,
                        int gated, const float* residual, float* out, size_t t, size_t k, size_t n);
 /* The seam between two blocks (f32, `[rows][cols]`): with norm(v; w, o)_i =

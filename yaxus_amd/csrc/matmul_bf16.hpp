@@ -89,6 +89,7 @@ using MatmulTileA = MatmulTile<128, 256, 4, 2, 1, 2>;
 using MatmulTileB = MatmulTile<128, 128, 4, 2, 1, 2>;
 using MatmulTileC = MatmulTile<64, 128, 2, 4, 2, 2>;
 using MatmulTileD = MatmulTile<64, 64, 2, 4, 2, 4>;
+using MatmulTileF = MatmulTile<96, 128, 2, 4, 2, 2>;
 using MatmulTileDGated = MatmulTile<64, 64, 4, 2, 2, 4>;  // two weight tiles per wave
 
 template <class T, class E, bool kRuns>
@@ -102,8 +103,8 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
   constexpr int TC = E::kGated ? TN / 2 : TN;                // output columns
   static_assert(!E::kGated || NT % 2 == 0, "a wave holds gate and up rows of its columns");
   // Chunks of 8 k per thread and stage.
-  constexpr int XC = TM * KT / 8 / TH, WC = TN * KT / 8 / TH;
-  static_assert(TM * KT / 8 == XC * TH && TN * KT / 8 == WC * TH, "whole rounds of chunks");
+  constexpr int XN = TM * KT / 8, XC = (XN + TH - 1) / TH, WC = TN * KT / 8 / TH;
+  static_assert(TN * KT / 8 == WC * TH && XN % 64 == 0, "whole rounds of chunks, of waves for x");
   constexpr int kOutside = 0x7ffffff0;  // beyond every resource: reads zeros
   __shared__ u16x8 xs[2][KU][3][TM * 4];
   __shared__ u16x8 ws[2][KU][TN * 4];
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
   for (int i = 0; i < XC; ++i) {
     const int id = i * TH + tid, row = id / (4 * KU), kc = id % (4 * KU);
     xk[i] = kc * 8;
-    xo[i] = (row * static_cast<int>(k) + kc * 8) * 4;
+    xo[i] = id < XN ? (row * static_cast<int>(k) + kc * 8) * 4 : kOutside;
     xd[i] = (kc / 4) * 3 * TM * 4 + row * 4 + ((kc & 3) ^ ((row >> 1) & 3));
   }
 #pragma unroll
@@ -208,6 +209,7 @@ __global__ __launch_bounds__(kMatmulThreads, T::kWavesPerSimd) void matmul_bf16_
     u16x8* wb = &ws[slot][0][0];
 #pragma unroll
     for (int i = 0; i < XC; ++i) {
+      if (XN % TH && i * TH + wave * 64 >= XN) break;  // uniform
 #pragma unroll
       for (int q = 0; q < 3; ++q) xb[xd[i] + q * TM * 4] = __builtin_bit_cast(u16x8, xp.p[i][q]);
     }

@@ -1593,14 +1593,15 @@ bool matmul_stream(yx_ctx* c, const float* x, const uint16_t* w, float* out, uin
   }
 }
 
-// The shapes of matmul_bf16_tiles.
+// The shapes of matmul_bf16_tiles; the last only with an epilogue.
 struct MatmulShape {
   uint32_t tm, tn, per_cu;  // workgroups per CU
   double stage_us;          // per 32 k, with per_cu workgroups on a CU
   uint32_t kt;              // k of a stage
 };
 constexpr MatmulShape kMatmulShapes[] = {
-    {128, 256, 1, 1.22, 32}, {128, 128, 1, 0.75, 32}, {64, 128, 1, 0.46, 64}, {64, 64, 2, 0.56, 64}};
+    {128, 256, 1, 1.22, 32}, {128, 128, 1, 0.75, 32}, {64, 128, 1, 0.46, 64}, {64, 64, 2, 0.56, 64},
+    {96, 128, 1, 0.60, 64}};
 
 // Its scratch, two tiles for each of one round of workgroups (64 MiB on 256 CUs).
 int matmul_tiles_scratch(yx_ctx* c) {
@@ -1651,11 +1652,13 @@ MatmulSplit matmul_tile_split(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
 // CUs idle in a round, all stages may be dealt out evenly in runs. Then up to two tiles of a
 // workgroup are shared, and each costs writing it through (about 20 GB/s a CU) and 2 us, and its
 // last workgroup reading the others' parts. (us, estimated and measured, whole tiles or parts / runs:
-// 333 x 1536 x 6001 34 and 37 / 39 and 35, 1000 x 2048 x 12000 164 and 144 / 142 and 131, 3000 x
-// 1000 x 3000 85 and 86 / 72 and 72; 64 x 2048 x 11024 23 and 21 / 25 and 23.)
+// 1000 x 2048 x 12000 164 and 144 / 142 and 131, 3000 x
+// 1000 x 3000 85 and 86 / 72 and 72; 64 x 2048 x 11024 23 and 21 / 25 and 23.) Tiles of 96 rows save
+// up to a quarter of the products: 80 x 2048 x 11024 30.0 -> 26.7, 190 x 2048 x 16384 48 -> 43, 180 x
+// 4096 x 4096 32.6 -> 28.5, 90 x 704 x 18000 21.5 -> 18.0.
 MatmulSplit matmul_tile_runs(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
   MatmulSplit best{0, 1, 1e30};
-  for (int s = 0; s < 4; ++s) {
+  for (int s = 0; s < 5; ++s) {
     const MatmulShape& sh = kMatmulShapes[s];
     const uint32_t stages = (k + sh.kt - 1) / sh.kt;
     const uint64_t tiles = static_cast<uint64_t>((t + sh.tm - 1) / sh.tm) * ((n + sh.tn - 1) / sh.tn);
@@ -1762,7 +1765,8 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
       case 0: go(yx::matmul_bf16_tiles<yx::MatmulTileA, E, kRuns>); break;
       case 1: go(yx::matmul_bf16_tiles<yx::MatmulTileB, E, kRuns>); break;
       case 2: go(yx::matmul_bf16_tiles<yx::MatmulTileC, E, kRuns>); break;
-      default: go(yx::matmul_bf16_tiles<D, E, kRuns>); break;
+      case 3: go(yx::matmul_bf16_tiles<D, E, kRuns>); break;
+      default: go(yx::matmul_bf16_tiles<yx::MatmulTileF, E, kRuns>); break;
     }
   };
   if constexpr (E::kFused) {
@@ -1803,7 +1807,7 @@ int matmul_few(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_
   const uint32_t groups = (n + cols - 1) / cols;
   const auto go = [&](auto* kern, uint32_t kc) {
     const uint32_t ks = std::max(1u, std::min({static_cast<uint32_t>(c->cus) / groups, (k + kc - 1) / kc, std::max(8u, k / 512)}));
-    c->mm_kernel = 7;
+    c->mm_kernel = 8;
     c->mm_k_parts = ks;
     hipLaunchKernelGGL(kern, dim3(groups, ks), dim3(yx::kFewThreads), 0, c->stream, x, w, out, t, k, n,
                        static_cast<yx::f32x4*>(c->mt_part.p), static_cast<uint32_t>(c->mt_part.cap),
