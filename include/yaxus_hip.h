@@ -10,6 +10,9 @@
  *                                          lib.rs:359-385, then attend, lib.rs:389-427);
  *                                          or its halves: yx_qk_rope_append_dev and
  *                                          yx_attention_dev; yx_kv_append stores K/V alone
+ * and what a backend with its rows on the device runs between attention calls and at the end:
+ *   products yx_matmul_bf16_dev and yx_linear_bf16_dev, block seams yx_add_norm_rows_dev,
+ *   yx_argmax_rows_dev and yx_logprobs_rows_dev.
  *
  * Conventions: int status, YX_OK = 0 (codes shared with yaxus_kv_cache.h);
  * yx_last_error() returns a thread-local message; no exception crosses the ABI. Every

@@ -7,6 +7,9 @@ the KV arena (crates/yaxus-model/src/lib.rs:95-171), over ``libyaxus_hip.so``.
     Backend::attention   (lib.rs:132)  -> HipBackend.append (the K/V store of
                                           write_rows) + HipBackend.attend
 
+The step after attention, on rows that stay on the device: ``matmul_bf16``, ``linear_bf16``
+(bias, activation, gate, residual), ``add_norm``, ``argmax_rows``, ``logprobs_rows``.
+
 Tensors are ``DeviceTensor`` values (device memory owned by the context); numpy arrays
 are accepted where a host round trip is intended. A missing library, or a context
 that cannot open a gfx950 device, raises: nothing here computes on the host.
