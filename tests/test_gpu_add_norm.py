@@ -137,6 +137,22 @@ def test_x_that_is_h(hip, put):
     assert np.all(np.abs(out.numpy() - ov) <= do)
 
 
+def test_more_rows_than_a_launch(hip):
+    """2^21 rows and some, over two launches, in place: the rows around the border and the last."""
+    rows, cols = (1 << 21) + 5, 3
+    x = normal(rows * cols, 51, 9).reshape(rows, cols)
+    w = 0.1 * normal(cols, 52, 9)
+    dx, dw = hip.tensor(x.shape).upload(x), hip.tensor(w.shape).upload(w)
+    try:
+        hip.add_norm(dx, w=dw, out=dx)
+        got = dx.numpy()
+        _, _, ov, do = want64(x, None, None, w, 1e-6)
+        assert np.all(np.abs(got - ov) <= do)
+    finally:
+        dx.free()
+        dw.free()
+
+
 def test_special_rows(hip, put):
     """Rows of zeros (with eps 0 too: 0 / 0), tiny and large values, infinities and NaN; each
     stays in its row."""

@@ -213,6 +213,37 @@ def test_forced_splits_of_k(hip, t, k, n, gated):
         hip.set_option("matmul_k_split", 0)
 
 
+def test_capture_of_a_first_call():
+    """Kernels whose scratch is the context's from the start are captured without an earlier call;
+    one that would have to grow it is refused, and works after an eager call."""
+    from yaxus_amd._lib import YxError
+    from yaxus_amd.backend import HipBackend
+
+    hip = HipBackend(0)
+    try:
+        for t, k, n, refused in ((16, 2048, 8192, False), (80, 2048, 2752, False), (3, 4096, 1000, True)):
+            x, w, b, r = inputs(t, k, n, True, 6)
+            want, bound = linear64(x, w, b, "silu", True, r)
+            dx, dw, db = hip.tensor(x.shape).upload(x), hip.tensor(w.shape, np.uint16).upload(w), hip.tensor(b.shape).upload(b)
+            dr, out = hip.tensor(r.shape).upload(r), hip.tensor(r.shape)
+            call = lambda: hip.linear_bf16(dx, dw, bias=db, act="silu", gated=True, residual=dr, out=out)
+            hip.graph_begin()
+            if refused:
+                with pytest.raises(YxError, match="before capturing"):
+                    call()
+                hip.graph_end()
+                call()
+                hip.graph_begin()
+            call()
+            hip.graph_end()
+            for _ in range(3):
+                out.upload(np.zeros(r.shape, np.float32))
+                hip.graph_launch()
+                assert np.all(np.abs(out.numpy() - want) <= bound)
+    finally:
+        hip.close()
+
+
 @pytest.mark.parametrize("t,k,n", [(2, 4096, 1000), (16, 2048, 8192), (80, 2048, 2752)])
 def test_graph_replays_match_eager(hip, t, k, n):
     """Captured after one eager call, in place on a residual; replays alternate with eager

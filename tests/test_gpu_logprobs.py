@@ -157,6 +157,11 @@ def test_given_tokens(hip, given):
     check(hip, logits(2000, 700), some(2000, 700, given), 3)
 
 
+def test_more_rows_than_a_launch(hip):
+    rows, cols = (1 << 21) + 3, 5
+    check(hip, logits(rows, cols), some(rows, cols), 2, ld=6, repeat=1)
+
+
 def patterns(cols):
     rng = np.random.default_rng(cols)
     base = logits(1, cols)[0]

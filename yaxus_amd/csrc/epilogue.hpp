@@ -1,10 +1,11 @@
 // What a weight product does with its sums before they leave the registers: nothing
 // (yx_matmul_bf16_dev), or bias, activation, gate and residual (yx_linear_bf16_dev):
 //   out = act(y + bias) + residual,  gated: act(y_gate + bias_gate) * (y_up + bias_up) + residual.
-// On its own each of these reads and writes the rows once more (16 MB for 4096 x 1024).
+// On its own each of these would read and write the rows once more (134 MB each way for 4096 x 8192).
 // Everything is f32; the activations' e^x and 1/x are the hardware's (within 1 ulp, e^x of an
 // argument rounded to f32), written so that no term cancels: silu and gelu_tanh divide by
-// 1 + e^-z, gelu uses erfc. The erfc costs ~40 vector instructions a value, the others ~10.
+// 1 + e^-z, gelu uses erfc. 4096 x 2048 x 8192 with bias: none 344 us, silu 348, gelu_tanh 350,
+// gelu 373.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

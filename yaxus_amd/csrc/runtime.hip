@@ -1698,6 +1698,9 @@ bool matmul_rows_faster(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n, double ti
   return rows_us < 1.05 * tiles_us - 1.5 + (n % 4 ? 0.9 : 0.0);
 }
 
+// Rows of one launch with a workgroup each: a launch has at most 2^32 - 1 threads.
+constexpr size_t kLaunchRows = size_t{1} << 21;
+
 // Workgroups of logprobs_rows that run at once (four per CU).
 size_t logprobs_slots(const yx_ctx* c) { return 4 * static_cast<size_t>(c->cus); }
 
@@ -1752,6 +1755,7 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
   const size_t cols = E::kGated ? sh.tn / 2 : sh.tn;
   const size_t tiles = ((t + sh.tm - 1) / sh.tm) * ((n + cols - 1) / cols);
   if (tiles > 0x7fffffff) return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
+  if (tiles > 0xffffffffu / yx::kMatmulThreads) return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
   const size_t stages = (k + sh.kt - 1) / sh.kt, grid = split.per ? (tiles * stages + split.per - 1) / split.per : tiles;
   const auto go = [&](auto* kern) {
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(grid), split.per ? 1 : split.ks), dim3(yx::kMatmulThreads), 0,
@@ -1805,6 +1809,7 @@ int matmul_few(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_
   constexpr int N = E::kGated ? 2 : 1;
   constexpr uint32_t cols = 128;
   const uint32_t groups = (n + cols - 1) / cols;
+  if (groups > 0xffffffffu / yx::kFewThreads) return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
   const auto go = [&](auto* kern, uint32_t kc) {
     const uint32_t ks = std::max(1u, std::min({static_cast<uint32_t>(c->cus) / groups, (k + kc - 1) / kc, std::max(8u, k / 512)}));
     c->mm_kernel = 8;
@@ -2603,9 +2608,16 @@ int yx_add_norm_rows_dev(yx_ctx* c, const float* x, const float* post_w, float p
   }
   int rc = c->set_device();
   if (rc) return rc;
-  const yx::AddNorm a{x, post_w, h, h_out, w, out, post_offset, offset, eps};
+  yx::AddNorm a{x, post_w, h, h_out, w, out, post_offset, offset, eps};
   const auto go = [&](auto* kern, int threads) {
-    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(rows)), dim3(threads), 0, c->stream, a, static_cast<uint32_t>(cols));
+    for (size_t r = 0; r < rows; r += kLaunchRows) {
+      const size_t now = std::min(kLaunchRows, rows - r);
+      hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(now)), dim3(threads), 0, c->stream, a, static_cast<uint32_t>(cols));
+      for (const float** p : {&a.x, &a.h})
+        if (*p) *p += now * cols;
+      for (float** p : {&a.h_out, &a.out})
+        if (*p) *p += now * cols;
+    }
   };
   if (cols <= 1024) go(yx::add_norm_rows<256, 1>, 256);
   else if (cols <= 2048) go(yx::add_norm_rows<256, 2>, 256);
@@ -2678,12 +2690,16 @@ int yx_logprobs_rows_dev(yx_ctx* c, const float* logits, size_t rows, size_t col
   size_t nsl = logprobs_slices(c, rows, quads);
   const size_t per = (quads + nsl - 1) / nsl;
   nsl = (quads + per - 1) / per;  // none of them empty
-  hipLaunchKernelGGL(yx::logprobs_rows, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(nsl)),
-                     dim3(yx::kLpThreads), 0, c->stream, logits, static_cast<uint32_t>(cols), ld, tokens,
-                     static_cast<uint32_t>(given), static_cast<uint32_t>(top),
-                     yx::LogprobsOut{logprob, entropy, top_ids, top_logprobs}, static_cast<uint32_t>(per),
-                     static_cast<unsigned long long*>(c->lp_keys.p), static_cast<float*>(c->lp_parts.p),
-                     static_cast<uint32_t*>(c->lp_counters.p));
+  for (size_t r = 0; r < rows; r += kLaunchRows) {  // (rows in slices are far fewer than a launch's)
+    hipLaunchKernelGGL(yx::logprobs_rows, dim3(static_cast<unsigned>(std::min(kLaunchRows, rows - r)), static_cast<unsigned>(nsl)),
+                       dim3(yx::kLpThreads), 0, c->stream, logits + r * ld, static_cast<uint32_t>(cols), ld,
+                       given ? tokens + r * given : nullptr, static_cast<uint32_t>(given), static_cast<uint32_t>(top),
+                       yx::LogprobsOut{logprob ? logprob + r * given : nullptr, entropy ? entropy + r : nullptr,
+                                       top ? top_ids + r * top : nullptr, top ? top_logprobs + r * top : nullptr},
+                       static_cast<uint32_t>(per),
+                       static_cast<unsigned long long*>(c->lp_keys.p), static_cast<float*>(c->lp_parts.p),
+                       static_cast<uint32_t*>(c->lp_counters.p));
+  }
   YX_HIP(hipGetLastError());
   return YX_OK;
 }
