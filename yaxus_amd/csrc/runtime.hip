@@ -1792,9 +1792,9 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
 // matmul_bf16_stream is faster where a row's k is short (gated, k 1024, n 8192 8.4 / 10.8; k 2048
 // 19.4 / 17.7). The number of rows does not decide up to 16: a row's bits stay the same.
 template <class E>
-bool matmul_few_faster(uint32_t t, uint32_t k, uint32_t n) {
+bool matmul_few_faster(const yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
   constexpr uint32_t W = E::kGated ? 2 : 1;
-  if (t <= 16 && k < 2048 && k % 256 == 0 && k >= 1024) return false;
+  if (t <= 16 && (k == 1024 || k == 1536) && W * ((n + 15) / 16) >= 2 * static_cast<uint32_t>(c->cus)) return false;
   return t <= 32 && k <= (1u << 20) && n >= 2048 * W && static_cast<uint64_t>(W) * n * k * 2 >= 12000000ull * W;
 }
 
@@ -1836,7 +1836,7 @@ int matmul_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32
   const size_t tiles16 = static_cast<size_t>((n + 15) / 16) * ((t + 15) / 16);
   const size_t slots = static_cast<size_t>(c->cus);
   if constexpr (E::kFused)
-    if (c->matmul_k_split == 0 && matmul_few_faster<E>(t, k, n)) return matmul_few(c, x, w, out, t, k, n, epi);
+    if (c->matmul_k_split == 0 && matmul_few_faster<E>(c, t, k, n)) return matmul_few(c, x, w, out, t, k, n, epi);
   if (c->matmul_k_split == 0 && W * tiles16 >= 2 * slots) {
     if (t <= 16) {
       if (matmul_stream(c, x, w, out, t, k, n, epi)) {
