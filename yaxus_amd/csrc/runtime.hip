@@ -1652,10 +1652,10 @@ MatmulSplit matmul_tile_split(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
 // CUs idle in a round, all stages may be dealt out evenly in runs. Then up to two tiles of a
 // workgroup are shared, and each costs writing it through (about 20 GB/s a CU) and 2 us, and its
 // last workgroup reading the others' parts. (us, estimated and measured, whole tiles or parts / runs:
-// 1000 x 2048 x 12000 164 and 144 / 142 and 131, 3000 x
-// 1000 x 3000 85 and 86 / 72 and 72; 64 x 2048 x 11024 23 and 21 / 25 and 23.) Tiles of 96 rows save
-// up to a quarter of the products: 80 x 2048 x 11024 30.0 -> 26.7, 190 x 2048 x 16384 48 -> 43, 180 x
-// 4096 x 4096 32.6 -> 28.5, 90 x 704 x 18000 21.5 -> 18.0.
+// 1000 x 2048 x 12000 164 and 144 / 142 and 131, 3000 x 1000 x 3000 85 and 86 / 72 and 72, 64 x 2048
+// x 11024 23 and 21 / 25 and 23.) Tiles of 96 rows save up to a quarter of the products (us, without
+// and with them: 80 x 2048 x 11024 30.0 and 26.7, 190 x 2048 x 16384 48 and 43, 180 x 4096 x 4096
+// 32.6 and 28.5, 90 x 704 x 18000 21.5 and 18.0).
 MatmulSplit matmul_tile_runs(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
   MatmulSplit best{0, 1, 1e30};
   for (int s = 0; s < 5; ++s) {
