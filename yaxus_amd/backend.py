@@ -364,16 +364,17 @@ class HipBackend:
         post_w where given, else x; h' = h + u where h is given, else u; out = norm(h') with w
         where given. norm(v) = v / sqrt(mean(v^2) + eps) * (offset + weight). x and h
         `[rows][cols]`, weights `[cols]`, f32. ``h_out`` (h' stored) and ``out`` may each be x or
-        h itself. Returns (h_out, out); h_out is made where h or post_w is given and it is not,
-        out where w is."""
+        h itself. Returns (h_out, out). A call with ``out`` and without ``h_out`` does not store
+        h' (None) and makes no buffer; without ``out``, out is made where w is given, and h_out
+        where it is not given and h or post_w is, or w is not."""
         rows, cols = x.shape
         b = rows * cols * 4
-        if w is not None and out is None:
-            out = self.tensor((rows, cols))
         if w is None and out is not None:
             raise ValueError("out needs the norm's weight w")
-        if h_out is None and (w is None or h is not None or post_w is not None):
+        if out is None and h_out is None and (w is None or h is not None or post_w is not None):
             h_out = self.tensor((rows, cols))
+        if w is not None and out is None:
+            out = self.tensor((rows, cols))
         for v, need, what in ((x, b, "x"), (h, b, "h"), (h_out, b, "h_out"), (out, b, "out"),
                               (w, cols * 4, "w"), (post_w, cols * 4, "post_w")):
             if v is not None:
