@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from tests.test_gpu_add_norm import inputs, want64
+from tests.test_gpu_logprobs import logits, some
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +30,23 @@ def test_add_norm_without_storing_the_sum(hip, monkeypatch, rows, cols, post, ad
     finally:
         for t in made:
             t.free()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 151936), (5, 9000), (700, 333)])
+def test_logprobs_without_the_entropy(hip, rows, cols):
+    """Outputs of None leave the others with the bits of the whole call."""
+    x, t = logits(rows, cols), some(rows, cols)
+    dx, dt = hip.tensor(x.shape).upload(x), hip.tensor(t.shape, np.uint32).upload(t.astype(np.uint32))
+    whole = hip.logprobs_rows(dx, tokens=dt, top=6)
+    fresh = lambda o: hip.tensor(o.shape, o.dtype).upload(np.zeros(o.shape, o.dtype))
+    made = [dx, dt, *whole]
+    try:
+        for keep in ((0, 2, 3), (0,), (1,), (2, 3)):
+            out = [fresh(o) if i in keep else None for i, o in enumerate(whole)]
+            made += [o for o in out if o]
+            hip.logprobs_rows(dx, tokens=dt if 0 in keep else None, top=6 if 2 in keep else 0, out=out)
+            for i in keep:
+                np.testing.assert_array_equal(out[i].numpy().view(np.uint32), whole[i].numpy().view(np.uint32))
+    finally:
+        for v in made:
+            v.free()

@@ -60,3 +60,27 @@ def test_add_norm_makes_what_the_caller_left_to_it(hip, given, made):
         assert out is rows.get("out")
     # The library gets null for what is not stored.
     assert (hip.L.args[5] is None) == (h_out is None) and (hip.L.args[8] is None) == (out is None)
+
+
+@pytest.mark.parametrize("given,top,outs", [
+    (1, 5, (True, False, True, True)),
+    (2, 0, (True, False, False, False)),
+    (0, 0, (False, True, False, False)),
+    (0, 3, (False, False, True, True)),
+    (1, 5, (True, True, True, True)),
+])
+def test_logprobs_takes_no_buffer_for_what_is_not_computed(hip, given, top, outs):
+    made = [Operand(4, 8) if o else None for o in outs]
+    got = hip.logprobs_rows(Operand(4, 100), tokens=Operand(4, given) if given else None, top=top, out=made)
+    assert got is made and not hip.made
+    for o, arg in zip(made, hip.L.args[8:]):
+        assert arg is (o.ptr if o else None)
+
+
+@pytest.mark.parametrize("missing,words", [(0, "logprob: asked"), (2, "top_ids: asked"), (3, "top_logprobs: asked")])
+def test_logprobs_refuses_without_a_buffer_it_needs(hip, missing, words):
+    outs = [Operand(4, 8) for _ in range(4)]
+    outs[missing] = outs[1] = None
+    with pytest.raises(ValueError, match=words):
+        hip.logprobs_rows(Operand(4, 100), tokens=Operand(4, 2), top=5, out=outs)
+    assert hip.L.args is None

@@ -388,7 +388,8 @@ class HipBackend:
         """Log probabilities, entropy and top alternatives of rows of logits
         (yx_logprobs_rows_dev). logits `[rows][ld]` f32, of each row the first ``cols`` (default:
         all) are the vocabulary; tokens `[rows][given]` (or `[rows]`) uint32. Returns
-        ``LogProbs``; ``out`` is four device tensors to use instead of new ones."""
+        ``LogProbs``; ``out`` is four device tensors to use instead of new ones, None for what is
+        not computed: the entropy, logprob without tokens, both of the alternatives with top 0."""
         rows, ld = logits.shape
         cols = ld if cols is None else cols
         given = 0 if tokens is None else tokens.shape[1] if len(tokens.shape) > 1 else 1
@@ -401,14 +402,17 @@ class HipBackend:
         _need(logits, rows * ld * 4, "logits")
         if given:
             _need(tokens, rows * given * 4, "tokens")
-            _need(lp, rows * given * 4, "logprob")
-        _need(entropy, rows * 4, "entropy")
-        if top:
-            _need(ids, rows * top * 4, "top_ids")
-            _need(tlp, rows * top * 4, "top_logprobs")
+        for v, each, what in ((lp, given, "logprob"), (entropy, 1, "entropy"), (ids, top, "top_ids"),
+                              (tlp, top, "top_logprobs")):
+            if v is None:
+                if each and what != "entropy":
+                    raise ValueError(f"{what}: asked for without a buffer")
+            else:
+                _need(v, rows * each * 4, what)
         check_hip(self.L.yx_logprobs_rows_dev(self.ctx, logits.ptr, rows, cols, ld,
-                                              tokens.ptr if given else None, given, top, lp.ptr,
-                                              entropy.ptr, ids.ptr, tlp.ptr))
+                                              tokens.ptr if given else None, given, top,
+                                              lp and lp.ptr, entropy and entropy.ptr, ids and ids.ptr,
+                                              tlp and tlp.ptr))
         return out
 
     def stat(self, key):
