@@ -62,13 +62,15 @@ __global__ __launch_bounds__(kFewThreads, 4) void matmul_bf16_few(
   for (int a = 0; a < NT; ++a)
     wo[a] = ((E::kGated ? wave : wave * NT + a) * 16 + c) * static_cast<int>(k) * 2 + 16 * g;
   u16x8 wv[STEPS][NT];
+  // (A resource's range counts from its scalar offset, so that stays inside it where nothing is
+  // read too: k - 8 is the last piece of a row.)
   const auto load_w = [&](int s, uint32_t ch) {  // past this part: zeros, nothing read
-    const uint32_t kb = ch * KC + s * 32;
+    const uint32_t kb = ch * KC + s * 32, at = min(kb, k - 8) * 2;
     const bool ok = (ch < c1) & (kb + 8 * g < k);
 #pragma unroll
     for (int a = 0; a < NT; ++a)
       wv[s][a] = __builtin_bit_cast(
-          u16x8, __builtin_amdgcn_raw_buffer_load_b128(E::kGated && a ? ru : rw, ok ? wo[a] : kOutside, kb * 2, 0));
+          u16x8, __builtin_amdgcn_raw_buffer_load_b128(E::kGated && a ? ru : rw, ok ? wo[a] : kOutside, at, 0));
   };
 
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(const_cast<float*>(x), t * k * 4);  // rows past t: zeros
@@ -85,13 +87,13 @@ __global__ __launch_bounds__(kFewThreads, 4) void matmul_bf16_few(
     f32x4 a[XC], b[XC];
   };
   const auto load_x = [&](XRegs& r, uint32_t ch) {
-    const uint32_t kb = ch * KC;
+    const uint32_t kb = ch * KC, at = min(kb, k - 8) * 4;
 #pragma unroll
     for (int i = 0; i < XC; ++i) {
       const bool ok = (ch < c1) & (kb + xk[i] < k);
       const int o = ok ? xo[i] : kOutside;
-      r.a[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, o, kb * 4, 0));
-      r.b[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, o, kb * 4 + 16, 0));
+      r.a[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, o, at, 0));
+      r.b[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, o, at + 16, 0));
     }
   };
   const auto write_x = [&](const XRegs& r, int slot) {
