@@ -34,3 +34,14 @@ def test_few_rows_and_a_last_group_of_one_column(hip, t, k, n, gated):
     """One row of the weight, or of x, is all that a resource holds, and k ends inside a chunk."""
     check(hip, t, k, n, gated)
     assert hip.stat("matmul_kernel") == FEW
+
+
+@pytest.mark.parametrize("t,k,n,gated,kernel", [
+    (16, 1024, 8192, False, STREAM), (7, 1024, 4081, True, STREAM), (16, 1536, 8200, False, STREAM), (1, 1536, 4096, True, STREAM),
+    (16, 2048, 4088, True, STREAM), (7, 2560, 4081, True, STREAM), (1, 2560, 4096, True, FEW), (16, 2048, 8192, False, FEW), (16, 2560, 8207, False, FEW),
+    (16, 4096, 2048, False, FEW), (16, 4096, 2047, False, ROWS), (16, 2048, 4080, True, ROWS), (16, 8192, 2032, False, ROWS), (16, 8192, 4000, True, ROWS),
+    (33, 9000, 2100, False, ROWS),
+])
+def test_few_rows(hip, t, k, n, gated, kernel):
+    check(hip, t, k, n, gated)
+    assert hip.stat("matmul_kernel") == kernel

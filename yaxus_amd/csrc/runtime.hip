@@ -1587,10 +1587,12 @@ bool matmul_stream(yx_ctx* c, const float* x, const uint16_t* w, float* out, uin
   switch (k / 256) {
     case 4: return go(yx::matmul_bf16_stream<4, E>);
     case 6: return go(yx::matmul_bf16_stream<6, E>);
-    case 8: return go(yx::matmul_bf16_stream<8, E>);
-    case 10: return go(yx::matmul_bf16_stream<10, E>);
-    default: return false;
   }
+  if constexpr (!E::kFused || E::kGated) {  // else matmul_bf16_few has taken them (matmul_few_faster)
+    if (k / 256 == 8) return go(yx::matmul_bf16_stream<8, E>);
+    if (k / 256 == 10) return go(yx::matmul_bf16_stream<10, E>);
+  }
+  return false;
 }
 
 // The shapes of matmul_bf16_tiles; the last only with an epilogue.
@@ -1770,7 +1772,8 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
       case 1: go(yx::matmul_bf16_tiles<yx::MatmulTileB, E, kRuns>); break;
       case 2: go(yx::matmul_bf16_tiles<yx::MatmulTileC, E, kRuns>); break;
       case 3: go(yx::matmul_bf16_tiles<D, E, kRuns>); break;
-      default: go(yx::matmul_bf16_tiles<yx::MatmulTileF, E, kRuns>); break;
+      default:
+        if constexpr (E::kFused) go(yx::matmul_bf16_tiles<yx::MatmulTileF, E, kRuns>);
     }
   };
   if constexpr (E::kFused) {
@@ -1790,7 +1793,9 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
 // n 2048 7.3 / 7.4, n 4096 11.1 / 8.0; k 8192, n 1024 11.8 / 14.0, n 2048 17.4 / 13.1; gated k
 // 2048, n 2048 8.7 / 10.2, n 4096 13.9 / 11.9; k 512, n 8192 7.9 / 8.4, n 16000 13.3 / 11.0), and
 // matmul_bf16_stream is faster where a row's k is short (gated, k 1024, n 8192 8.4 / 10.8; k 2048
-// 19.4 / 17.7). The number of rows does not decide up to 16: a row's bits stay the same.
+// 19.4 / 17.7; of k 2048 and 2560 it keeps gated products of 4081 to 4095 columns, 16 x 2048 x 4088
+// 12.3 / 13.4, 16 x 2560 x 4081 12.9 / 18.2, weights from HBM). The number of rows does not decide
+// up to 16: a row's bits stay the same.
 template <class E>
 bool matmul_few_faster(const yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
   constexpr uint32_t W = E::kGated ? 2 : 1;
