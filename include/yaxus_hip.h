@@ -99,8 +99,10 @@ int yx_ctx_set_option(yx_ctx* ctx, const char* key, long value);
  * the items, of all heads, of the latest list of decode items. And of its
  * latest yx_matmul_bf16_dev or yx_linear_bf16_dev: "matmul_kernel" (0 none yet, 1 the kernel of 16 x 16 tiles, 2 the
  * one that streams the weight, 3 to 6 LDS tiles of 128 x 256, 128 x 128, 64 x 128, 64 x 64; of
- * yx_linear_bf16_dev also 7, tiles of 96 x 128, and 8, the kernel of few rows) and "matmul_k_parts"
- * (the workgroups of a tile along k, at most).
+ * yx_linear_bf16_dev also 7, tiles of 96 x 128, and 8, the kernel of few rows), "matmul_k_parts"
+ * (the workgroups of a tile along k, at most) and "matmul_run_stages" (where the stages of all
+ * tiles are dealt out evenly, those of a workgroup; 32 of k each for the tiles 3 and 4, 64 for the
+ * others; else 0).
  * A pass whose groups keep their order and fit the device regions of the previous pass
  * sends only the entries that changed. */
 int yx_ctx_get_stat(yx_ctx* ctx, const char* key, uint64_t* out);

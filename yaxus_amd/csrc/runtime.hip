@@ -361,7 +361,7 @@ struct yx_ctx {
   // Rows of logits read in slices: the slices' sums and keys and the rows' arrival counters,
   // for logprobs_slots slices in all, allocated with the context too.
   DevBuf lp_keys, lp_parts, lp_counters;
-  uint64_t mm_kernel = 0, mm_k_parts = 0;  // what the latest matmul ran (tests)
+  uint64_t mm_kernel = 0, mm_k_parts = 0, mm_run_stages = 0;  // what the latest matmul ran (tests)
   // options
   long target_waves = 0;  // 0: one work item per CU
   int cus = 256;
@@ -1754,6 +1754,7 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
   const MatmulShape& sh = kMatmulShapes[split.shape];
   c->mm_kernel = 3 + static_cast<uint64_t>(split.shape);
   c->mm_k_parts = split.ks;
+  c->mm_run_stages = split.per;
   const size_t cols = E::kGated ? sh.tn / 2 : sh.tn;
   const size_t tiles = ((t + sh.tm - 1) / sh.tm) * ((n + cols - 1) / cols);
   if (tiles > 0x7fffffff) return fail(YX_ERR_UNSUPPORTED, "matmul dimensions too large");
@@ -1840,6 +1841,7 @@ int matmul_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32
   const size_t steps = (static_cast<size_t>(k) + 31) / 32;
   const size_t tiles16 = static_cast<size_t>((n + 15) / 16) * ((t + 15) / 16);
   const size_t slots = static_cast<size_t>(c->cus);
+  c->mm_run_stages = 0;
   if constexpr (E::kFused)
     if (c->matmul_k_split == 0 && matmul_few_faster<E>(c, t, k, n)) return matmul_few(c, x, w, out, t, k, n, epi);
   if (c->matmul_k_split == 0 && W * tiles16 >= 2 * slots) {
@@ -2341,6 +2343,8 @@ int yx_ctx_get_stat(yx_ctx* c, const char* key, uint64_t* out) {
     *out = c->mm_kernel;
   else if (!std::strcmp(key, "matmul_k_parts"))
     *out = c->mm_k_parts;
+  else if (!std::strcmp(key, "matmul_run_stages"))
+    *out = c->mm_run_stages;
   else
     return fail(YX_ERR_INVALID, std::string("unknown statistic ") + key);
   return YX_OK;
