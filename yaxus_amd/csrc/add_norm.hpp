@@ -103,7 +103,9 @@ __global__ __launch_bounds__(TH) void add_norm_rows(AddNorm a, uint32_t cols) {
 
 static constexpr int kNormLongThreads = 1024;
 
-// The same for rows of any length, which are read again after each sum.
+// The same for rows of any length, which are read again after each sum, in 4-byte accesses. 2048 x
+// 20000 with an addition 182 us, 3.6 TB/s of the values read and written once (16384 columns in
+// registers 105, 5.1); 16 x 20000 12.
 __global__ __launch_bounds__(kNormLongThreads) void add_norm_long_rows(AddNorm a, uint32_t cols) {
   __shared__ float ws[kNormLongThreads / 64];
   const size_t base = static_cast<size_t>(blockIdx.x) * cols;

@@ -71,8 +71,7 @@ __device__ __forceinline__ void split_bf16x3(float f0, float f1, uint32_t& h, ui
 // their tiles over as matmul_bf16_rows does.
 // kRuns: workgroups are not tied to tiles. The stages of all tiles, one tile's after the other's,
 // are dealt out in runs of `per`, so few tiles, or a few more than fill the GPU once, load all CUs
-// alike (1000 x 2048 x 12000 144 -> 131 us, 3000 x 1000 x 3000 86 -> 72, 333 x 4096 x 11008 118 ->
-// 96). A run may end one tile, do whole ones and begin another; a tile of several workgroups is
+// alike (333 x 4096 x 11008 145 -> 102 us, 1360 x 2736 x 3504 109 -> 89, weights from HBM). A run may end one tile, do whole ones and begin another; a tile of several workgroups is
 // joined in k order by the last of them to arrive, which adds its own part from its registers. At
 // most the first and the last tile of a run are shared, so scratch is two tiles per workgroup, and
 // a shared tile's counter is that of its first workgroup. Where every workgroup has one tile

@@ -14,8 +14,8 @@
 // Layouts as in step_after.hpp (A: 16 weight rows, B: 16 rows of a part of x).
 // With ks > 1 (grid y) the workgroups of a column group take consecutive chunks of k and hand
 // their tiles over as matmul_bf16_rows does.
-// Measured, 16 rows: k 2048, n 8192 gated (67 MB) 17.7 us, k 8192, n 2048 13.1 (33.5 MB), k 4096,
-// n 14336 gated 51 (4.6 TB/s), k 8192, n 16000 gated 104 (5.1 TB/s). Tried: a wave streaming
+// Measured, 16 rows, weights from HBM: k 2048, n 8192 gated (67 MB) 17.7 us, k 8192, n 2048 14.1 (33.5
+// MB), k 4096, n 14336 gated 52 (4.6 TB/s), k 8192, n 16000 gated 104 (5.1 TB/s). Tried: a wave streaming
 // tiles past x in registers (16 rows of 2 KiB at a time, no LDS) 100 us for the last, but 18-29%
 // slower up to 34 MB, where each part of x is cut up for too few tiles.
 #pragma once

@@ -1653,9 +1653,10 @@ MatmulSplit matmul_tile_split(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
 // The same with an epilogue, where a tile's parts may be any number up to 8, and, where that leaves
 // CUs idle in a round, all stages may be dealt out evenly in runs. Then up to two tiles of a
 // workgroup are shared, and each costs writing it through (about 20 GB/s a CU) and 2 us, and its
-// last workgroup reading the others' parts. (us, estimated and measured, whole tiles or parts / runs:
-// 1000 x 2048 x 12000 164 and 144 / 142 and 131, 3000 x 1000 x 3000 85 and 86 / 72 and 72, 64 x 2048
-// x 11024 23 and 21 / 25 and 23.) Tiles of 96 rows save up to a quarter of the products (us, without
+// last workgroup reading the others' parts. (us, weights from HBM, whole tiles or parts / runs: 333 x
+// 4096 x 11008 145 / 102, 1360 x 2736 x 3504 109 / 89, 145 x 1648 x 12427 gated 69 / 64, 1000 x 2048 x
+// 12000 169 / 164; not the fastest: 1234 x 1464 x 3328 57.7 / 60, gated 1045 x 1696 x 6080 118 / 130
+// and 700 x 4096 x 4100 123 / 138.) Tiles of 96 rows save up to a quarter of the products (us, without
 // and with them: 80 x 2048 x 11024 30.0 and 26.7, 190 x 2048 x 16384 48 and 43, 180 x 4096 x 4096
 // 32.6 and 28.5, 90 x 704 x 18000 21.5 and 18.0).
 MatmulSplit matmul_tile_runs(yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
@@ -1790,13 +1791,14 @@ int matmul_tiled(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint3
 }
 
 // Whether matmul_bf16_few takes a product of at most 32 rows: much weight in many rows. On the
-// other side matmul_bf16_rows starts sooner and hands over less (us, 16 rows, that / few: k 2048,
-// n 2048 7.3 / 7.4, n 4096 11.1 / 8.0; k 8192, n 1024 11.8 / 14.0, n 2048 17.4 / 13.1; gated k
-// 2048, n 2048 8.7 / 10.2, n 4096 13.9 / 11.9; k 512, n 8192 7.9 / 8.4, n 16000 13.3 / 11.0), and
-// matmul_bf16_stream is faster where a row's k is short (gated, k 1024, n 8192 8.4 / 10.8; k 2048
-// 19.4 / 17.7; of k 2048 and 2560 it keeps gated products of 4081 to 4095 columns, 16 x 2048 x 4088
-// 12.3 / 13.4, 16 x 2560 x 4081 12.9 / 18.2, weights from HBM). The number of rows does not decide
-// up to 16: a row's bits stay the same.
+// other side matmul_bf16_rows starts sooner and hands over less (us, 16 rows, weights from HBM, that
+// / few: k 2048, n 2048 7.3 / 7.8, n 4096 11.1 / 8.8; k 8192, n 1024 11.9 / 11.9, n 2048 17.5 / 14.1;
+// k 512, n 8192 6.5 / 6.3, n 16000 9.9 / 7.8; gated k 2048, n 2048 8.9 / 11.1; k 4096, n 2048 14.2 /
+// 15.8; not the fastest: gated k 7168, n 2048 23.2 / 19.9, k 8192, n 4000 46 / 32), and
+// matmul_bf16_stream is faster where a row's k is short (gated, k 1024, n 8192 9.0 / 11.6; k 2048, n
+// 4096 14.2 / 14.2, n 8192 19.4 / 17.7; of k 2048 and 2560 it keeps gated products of 4081 to 4095
+// columns, 16 x 2048 x 4088 12.3 / 13.4, 16 x 2560 x 4081 12.9 / 18.2). 32 x 2048 x 8192 16.1 by tiles,
+// 12.9. The number of rows does not decide up to 16: a row's bits stay the same.
 template <class E>
 bool matmul_few_faster(const yx_ctx* c, uint32_t t, uint32_t k, uint32_t n) {
   constexpr uint32_t W = E::kGated ? 2 : 1;
@@ -1833,7 +1835,10 @@ int matmul_few(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_
 }
 
 // A product whose arguments are checked: the kernel for its sizes. What decides are the weight's
-// rows (two per output column where the epilogue is gated).
+// rows (two per output column where the epilogue is gated). Below two 16 x 16 tiles per CU
+// matmul_bf16_rows (us, with an epilogue, that / tiles: 24 x 2048 x 2048 10.0 / 11.1, 100 x 2048 x 512
+// 9.7 / 10.4; where few tiles meet a longer k it is not the fastest, 48 x 2048 x 2048 12.8 / 11.3,
+// 40 x 4096 x 2048 20.7 / 13.8, 40 x 8192 x 2048 36.4 / 19.0).
 template <class E>
 int matmul_impl(yx_ctx* c, const float* x, const uint16_t* w, float* out, uint32_t t, uint32_t k, uint32_t n,
                 const E& epi) {
