@@ -75,6 +75,8 @@ unsafe extern "C" {
                         v: *const f32) -> c_int;
     pub fn yx_kv_append_dev(ctx: *mut yx_ctx, kv: *mut yx_kv, layer: usize, k: *const f32,
                             v: *const f32) -> c_int;
+    pub fn yx_kv_rows_dev(ctx: *mut yx_ctx, kv: *mut yx_kv, layer: usize, k_out: *mut f32,
+                          v_out: *mut f32) -> c_int;
 
     pub fn yx_qk_rope_append_dev(ctx: *mut yx_ctx, kv: *mut yx_kv, layer: usize, qkv: *const f32,
                                  q_norm: *const f32, k_norm: *const f32, rope_cs: *const f32,

@@ -39,7 +39,7 @@ extern "C" {
 typedef struct yx_ctx yx_ctx;
 typedef struct yx_kv yx_kv;
 
-enum { YX_DTYPE_F32 = 0, YX_DTYPE_F16 = 1 };
+enum { YX_DTYPE_F32 = 0, YX_DTYPE_F16 = 1, YX_DTYPE_Q4 = 2 };
 enum { YX_K = 0, YX_V = 1 };
 /* Activations of yx_linear_bf16_dev; gelu with the error function, or its tanh form. */
 enum { YX_ACT_NONE = 0, YX_ACT_RELU = 1, YX_ACT_SILU = 2, YX_ACT_GELU = 3, YX_ACT_GELU_TANH = 4 };
@@ -114,7 +114,9 @@ int yx_ctx_get_stat(yx_ctx* ctx, const char* key, uint64_t* out);
  * f32 MFMAs, or prefill tiles of 128 or 64 (the 128 on exact bf16 parts of the f32 values,
  * except where those would not do), chosen as the options prefill_min_rows and
  * prefill_f32_waves of yx_ctx_set_option describe;
- * at most 16 q heads per KV head; write_rows as its own launch). */
+ * at most 16 q heads per KV head; write_rows as its own launch) or YX_DTYPE_Q4 (no counterpart
+ * in the reference: 72 bytes per head vector, see yx_kv_rows_dev for what it keeps; attention at
+ * f32's precision on the values it holds, write_rows as its own launch). */
 int yx_kv_create(yx_ctx* ctx, size_t layers, size_t pages, size_t page_size, size_t hkv,
                  size_t head_dim, int dtype, yx_kv** out);
 int yx_kv_destroy(yx_ctx* ctx, yx_kv* kv);
@@ -127,7 +129,8 @@ size_t yx_kv_page_bytes(const yx_kv* kv);
 int yx_kv_copy_pages(yx_ctx* ctx, yx_kv* kv, const uint32_t* src, const uint32_t* dst, size_t n);
 
 /* Raw page contents, `[n][hkv][page_size][128]` binary16 bits (f32 bits for an f32
- * arena), synchronous. */
+ * arena), synchronous. Of a 4-bit arena `[n][hkv][page_size][72]` bytes: 64 of codes, two dims a
+ * byte, the lower dim in the low half, then the four steps (binary16 bits). */
 int yx_kv_read_pages(yx_ctx* ctx, yx_kv* kv, size_t layer, const uint32_t* pages, size_t n,
                      void* k_out, void* v_out);
 int yx_kv_write_pages(yx_ctx* ctx, yx_kv* kv, size_t layer, const uint32_t* pages, size_t n,
@@ -147,6 +150,17 @@ int yx_pass_begin(yx_ctx* ctx, size_t rows, const uint32_t* pos, const uint32_t*
  * to binary16 (nearest-even) and scattered to each row's kv_slot of `layer`. */
 int yx_kv_append(yx_ctx* ctx, yx_kv* kv, size_t layer, const float* k, const float* v);
 int yx_kv_append_dev(yx_ctx* ctx, yx_kv* kv, size_t layer, const float* k, const float* v);
+
+/* What the arena holds of the pass's rows, as f32 `[rows][hkv][128]` each (device pointers,
+ * 16-byte aligned; either may be null): the K and V that attention sees at the rows' slots.
+ * An f32 arena holds what was stored, a binary16 one that rounded. A 4-bit one, of every 32
+ * consecutive values of a head: with m the one of the largest magnitude (the first of equals),
+ * the step s = m / -8 rounded to binary16 (at most 65504 in magnitude), a value x is kept as
+ * s * n, n = x / s rounded to the nearest whole number (ties to even) and limited to -8 .. 7:
+ * where 2^-11 <= |m| <= 524032 within |m| / 16 of x, |m| / 8 where x lies opposite m and beyond
+ * 15/16 |m| (both times 1 + 2^-6 at most, the step's rounding); a step of 0 keeps zeros; 32 values
+ * with an infinity or NaN among them all become NaN. */
+int yx_kv_rows_dev(yx_ctx* ctx, yx_kv* kv, size_t layer, float* k_out, float* v_out);
 
 /* write_rows (backend-cpu lib.rs:359-385; QK_ROPE, yaxus-backend-gpu shaders.rs:285-341),
  * device pointers: per row of the pass, qkv `[rows][(hq + 2 hkv) * 128]` f32 holds the

@@ -21,6 +21,7 @@ YX_ERR_UNSUPPORTED = 6
 
 YX_DTYPE_F32 = 0
 YX_DTYPE_F16 = 1
+YX_DTYPE_Q4 = 2
 YX_K = 0
 YX_V = 1
 YX_ACT_NONE = 0
@@ -89,6 +90,7 @@ HIP_SYMBOLS = {
     "yx_pass_begin": (I, [P, S, P, P, P, P, S]),
     "yx_kv_append": (I, [P, P, S, P, P]),
     "yx_kv_append_dev": (I, [P, P, S, P, P]),
+    "yx_kv_rows_dev": (I, [P, P, S, P, P]),
     "yx_qk_rope_append_dev": (I, [P, P, S, P, P, P, P, S, F, S, S, P]),
     "yx_attention_qkv_dev": (I, [P, P, S, P, P, P, P, S, F, P, S, S, S, F]),
     "yx_attention": (I, [P, P, S, P, P, S, S, S, F]),

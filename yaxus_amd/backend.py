@@ -79,14 +79,15 @@ class DeviceTensor:
 
 
 class Kv:
-    """The arena of one model: ``layers`` layers of ``pages`` pages (binary16 K/V, or
-    f32 with ``f32=True``)."""
+    """The arena of one model: ``layers`` layers of ``pages`` pages (binary16 K/V, f32 with
+    ``f32=True`` or 4-bit with ``q4=True``)."""
 
-    def __init__(self, backend, handle, layers, pages, page, hkv, d, f32=False):
+    def __init__(self, backend, handle, layers, pages, page, hkv, d, f32=False, q4=False):
         self.backend, self.h = backend, handle
         self.layers, self.pages, self.page, self.hkv, self.d = layers, pages, page, hkv, d
-        self.f32 = f32
-        self.bits = np.uint32 if f32 else np.uint16
+        self.f32, self.q4 = f32, q4
+        self.bits = np.uint32 if f32 else np.uint8 if q4 else np.uint16
+        self.row = 72 if q4 else d  # entries of a head vector in read_pages and write_pages
 
     def layer_ptr(self, layer, which):
         p = ctypes.c_void_p()
@@ -98,9 +99,10 @@ class Kv:
         return self.backend.L.yx_kv_page_bytes(self.h)
 
     def read_pages(self, layer, pages):
-        """(K, V) bits of the pages, each ``[n][hkv][page][d]`` uint16 (uint32 for f32)."""
+        """(K, V) bits of the pages, each ``[n][hkv][page][d]`` uint16 (uint32 for f32; of a
+        4-bit arena ``[n][hkv][page][72]`` uint8, codes then steps, see yx_kv_read_pages)."""
         pg = np.ascontiguousarray(pages, dtype=np.uint32)
-        k = np.empty((len(pg), self.hkv, self.page, self.d), self.bits)
+        k = np.empty((len(pg), self.hkv, self.page, self.row), self.bits)
         v = np.empty_like(k)
         check_hip(self.backend.L.yx_kv_read_pages(self.backend.ctx, self.h, layer, ptr(pg),
                                                   len(pg), ptr(k), ptr(v)))
@@ -109,9 +111,9 @@ class Kv:
     def write_pages(self, layer, pages, k, v):
         pg = np.ascontiguousarray(pages, dtype=np.uint32)
         k, v = self._as_bits(k), self._as_bits(v)
-        n = len(pg) * self.hkv * self.page * self.d
+        n = len(pg) * self.hkv * self.page * self.row
         if k.size != n or v.size != n:
-            raise ValueError("k/v must be [n][hkv][page][d] of the arena's dtype")
+            raise ValueError(f"k/v must be [n][hkv][page][{72 if self.q4 else 'd'}] of the arena's dtype")
         check_hip(self.backend.L.yx_kv_write_pages(self.backend.ctx, self.h, layer, ptr(pg),
                                                    len(pg), ptr(k), ptr(v)))
 
@@ -153,12 +155,13 @@ class HipBackend:
         return DeviceTensor(self, shape, dtype)
 
     # Backend::new_kv (lib.rs:118)
-    def new_kv(self, layers, pages, page, hkv, d=128, f32=False):
+    def new_kv(self, layers, pages, page, hkv, d=128, f32=False, q4=False):
+        if f32 and q4:
+            raise ValueError("an arena is f32 or 4-bit, not both")
         h = ctypes.c_void_p()
-        check_hip(self.L.yx_kv_create(self.ctx, layers, pages, page, hkv, d,
-                                      _lib.YX_DTYPE_F32 if f32 else _lib.YX_DTYPE_F16,
-                                      ctypes.byref(h)))
-        return Kv(self, h, layers, pages, page, hkv, d, f32)
+        dtype = _lib.YX_DTYPE_F32 if f32 else _lib.YX_DTYPE_Q4 if q4 else _lib.YX_DTYPE_F16
+        check_hip(self.L.yx_kv_create(self.ctx, layers, pages, page, hkv, d, dtype, ctypes.byref(h)))
+        return Kv(self, h, layers, pages, page, hkv, d, f32, q4)
 
     # Backend::copy_page (lib.rs:120), batched in list order
     def copy_pages(self, kv, copies):
@@ -196,6 +199,18 @@ class HipBackend:
         if k.size != self.rows * kv.hkv * kv.d or v.size != k.size:
             raise ValueError("k/v must be [rows][hkv][head_dim] f32")
         check_hip(self.L.yx_kv_append(self.ctx, kv.h, layer, ptr(k), ptr(v)))
+
+    def kv_rows(self, kv, layer, out=None):
+        """What the arena holds of the pass's rows (yx_kv_rows_dev): device tensors (K, V), each
+        ``[rows][hkv][d]`` f32. ``out``: the two to use, None for one that is not wanted."""
+        if out is None:
+            out = tuple(self.tensor((self.rows, kv.hkv, kv.d)) for _ in range(2))
+        k, v = out
+        for t, what in ((k, "k out"), (v, "v out")):
+            if t is not None:
+                _need(t, self.rows * kv.hkv * kv.d * 4, what)
+        check_hip(self.L.yx_kv_rows_dev(self.ctx, kv.h, layer, k and k.ptr, v and v.ptr))
+        return out
 
     # write_rows (backend-cpu lib.rs:359-385): q/k RMSNorm + RoPE of the pass's rows, K/V
     # stored at their slots; returns q. qkv `[rows][(hq + 2 hkv) * d]`, q_norm/k_norm

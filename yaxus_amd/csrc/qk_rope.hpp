@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include "kv_kernels.hpp"
+#include "q4.hpp"
 
 namespace yx {
 
@@ -101,7 +102,7 @@ __device__ __forceinline__ void store_kv_head(float k0, float k1, const float* _
 static constexpr int kRopeVecs = 16;  // 16: 18.0 us at 4096 rows; 32: 19.1; 64: 24.6
 static constexpr int kRopeThreads = 256;
 
-// T: the arena's element type (_Float16 or float).
+// T: the arena's element type (_Float16, float or q4_t).
 template <typename T>
 __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_append(
     const float* __restrict__ qkv, const float* __restrict__ q_norm,

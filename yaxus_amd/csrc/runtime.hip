@@ -19,10 +19,12 @@
 #include "attn_decode.hpp"
 #include "attn_prefill.hpp"
 #include "attn_prefill_f32.hpp"
+#include "attn_q4.hpp"
 #include "deal.hpp"
 #include "kv_kernels.hpp"
 #include "logprobs.hpp"
 #include "matmul_few.hpp"
+#include "q4.hpp"
 #include "qk_rope.hpp"
 #include "step_after.hpp"
 
@@ -178,6 +180,7 @@ struct AttnPlan {
   bool small_units = false;  // balanced with items of at most 2 * kBalQuads blocks: 2-block units
   bool wide = false;  // 16-row tiles (the wide kernel) instead of 8-row ones
   bool f32 = false;   // the f32-arena kernel
+  bool q4 = false;    // the 4-bit-arena kernels
   int pf32_waves = 8;  // f32 prefill tiles: 8 waves (128 logical rows) or 4 (64)
   std::vector<yx::AttnItem> items;
   DevBuf d_items;
@@ -241,7 +244,7 @@ void* g_scratch_ptr[kMaxDevices] = {};
 // another context first makes its stream wait for the previous user's stream (an event
 // recorded there at the hand-over), so calls on different streams do not overlap on
 // the scratch.
-using PlanKey = std::tuple<size_t, size_t, size_t, bool, size_t>;  // (window, hq, hkv, f32, page)
+using PlanKey = std::tuple<size_t, size_t, size_t, int, size_t>;  // (window, hq, hkv, dtype, page)
 struct ScratchOwner {
   const yx_ctx* ctx = nullptr;
   hipStream_t stream = nullptr;
@@ -294,12 +297,21 @@ struct ScratchMap {
 
 struct yx_kv {
   size_t layers, pages, page, hkv, d;
+  int dtype = YX_DTYPE_F16;
   bool f32 = false;  // f32 K/V (K in V's layout) instead of binary16
-  std::vector<_Float16*> k, v;  // per layer; float* when f32
+  bool q4 = false;   // 4-bit K/V (q4.hpp)
+  std::vector<_Float16*> k, v;  // per layer; float* when f32, q4_t* when q4
   DevBuf bases;  // 2 * layers pointers for the copy kernel
-  size_t page_bytes() const { return hkv * page * d * (f32 ? 4 : 2); }
+  size_t page_bytes() const { return hkv * page * (q4 ? yx::kQ4Row : d * (f32 ? 4 : 2)); }
+  uint32_t page_shift() const {
+    uint32_t s = 0;
+    while ((1u << s) < page) ++s;
+    return s;
+  }
   float* kf(size_t l) const { return reinterpret_cast<float*>(k[l]); }
   float* vf(size_t l) const { return reinterpret_cast<float*>(v[l]); }
+  yx::q4_t* kq(size_t l) const { return reinterpret_cast<yx::q4_t*>(k[l]); }
+  yx::q4_t* vq(size_t l) const { return reinterpret_cast<yx::q4_t*>(v[l]); }
 };
 
 struct yx_ctx {
@@ -323,13 +335,13 @@ struct yx_ctx {
   const uint32_t* dev_slot = nullptr;
   std::vector<uint32_t> region_off, region_cap;  // per group of the previous pass
   std::vector<uint32_t> dev_mirror;              // what d_pages holds, entry by entry
-  std::vector<std::tuple<size_t, size_t, size_t, bool, size_t>> used_keys;  // plans used this pass
+  std::vector<PlanKey> used_keys;  // plans used this pass
   uint64_t pages_sent = 0, runs_sent = 0;        // page-table entries and runs uploaded (tests)
   uint64_t split_tiles = 0;                       // prefill tiles split along keys (tests)
   uint64_t decode_items = 0;                      // items, of all heads, of the latest list of decode items (tests)
   uint64_t prefill_plans = 0;                     // work lists built as prefill tiles (tests)
   bool have_pass = false;
-  std::map<std::tuple<size_t, size_t, size_t, bool, size_t>, AttnPlan> plans;  // (window, hq, hkv, f32, page)
+  std::map<PlanKey, AttnPlan> plans;
   // Work-list buffers of dropped plans, reused by the next pass's plans: a new pass
   // uploads into them on the stream, after the launches that read them, so it needs
   // neither a hipFree (which waits for the device) nor a hipMalloc.
@@ -526,9 +538,10 @@ static constexpr uint32_t kFanIn = 32;  // chunks per group the automatic split 
 // f32: the f32 arena's plan: its prefill kernel's items for passes with many rows per
 // sequence (as for f16), else its split-K decode kernel's (16 logical rows per item).
 // page_size: the arena's (shared prefixes are found by page ids).
-int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, bool f32, size_t page_size,
+int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_t page_size,
                AttnPlan** out) {
-  auto key = std::make_tuple(window, hq, hkv, f32, page_size);
+  const bool f32 = dtype == YX_DTYPE_F32, q4 = dtype == YX_DTYPE_Q4;
+  auto key = std::make_tuple(window, hq, hkv, dtype, page_size);
   auto it = c->plans.find(key);
   if (it != c->plans.end()) {
     *out = &it->second;
@@ -602,8 +615,10 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, bool f32, size_t
     AttnPlan plan;
     plan.prefill = true;
     plan.f32 = f32;
+    plan.q4 = q4;
     // f32 tiles of 128 logical rows (option prefill_f32_waves: 4 takes 64, on f32 products).
     if (f32) plan.pf32_waves = c->pf32_waves ? static_cast<int>(c->pf32_waves) : 8;
+    static_assert(yx::kQ4TileRows == yx::kPrefillRows, "tiles of the 4-bit arena are cut as the binary16 arena's");
     const size_t tile_rows = !f32 ? yx::kPrefillRows : plan.pf32_waves == 4 ? yx::kPf32SmallRows : yx::kPf32Rows;
     const uint32_t per = static_cast<uint32_t>(std::max<size_t>(1, tile_rows / G));
     // f32 partials hold the rows in use (a tile of few rows and many chunks).
@@ -874,7 +889,7 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, bool f32, size_t
   // per CU: more would run in a second round.
   // (Four 8-row tiles do not fit one wave's registers: a row with more than 24 q heads
   // per KV head takes the 16-row-tile kernel whatever the shape option.)
-  const bool wide = f32 || (nt > 1 && c->decode_shape == 0) || c->decode_shape == 2 || nt > 3;
+  const bool wide = f32 || q4 || (nt > 1 && c->decode_shape == 0) || c->decode_shape == 2 || nt > 3;
   const size_t waves = nt == 1 ? yx::DecodeWaves<1>::value
                                : (wide ? yx::kWideWaves : yx::DecodeWaves<2>::value);
   const size_t target_items = c->target_waves > 0
@@ -1221,7 +1236,8 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, bool f32, size_t
     }
   }
   plan.f32 = f32;
-  plan.balanced = !f32 && nt == 1 && c->decode_shape == 0;
+  plan.q4 = q4;
+  plan.balanced = !f32 && !q4 && nt == 1 && c->decode_shape == 0;
   for (const yx::AttnItem& w : plan.items)
     if (w.blk1 - w.blk0 > 4 * yx::kBalQuads) plan.balanced = false;
   plan.small_units = plan.balanced;
@@ -1232,7 +1248,7 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, bool f32, size_t
   // long for the queue; the queue kernel where waves would otherwise get unequal shares.
   // (Measured: B=16 ctx 4096, 64-block items, 25.9 against 26.3 us; cfg4's 128-block
   // items 47.3 against 48.4; cfg2's ~44-block items 25.4 against 24.9.)
-  if (!f32 && nt == 1 && c->decode_shape == 0) {
+  if (!f32 && !q4 && nt == 1 && c->decode_shape == 0) {
     bool exact = true;
     for (const yx::AttnItem& w : plan.items)
       if ((w.blk1 - w.blk0) % yx::kWideWaves != 0) exact = false;
@@ -1301,11 +1317,11 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
   if (c->rows == 0) return YX_OK;
   if (!out || (!q && !qkv)) return fail(YX_ERR_INVALID, "null q or out");
   AttnPlan* plan;
-  if (c->capturing && !c->plans.count(std::make_tuple(window, hq, hkv, kv->f32, kv->page)))
+  if (c->capturing && !c->plans.count(std::make_tuple(window, hq, hkv, kv->dtype, kv->page)))
     return fail(YX_ERR_INVALID, "run the call once before capturing it (its work list is uploaded then)");
-  if ((rc = build_plan(c, window, hq, hkv, kv->f32, kv->page, &plan))) return rc;
+  if ((rc = build_plan(c, window, hq, hkv, kv->dtype, kv->page, &plan))) return rc;
   {
-    const auto key = std::make_tuple(window, hq, hkv, kv->f32, kv->page);
+    const auto key = std::make_tuple(window, hq, hkv, kv->dtype, kv->page);
     if (std::find(c->used_keys.begin(), c->used_keys.end(), key) == c->used_keys.end())
       c->used_keys.push_back(key);
   }
@@ -1324,7 +1340,7 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
   if (noalloc) {
     ScratchMap m;
     if ((rc = scratch_map(c, pml_need, po_need, cnt_need, &m))) return rc;
-    if ((rc = scratch_take(c, std::make_tuple(window, hq, hkv, kv->f32, kv->page), plan, &m))) return rc;
+    if ((rc = scratch_take(c, std::make_tuple(window, hq, hkv, kv->dtype, kv->page), plan, &m))) return rc;
     d_items = m.items;
     d_members = plan->members.empty() ? nullptr : static_cast<const yx::SubRef*>(m.members);
     po = static_cast<float*>(m.part_o);
@@ -1345,14 +1361,14 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
     po_cap = c->part_o.cap;
     pml_cap = c->part_ml.cap;
   }
-  if (knew && (plan->prefill || !plan->fusable)) {
+  if (knew && (plan->prefill || !plan->fusable || plan->q4)) {
     if ((rc = append_impl(c, kv, layer, knew, vnew))) return rc;
     knew = vnew = nullptr;
   }
-  if (qkv && plan->prefill && !plan->f32) {
+  if (qkv && plan->prefill && !plan->f32 && !plan->q4) {
     // The f16 prefill kernel normalises and rotates its rows' q heads itself; K/V first.
     if ((rc = qk_rope_impl(c, kv, layer, *qkv, hq, nullptr, true))) return rc;
-  } else if (qkv && (plan->f32 || !(plan->fusable && (plan->wide ? plan->nt <= 2 : plan->balanced)))) {
+  } else if (qkv && (plan->f32 || plan->q4 || !(plan->fusable && (plan->wide ? plan->nt <= 2 : plan->balanced)))) {
     // (Two-tile passes keep write_rows as its own launch: fused, each work item
     // normalises and rotates up to 32 q heads before its first block, and cfg5's
     // Backend::attention took 28.9 us in one launch against 28.5 in two.)
@@ -1380,7 +1396,13 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
                          static_cast<uint32_t>(hq), static_cast<uint32_t>(hkv), shift,
                          static_cast<uint32_t>(window), scale * yx::kLog2e, po, pml, cnt,
                          pf_po_bytes, pf_pml_bytes, plan->part_rows);
-    } else if (qkv)
+    } else if (plan->q4)
+      hipLaunchKernelGGL(yx::paged_attn_prefill_q4, pgrid, dim3(64 * yx::kQ4TileWaves), 0, c->stream,
+                         static_cast<const yx::PrefillItem*>(d_items), c->dev_pos,
+                         static_cast<const uint32_t*>(c->d_pages.p), kv->kq(layer), kv->vq(layer), q, out,
+                         static_cast<uint32_t>(hq), static_cast<uint32_t>(hkv), shift, static_cast<uint32_t>(window),
+                         scale * yx::kLog2e, po, pml, cnt, pf_po_bytes, pf_pml_bytes);
+    else if (qkv)
       hipLaunchKernelGGL((yx::paged_attn_prefill<true>), pgrid, dim3(64 * yx::kPrefillWaves), 0, c->stream,
                        static_cast<const yx::PrefillItem*>(d_items),
                        c->dev_pos, static_cast<const uint32_t*>(c->d_pages.p),
@@ -1428,6 +1450,10 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
                        items, pos, pages, kv->kf(layer), kv->vf(layer), q, out, po, pml, cnt, knew,
                        vnew, c->dev_slot, kv->kf(layer),
                        kv->vf(layer), po_bytes, pml_bytes, H, HK, P, W, scale_log2, mem, by_item);
+  } else if (plan->q4) {
+    auto* kern = plan->nt <= 2 ? yx::paged_attn_decode_q4<1> : yx::paged_attn_decode_q4<2>;
+    hipLaunchKernelGGL(kern, grid, dim3(64 * yx::kWideWaves), 0, c->stream, items, pos, pages, kv->kq(layer),
+                       kv->vq(layer), q, out, po, pml, cnt, po_bytes, pml_bytes, H, HK, P, W, scale_log2, mem, by_item);
   } else if (plan->balanced && !plan->wide) {
 #define YX_LAUNCH_BAL(QKV, UB, KN, VN, IN)                                                          \
   hipLaunchKernelGGL((yx::paged_attn_decode_balanced<QKV, UB>), grid, dim3(64 * yx::kBalWaves), 0,  \
@@ -1477,6 +1503,12 @@ int append_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* k, const float*
                        c->dev_slot, kv->kf(layer), kv->vf(layer),
                        static_cast<uint32_t>(c->rows), static_cast<uint32_t>(kv->hkv),
                        static_cast<uint32_t>(kv->page));
+  } else if (kv->q4) {
+    const size_t vecs = c->rows * kv->hkv;
+    if (vecs > 0xffffffffu) return fail(YX_ERR_UNSUPPORTED, "too many head vectors in the pass");
+    hipLaunchKernelGGL(yx::kv_append_q4, dim3(static_cast<unsigned>((vecs + 3) / 4), 2), dim3(256), 0, c->stream, k, v,
+                       c->dev_slot, kv->kq(layer), kv->vq(layer), static_cast<uint32_t>(vecs),
+                       static_cast<uint32_t>(kv->hkv), kv->page_shift());
   } else {
     hipLaunchKernelGGL(yx::kv_append_f16, grid, dim3(256), 0, c->stream, k, v,
                        c->dev_slot, kv->k[layer], kv->v[layer],
@@ -1515,6 +1547,12 @@ int qk_rope_impl(yx_ctx* c, yx_kv* kv, size_t layer, const yx::QkvIn& in, size_t
                        in.qkv, in.q_norm, in.k_norm, in.rope_cs, in.rope_len, in.eps,
                        c->dev_pos, c->dev_slot,
                        kv->kf(layer), kv->vf(layer), q_out, static_cast<uint32_t>(hq),
+                       static_cast<uint32_t>(hkv), page_shift, static_cast<uint32_t>(nvec),
+                       static_cast<uint32_t>(kv_only ? hq : 0));
+  else if (kv->q4)
+    hipLaunchKernelGGL(yx::qk_norm_rope_append<yx::q4_t>, grid, dim3(yx::kRopeThreads), 0, c->stream,
+                       in.qkv, in.q_norm, in.k_norm, in.rope_cs, in.rope_len, in.eps, c->dev_pos, c->dev_slot,
+                       kv->kq(layer), kv->vq(layer), q_out, static_cast<uint32_t>(hq),
                        static_cast<uint32_t>(hkv), page_shift, static_cast<uint32_t>(nvec),
                        static_cast<uint32_t>(kv_only ? hq : 0));
   else
@@ -1994,7 +2032,8 @@ int yx_ctx_set_option(yx_ctx* c, const char* key, long value) {
 int yx_kv_create(yx_ctx* c, size_t layers, size_t pages, size_t page_size, size_t hkv,
                  size_t head_dim, int dtype, yx_kv** out) {
   if (!c || !out) return fail(YX_ERR_INVALID, "null argument");
-  if (dtype != YX_DTYPE_F16 && dtype != YX_DTYPE_F32) return fail(YX_ERR_UNSUPPORTED, "dtype must be f16 or f32");
+  if (dtype != YX_DTYPE_F16 && dtype != YX_DTYPE_F32 && dtype != YX_DTYPE_Q4)
+    return fail(YX_ERR_UNSUPPORTED, "dtype must be f16, f32 or q4");
   if (head_dim != 128) return fail(YX_ERR_UNSUPPORTED, "head_dim must be 128");
   if (page_size < 16 || (page_size & (page_size - 1)) != 0)
     return fail(YX_ERR_UNSUPPORTED, "page size must be a power of two, at least 16");
@@ -2008,7 +2047,9 @@ int yx_kv_create(yx_ctx* c, size_t layers, size_t pages, size_t page_size, size_
   kv->page = page_size;
   kv->hkv = hkv;
   kv->d = head_dim;
+  kv->dtype = dtype;
   kv->f32 = dtype == YX_DTYPE_F32;
+  kv->q4 = dtype == YX_DTYPE_Q4;
   const size_t bytes = pages * kv->page_bytes();
   std::vector<void*> bases;
   for (size_t l = 0; l < layers; ++l) {
@@ -2128,6 +2169,30 @@ static int page_io(yx_ctx* c, yx_kv* kv, size_t layer, const uint32_t* pages, si
           std::memcpy(dst, src, 16);
         }
   };
+  // A 4-bit page: rows of 72 bytes (64 of codes, two dims a byte, the lower first; 4 steps) from
+  // or into the arena's blocks.
+  auto permute_q4 = [&](uint8_t* rows, uint8_t* arena, bool is_k, bool to_arena) {
+    for (size_t r = 0; r < kv->hkv * kv->page; ++r) {
+      uint8_t* blk = arena + r / 16 * yx::kQ4Block;  // a head's keys fill whole blocks
+      uint8_t* row = rows + r * yx::kQ4Row;
+      const uint32_t key = static_cast<uint32_t>(r % 16);
+      uint8_t* st = blk + yx::kQ4Steps + key * 8;
+      std::memcpy(to_arena ? st : row + 64, to_arena ? row + 64 : st, 8);
+      if (!to_arena) std::memset(row, 0, 64);
+      for (uint32_t d = 0; d < 128; ++d) {
+        const uint32_t word = is_k ? yx::q4_k_word(key, d / 8 % 4, d / 32) : yx::q4_v_word(key, d % 16);
+        const uint32_t sh = 4 * (is_k ? yx::q4_k_nibble(d % 8) : d / 16);
+        uint32_t w;
+        std::memcpy(&w, blk + word, 4);
+        if (to_arena) {
+          w = (w & ~(15u << sh)) | static_cast<uint32_t>(row[d / 2] >> (4 * (d % 2)) & 15) << sh;
+          std::memcpy(blk + word, &w, 4);
+        } else {
+          row[d / 2] = static_cast<uint8_t>(row[d / 2] | (w >> sh & 15u) << (4 * (d % 2)));
+        }
+      }
+    }
+  };
   for (size_t i = 0; i < n; ++i) {
     if (pages[i] >= kv->pages) return fail(YX_ERR_INVALID, "page beyond the arena");
     char* kd = reinterpret_cast<char*>(kv->k[layer]) + pages[i] * pb;
@@ -2139,6 +2204,23 @@ static int page_io(yx_ctx* c, yx_kv* kv, size_t layer, const uint32_t* pages, si
       } else {
         if (k) YX_HIP(hipMemcpyAsync(kd, static_cast<const char*>(k) + i * pb, pb, hipMemcpyHostToDevice, c->stream));
         if (v) YX_HIP(hipMemcpyAsync(vd, static_cast<const char*>(v) + i * pb, pb, hipMemcpyHostToDevice, c->stream));
+      }
+    } else if (kv->q4) {
+      uint8_t* bytes = reinterpret_cast<uint8_t*>(tmp.data());
+      for (int which : {YX_K, YX_V}) {
+        uint8_t* rows = static_cast<uint8_t*>(which == YX_K ? k : v);
+        char* dev = which == YX_K ? kd : vd;
+        if (!rows) continue;
+        rows += i * pb;
+        if (read) {
+          YX_HIP(hipMemcpyAsync(bytes, dev, pb, hipMemcpyDeviceToHost, c->stream));
+          YX_HIP(hipStreamSynchronize(c->stream));
+          permute_q4(rows, bytes, which == YX_K, false);
+        } else {
+          permute_q4(rows, bytes, which == YX_K, true);
+          YX_HIP(hipMemcpyAsync(dev, bytes, pb, hipMemcpyHostToDevice, c->stream));
+          YX_HIP(hipStreamSynchronize(c->stream));
+        }
       }
     } else if (read) {
       if (k) {
@@ -2403,6 +2485,32 @@ int yx_kv_append(yx_ctx* c, yx_kv* kv, size_t layer, const float* k, const float
   if ((rc = yx_kv_append_dev(c, kv, layer, static_cast<float*>(c->io_a.p), static_cast<float*>(c->io_b.p))))
     return rc;
   YX_HIP(hipStreamSynchronize(c->stream));
+  return YX_OK;
+}
+
+int yx_kv_rows_dev(yx_ctx* c, yx_kv* kv, size_t layer, float* k_out, float* v_out) {
+  int rc = check_kv(c, kv, layer);
+  if (rc) return rc;
+  if (!k_out && !v_out) return fail(YX_ERR_INVALID, "null k_out and v_out");
+  if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16)
+    return fail(YX_ERR_INVALID, "k_out and v_out must be 16-byte aligned");
+  const size_t vecs = c->rows * kv->hkv;
+  if (vecs > 0xffffffffu) return fail(YX_ERR_UNSUPPORTED, "too many head vectors in the pass");
+  if (k_out && v_out && overlap(k_out, vecs * 512, v_out, vecs * 512)) return fail(YX_ERR_INVALID, "k_out and v_out overlap");
+  if ((rc = c->set_device())) return rc;
+  if (vecs == 0) return YX_OK;
+  const dim3 grid(static_cast<unsigned>((vecs + 15) / 16), 2);
+  const uint32_t n = static_cast<uint32_t>(vecs), heads = static_cast<uint32_t>(kv->hkv);
+  if (kv->q4)
+    hipLaunchKernelGGL(yx::kv_rows<yx::q4_t>, grid, dim3(256), 0, c->stream, kv->kq(layer), kv->vq(layer), c->dev_slot,
+                       k_out, v_out, n, heads, kv->page_shift());
+  else if (kv->f32)
+    hipLaunchKernelGGL(yx::kv_rows<float>, grid, dim3(256), 0, c->stream, kv->kf(layer), kv->vf(layer), c->dev_slot,
+                       k_out, v_out, n, heads, kv->page_shift());
+  else
+    hipLaunchKernelGGL(yx::kv_rows<_Float16>, grid, dim3(256), 0, c->stream, kv->k[layer], kv->v[layer], c->dev_slot,
+                       k_out, v_out, n, heads, kv->page_shift());
+  YX_HIP(hipGetLastError());
   return YX_OK;
 }
 
