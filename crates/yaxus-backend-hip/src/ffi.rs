@@ -31,6 +31,7 @@ pub const YX_ERR_HIP: c_int = 5;
 pub const YX_ERR_UNSUPPORTED: c_int = 6;
 pub const YX_DTYPE_F32: c_int = 0;
 pub const YX_DTYPE_F16: c_int = 1;
+pub const YX_DTYPE_Q4: c_int = 2;
 pub const YX_K: c_int = 0;
 pub const YX_V: c_int = 1;
 pub const YX_ACT_NONE: c_int = 0;
@@ -125,6 +126,10 @@ unsafe extern "C" {
     pub fn yx_memcpy_d2h(ctx: *mut yx_ctx, dst: *mut c_void, src: *const c_void, bytes: usize) -> c_int;
     pub fn yx_dev_copy(ctx: *mut yx_ctx, dst: *mut c_void, src: *const c_void, bytes: usize) -> c_int;
     pub fn yx_dev_checksum(ctx: *mut yx_ctx, src: *const c_void, bytes: usize, out: *mut u64) -> c_int;
+    pub fn yx_verify_drafts_dev(ctx: *mut yx_ctx, logits: *const f32, cols: usize, ld: usize, row_off: *const u32,
+                                seqs: usize, drafts: *const u32, draft_logits: *const f32, draft_ld: usize,
+                                temperature: *const f32, accept_u: *const f32, pick_u: *const f32,
+                                accepted: *mut u32, next: *mut u32) -> c_int;
     pub fn yx_fill_normal(ctx: *mut yx_ctx, dst: *mut c_void, n: usize, dtype: c_int, seed: u64,
                           offset: u64) -> c_int;
 

@@ -12,7 +12,7 @@
  *                                          yx_attention_dev; yx_kv_append stores K/V alone
  * and what a backend with its rows on the device runs between attention calls and at the end:
  *   products yx_matmul_bf16_dev and yx_linear_bf16_dev, block seams yx_add_norm_rows_dev,
- *   yx_argmax_rows_dev and yx_logprobs_rows_dev.
+ *   yx_argmax_rows_dev, yx_logprobs_rows_dev and yx_verify_drafts_dev.
  *
  * Conventions: int status, YX_OK = 0 (codes shared with yaxus_kv_cache.h);
  * yx_last_error() returns a thread-local message; no exception crosses the ABI. Every
@@ -276,6 +276,30 @@ int yx_add_norm_rows_dev(yx_ctx* ctx, const float* x, const float* post_w, float
 int yx_logprobs_rows_dev(yx_ctx* ctx, const float* logits, size_t rows, size_t cols, size_t ld,
                          const uint32_t* tokens, size_t given, size_t top, float* logprob,
                          float* entropy, uint32_t* top_ids, float* top_logprobs);
+
+/* Verification of drafted tokens (speculative sampling; no counterpart in the reference, which
+ * compares greedy picks): of each of `seqs` sequences with k drafts and the k + 1 rows of logits
+ * after them, how many drafts stand, and the token that follows them. row_off `[seqs + 1]`, host:
+ * sequence s has the target rows row_off[s] .. row_off[s + 1] - 1 of logits (f32, `cols` values a
+ * row, rows `ld` apart; row_off[0] = 0, at least one row each) and as many drafts less one:
+ * drafts, accept_u `[rows - seqs]` and the rows of draft_logits (`draft_ld` apart) are those of
+ * the sequences one after the other. With p the softmax of a target row over temperature[s] and
+ * q the draft row's, draft x is accepted while accept_u q(x) < p(x); next[s] is the first token
+ * whose cumulative weight, in index order, exceeds pick_u[s] times all weights, of max(p - q, 0)
+ * at the first rejected draft (of p where that is nowhere positive), or of the last row's p when
+ * every draft stands: accepted[s] of them. Uniform numbers from [0, 1); all comparisons and sums
+ * in 64 bits, the same answer every time.
+ * draft_logits null: the drafts were certain (copied, not drawn), q(x) = 1. temperature null: 1
+ * everywhere; a temperature of 0 (or below, or NaN): p is 1 at the first of the largest logits,
+ * and q does not matter. Logits of -inf, and NaN, are masked tokens: probability 0, never
+ * accepted, never drawn; +inf takes all of its row. A target row of nothing else accepts nothing
+ * and gives YX_NO_TOKEN; a draft row of nothing else counts as q = 0. A draft of `cols` or more is
+ * rejected. At most 4194304 columns. Everything but row_off lies on the device; accepted and next
+ * `[seqs]` overlap neither the inputs nor each other. A captured call keeps its row_off. */
+int yx_verify_drafts_dev(yx_ctx* ctx, const float* logits, size_t cols, size_t ld, const uint32_t* row_off,
+                         size_t seqs, const uint32_t* drafts, const float* draft_logits, size_t draft_ld,
+                         const float* temperature, const float* accept_u, const float* pick_u,
+                         uint32_t* accepted, uint32_t* next);
 
 /* Device memory and copies on the context's stream (h2d/d2h are synchronous). */
 int yx_dev_alloc(yx_ctx* ctx, size_t bytes, void** out);

@@ -112,6 +112,7 @@ HIP_SYMBOLS = {
     "yx_linear_bf16_dev": (I, [P, P, P, P, I, I, P, P, S, S, S]),
     "yx_add_norm_rows_dev": (I, [P, P, P, F, P, P, P, F, P, F, S, S]),
     "yx_logprobs_rows_dev": (I, [P, P, S, S, S, P, S, S, P, P, P, P]),
+    "yx_verify_drafts_dev": (I, [P, P, S, S, P, S, P, P, S, P, P, P, P, P]),
     "yx_fill_normal": (I, [P, P, S, I, U64, U64]),
     "yx_graph_begin": (I, [P]),
     "yx_graph_end": (I, [P]),

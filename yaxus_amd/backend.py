@@ -8,7 +8,8 @@ the KV arena (crates/yaxus-model/src/lib.rs:95-171), over ``libyaxus_hip.so``.
                                           write_rows) + HipBackend.attend
 
 The step after attention, on rows that stay on the device: ``matmul_bf16``, ``linear_bf16``
-(bias, activation, gate, residual), ``add_norm``, ``argmax_rows``, ``logprobs_rows``.
+(bias, activation, gate, residual), ``add_norm``, ``argmax_rows``, ``logprobs_rows``,
+``verify_drafts``.
 
 Tensors are ``DeviceTensor`` values (device memory owned by the context); numpy arrays
 are accepted where a host round trip is intended. A missing library, or a context
@@ -428,6 +429,41 @@ class HipBackend:
                                               tokens.ptr if given else None, given, top,
                                               lp and lp.ptr, entropy and entropy.ptr, ids and ids.ptr,
                                               tlp and tlp.ptr))
+        return out
+
+    def verify_drafts(self, logits, row_off, drafts, accept_u, pick_u, draft_logits=None, temperature=None,
+                      cols=None, out=None):
+        """Drafted tokens against the target's probabilities (yx_verify_drafts_dev). logits
+        `[rows][ld]` f32, of each row the first ``cols`` (default: all) are the vocabulary; row_off
+        (host) the first row of every sequence and their end; drafts and accept_u `[rows - seqs]`
+        (None without any), draft_logits `[rows - seqs][ld]` or None (certain drafts), temperature
+        `[seqs]` or None (1), pick_u `[seqs]`. Returns (accepted, next), uint32 `[seqs]`: ``out``,
+        or new device tensors."""
+        off = np.ascontiguousarray(row_off, np.uint32)
+        if off.ndim != 1 or len(off) < 1:
+            raise ValueError("row_off holds every sequence's first row and the end of the last")
+        seqs, rows = len(off) - 1, int(off[-1])
+        nd = rows - seqs
+        ld = logits.shape[1]
+        cols = ld if cols is None else cols
+        out = out if out is not None else tuple(self.tensor((seqs,), np.uint32) for _ in range(2))
+        if logits.shape[0] < rows:
+            raise ValueError("fewer rows of logits than row_off names")
+        if nd > 0 and (drafts is None or accept_u is None):
+            raise ValueError("drafts without their tokens or numbers")
+        if draft_logits is not None and draft_logits.shape[0] < nd:
+            raise ValueError("fewer rows of draft logits than drafts")
+        _need(logits, rows * ld * 4, "logits")
+        if draft_logits is not None:
+            _need(draft_logits, nd * draft_logits.shape[1] * 4, "draft_logits")
+        for t, n, what in ((drafts, nd, "drafts"), (accept_u, nd, "accept_u"), (pick_u, seqs, "pick_u"),
+                           (temperature, seqs, "temperature"), (out[0], seqs, "accepted"), (out[1], seqs, "next")):
+            if t is not None and n > 0:
+                _need(t, n * 4, what)
+        check_hip(self.L.yx_verify_drafts_dev(
+            self.ctx, logits.ptr, cols, ld, ptr(off), seqs, drafts and drafts.ptr, draft_logits and draft_logits.ptr,
+            draft_logits.shape[1] if draft_logits is not None else 0, temperature and temperature.ptr,
+            accept_u and accept_u.ptr, pick_u.ptr, out[0].ptr, out[1].ptr))
         return out
 
     def stat(self, key):

@@ -27,6 +27,7 @@
 #include "q4.hpp"
 #include "qk_rope.hpp"
 #include "step_after.hpp"
+#include "verify.hpp"
 
 namespace {
 
@@ -373,6 +374,7 @@ struct yx_ctx {
   // Rows of logits read in slices: the slices' sums and keys and the rows' arrival counters,
   // for logprobs_slots slices in all, allocated with the context too.
   DevBuf lp_keys, lp_parts, lp_counters;
+  DevBuf vd_parts, vd_stops, vd_sums, vd_counters;  // drafts verified: chunk sums, where each sequence stopped, arrivals
   uint64_t mm_kernel = 0, mm_k_parts = 0, mm_run_stages = 0;  // what the latest matmul ran (tests)
   // options
   long target_waves = 0;  // 0: one work item per CU
@@ -405,7 +407,8 @@ struct yx_ctx {
   uint64_t buffer_gens() const {
     uint64_t s = 0;
     for (const DevBuf* b : {&d_meta, &d_pages, &part_o, &part_ml, &counters, &io_a, &io_b, &io_c,
-                            &io_q, &am_keys, &am_counters, &mm_part, &mm_counters})
+                            &io_q, &am_keys, &am_counters, &mm_part, &mm_counters, &vd_parts, &vd_stops, &vd_sums,
+                            &vd_counters})
       s += b->gen;
     return s;
   }
@@ -1968,6 +1971,7 @@ int yx_ctx_destroy(yx_ctx* c) {
   c->spare.clear();
   for (DevBuf* b : {&c->d_meta, &c->d_pages, &c->am_keys, &c->am_counters, &c->mm_part, &c->mm_counters,
                     &c->mt_part, &c->mt_counters, &c->lp_keys, &c->lp_parts, &c->lp_counters,
+                    &c->vd_parts, &c->vd_stops, &c->vd_sums, &c->vd_counters,
                     &c->part_o, &c->part_ml, &c->counters,
                     &c->io_a, &c->io_b, &c->io_c, &c->io_q})
     b->release();
@@ -2821,6 +2825,87 @@ int yx_logprobs_rows_dev(yx_ctx* c, const float* logits, size_t rows, size_t col
                        static_cast<uint32_t>(per),
                        static_cast<unsigned long long*>(c->lp_keys.p), static_cast<float*>(c->lp_parts.p),
                        static_cast<uint32_t*>(c->lp_counters.p));
+  }
+  YX_HIP(hipGetLastError());
+  return YX_OK;
+}
+
+int yx_verify_drafts_dev(yx_ctx* c, const float* logits, size_t cols, size_t ld, const uint32_t* row_off, size_t seqs,
+                         const uint32_t* drafts, const float* draft_logits, size_t draft_ld, const float* temperature,
+                         const float* accept_u, const float* pick_u, uint32_t* accepted, uint32_t* next) {
+  if (!c) return fail(YX_ERR_INVALID, "null context");
+  if (seqs == 0) return YX_OK;
+  if (!logits || !row_off || !pick_u || !accepted || !next)
+    return fail(YX_ERR_INVALID, "null logits, row_off, pick_u, accepted or next");
+  if (cols == 0) return fail(YX_ERR_INVALID, "empty rows");
+  if (ld < cols) return fail(YX_ERR_INVALID, "the row stride is below the row's length");
+  if (row_off[0] != 0) return fail(YX_ERR_INVALID, "row_off starts at 0");
+  if (seqs > 0x7fffffffu) return fail(YX_ERR_UNSUPPORTED, "too many sequences");
+  for (size_t s = 0; s < seqs; ++s)
+    if (row_off[s + 1] <= row_off[s]) return fail(YX_ERR_INVALID, "every sequence has a row: row_off rises");
+  const size_t rows = row_off[seqs], nd = rows - seqs;
+  if (nd && (!drafts || !accept_u)) return fail(YX_ERR_INVALID, "null drafts or accept_u");
+  if (!nd) draft_logits = nullptr;
+  if (draft_logits && draft_ld < cols) return fail(YX_ERR_INVALID, "the draft logits' row stride is below the row's length");
+  const size_t nch = (cols + yx::kVdChunk - 1) / yx::kVdChunk;
+  constexpr size_t kMost = size_t{1} << 48;  // values of one buffer
+  if (nch > yx::kVdMaxChunks || ld > kMost / rows || (draft_logits && draft_ld > kMost / nd))
+    return fail(YX_ERR_UNSUPPORTED, "verification dimensions too large (at most 4194304 columns)");
+  const struct {
+    const void* p;
+    size_t bytes;
+  } ins[] = {{logits, ((rows - 1) * ld + cols) * 4}, {draft_logits, nd ? ((nd - 1) * draft_ld + cols) * 4 : 0},
+             {nd ? drafts : nullptr, nd * 4}, {temperature, seqs * 4}, {nd ? accept_u : nullptr, nd * 4}, {pick_u, seqs * 4}},
+    outs[] = {{accepted, seqs * 4}, {next, seqs * 4}};
+  for (const auto& i : ins)
+    if (reinterpret_cast<uintptr_t>(i.p) % 4) return fail(YX_ERR_INVALID, "verification buffers must be 4-byte aligned");
+  for (const auto& o : outs) {
+    if (reinterpret_cast<uintptr_t>(o.p) % 4) return fail(YX_ERR_INVALID, "verification buffers must be 4-byte aligned");
+    for (const auto& i : ins)
+      if (overlap(o.p, o.bytes, i.p, i.bytes)) return fail(YX_ERR_INVALID, "an output overlaps an input");
+  }
+  if (overlap(accepted, seqs * 4, next, seqs * 4)) return fail(YX_ERR_INVALID, "two outputs overlap");
+  // Sequences of one launch: their offsets go with it, their rows are its grid.
+  constexpr size_t kMostRows = 0xffff;
+  const auto launch_rows = [&](size_t a, size_t b) {  // of sequences [a, b)
+    const size_t t = row_off[b] - row_off[a];
+    return draft_logits ? 2 * t - (b - a) : t;
+  };
+  const size_t most = std::min(kMostRows, (size_t{1} << 28) / nch - 1);
+  std::vector<size_t> cuts{0};
+  size_t part_rows = 0;
+  while (cuts.back() < seqs) {
+    const size_t a = cuts.back();
+    size_t b = a + 1;
+    if (launch_rows(a, b) > most) return fail(YX_ERR_UNSUPPORTED, "too many drafts of one sequence");
+    while (b < seqs && b - a < yx::kVdSeqs && launch_rows(a, b + 1) <= most) ++b;
+    part_rows = std::max(part_rows, launch_rows(a, b));
+    cuts.push_back(b);
+  }
+  int rc = c->set_device();
+  if (rc) return rc;
+  const size_t part_bytes = part_rows * nch * sizeof(yx::VerifyPart), now = std::min<size_t>(seqs, yx::kVdSeqs);
+  const size_t counter_bytes = yx::kVdSeqs * 4 * yx::kCounterStride;
+  if ((rc = c->vd_parts.ensure(part_bytes, c->stream))) return rc;
+  if ((rc = c->vd_stops.ensure(yx::kVdSeqs * sizeof(yx::VerifyStop), c->stream))) return rc;
+  if ((rc = c->vd_sums.ensure(now * nch * sizeof(double), c->stream))) return rc;
+  if ((rc = c->vd_counters.ensure(counter_bytes, c->stream, true))) return rc;
+  auto* parts = static_cast<yx::VerifyPart*>(c->vd_parts.p);
+  auto* stops = static_cast<yx::VerifyStop*>(c->vd_stops.p);
+  auto* counters = static_cast<uint32_t*>(c->vd_counters.p);
+  for (size_t i = 0; i + 1 < cuts.size(); ++i) {
+    const size_t a = cuts[i], n = cuts[i + 1] - a, row0 = row_off[a], d0 = row0 - a;
+    yx::VerifyRows vr{};
+    vr.seqs = static_cast<uint32_t>(n);
+    for (size_t s = 0; s <= n; ++s) vr.off[s] = row_off[a + s] - row_off[a];
+    const yx::VerifyIn in{logits + row0 * ld, draft_logits ? draft_logits + d0 * draft_ld : nullptr, nd ? drafts + d0 : nullptr,
+                          temperature ? temperature + a : nullptr, nd ? accept_u + d0 : nullptr, pick_u + a, ld, draft_ld,
+                          static_cast<uint32_t>(cols), static_cast<uint32_t>(nch)};
+    hipLaunchKernelGGL(yx::verify_sums, dim3(static_cast<unsigned>(nch), static_cast<unsigned>(launch_rows(a, a + n))),
+                       dim3(yx::kVdThreads), 0, c->stream, vr, in, parts, part_bytes, stops, counters, accepted + a, next + a);
+    if (in.dlogits)
+      hipLaunchKernelGGL(yx::verify_residual, dim3(static_cast<unsigned>(nch), static_cast<unsigned>(n)), dim3(yx::kVdThreads), 0,
+                         c->stream, vr, in, parts, part_bytes, stops, static_cast<double*>(c->vd_sums.p), counters, next + a);
   }
   YX_HIP(hipGetLastError());
   return YX_OK;
