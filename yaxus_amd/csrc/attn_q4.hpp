@@ -1,19 +1,22 @@
 // Paged attention over a 4-bit arena (q4.hpp) for gfx950: decode and verify items, and prefill
 // tiles.
 //
-// out = softmax(q K^T scale) V with K, V = s (code - 8), s the binary16 step of 32 dims. Codes and
-// steps go into the matrix products apart, so that both stay exact (their product has 15 bits,
-// more than a binary16 holds):
+// out = softmax(q K^T scale) V with K, V = s (code - 8), s the binary16 step of 32 dims: up to 15
+// bits, more than a binary16 holds.
 //   S[key] = sum_p s_p[key] sum_d q_d (code_d - 8)          p: a group of 32 dims
 //     one v_mfma_f32_16x16x32_f16 per group and part of q, the codes as binary16 (below); then
 //     one fused multiply-add per score and group;
-//   O_d = sum_key (P s_p) (code_d - 8)
-//     P s_p per group as a binary16 hi and lo part.
-// q is scaled by a power of two of its row (its largest value near 2^12) before it is cut into hi
-// and lo, so its size does not matter; both cuts keep ~2^-22. P s_p is cut at a fixed scale that
-// holds steps below 8; where a larger one overflows it, the wave starts again at a scale that
-// holds every binary16 (V beyond 64 in magnitude). A masked key has weight 0 and its step is left
-// out, so whatever lies behind a sequence's last token has no effect, NaN steps included.
+//   O_d = sum_key P V_d
+//     V as a binary16 hi part (the rounded product of step and code) and a lo part (what that left,
+//     exact: one packed fused multiply-add), P as hi and lo too; all products but lo lo.
+// K's steps stay apart since a score needs one multiply-add per group where K's lo part would need
+// a third matrix product per group; V's go in since they would cost a cut of P per group and row.
+// q is scaled by a power of two of its row (its largest value near 2^12) before it is cut, so its
+// size does not matter; the cuts keep ~2^-22. A binary16 holds V's parts (and 16 times them) below
+// 4096: a wave whose result is not finite runs again, once for the steps from 1 up, scaled down,
+// and once for the others, with steps of NaN (or infinite) left out and noted where a row sees them.
+// Steps of keys that no row of the wave sees are cleared at once. So a masked key never has an
+// effect, whatever it holds.
 //
 // Operands (lane l, c = l % 16, g = l / 16): columns are logical rows ((row, q head) pairs), 16 a
 // tile. S^T and P^T: keys 4 g + i of column c. O^T: dims 16 n + 4 g + i of column c (n: tile of V).
@@ -29,228 +32,224 @@
 
 namespace yx {
 
-// One 16-key block of a lane: K and V codes, the steps of keys 4 g .. 4 g + 3 of both.
-struct Q4Regs {
-  u32x4 k, v, ks[2], vs[2];
+typedef _Float16 half2_q4 __attribute__((ext_vector_type(2)));
+
+// K of a 16-key block as a lane holds it: codes, and the steps of keys 4 g .. 4 g + 3. V likewise.
+struct Q4Half {
+  u32x4 codes, steps[2];
 };
 
 template <int kPolicy>
-__device__ __forceinline__ void q4_load(Q4Regs& r, const q4_t* kblk, const q4_t* vblk, bool valid, int lane) {
-  const int bytes = valid ? static_cast<int>(kQ4Block) : 0;
-  const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<q4_t*>(kblk), 0, bytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<q4_t*>(vblk), 0, bytes, 0x00020000);
+__device__ __forceinline__ void q4_load(Q4Half& r, const q4_t* blk, bool valid, int lane) {
+  const __amdgpu_buffer_rsrc_t rs =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<q4_t*>(blk), 0, valid ? static_cast<int>(kQ4Block) : 0, 0x00020000);
   const int st = static_cast<int>(kQ4Steps) + (lane >> 4) * 32;
-  r.k = __builtin_amdgcn_raw_buffer_load_b128(rk, lane * 16, 0, kPolicy);
-  r.ks[0] = __builtin_amdgcn_raw_buffer_load_b128(rk, st, 0, kPolicy);
-  r.ks[1] = __builtin_amdgcn_raw_buffer_load_b128(rk, st, 16, kPolicy);
-  r.v = __builtin_amdgcn_raw_buffer_load_b128(rv, lane * 16, 0, kPolicy);
-  r.vs[0] = __builtin_amdgcn_raw_buffer_load_b128(rv, st, 0, kPolicy);
-  r.vs[1] = __builtin_amdgcn_raw_buffer_load_b128(rv, st, 16, kPolicy);
-}
-
-// Step of key 4 g + i, group p.
-__device__ __forceinline__ float q4_step(const u32x4* s, int i, int p) {
-  return static_cast<float>(__builtin_bit_cast(half8, s[i >> 1])[(i & 1) * 4 + p]);
+  r.codes = __builtin_amdgcn_raw_buffer_load_b128(rs, lane * 16, 0, kPolicy);
+  r.steps[0] = __builtin_amdgcn_raw_buffer_load_b128(rs, st, 0, kPolicy);
+  r.steps[1] = __builtin_amdgcn_raw_buffer_load_b128(rs, st, 16, kPolicy);
 }
 
 // Two codes in the low nibbles of w's halves (kOdd: the second nibbles) less 8 (kOdd: 16 times
 // that) as binary16: or-ed under the exponent of 1024 they read 1024 + code (1024 + 16 code), and
 // the difference is exact. (As they lie, read as subnormals code * 2^-24, they would need no
 // exponent, but the matrix unit aligns a subnormal's products by its nominal exponent and drops
-// up to 7 of their bits: outputs 6e-6 off after 600 keys and 1.3e-5 after 4000, against 4e-7.)
+// up to 7 of their bits: outputs 6e-6 off after 600 keys and 1.3e-5 after 4000, against 3e-7.)
 template <bool kOdd>
-__device__ __forceinline__ uint32_t q4_codes(uint32_t w) {
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  const h2 c = __builtin_bit_cast(h2, (w & (kOdd ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
+__device__ __forceinline__ half2_q4 q4_codes(uint32_t w) {
+  const half2_q4 c = __builtin_bit_cast(half2_q4, (w & (kOdd ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
   const _Float16 base = static_cast<_Float16>(kOdd ? 1152.0f : 1032.0f);
-  return __builtin_bit_cast(uint32_t, c - h2{base, base});
+  return c - half2_q4{base, base};
 }
 
 // The codes of a K dword as a matrix operand (dims 32 p + 8 g + 0 .. 7; 2, 3, 6, 7 times 16).
 __device__ __forceinline__ half8 q4_k_codes(uint32_t w) {
-  return __builtin_bit_cast(half8, u32x4{q4_codes<false>(w), q4_codes<true>(w), q4_codes<false>(w >> 8), q4_codes<true>(w >> 8)});
-}
-
-// V dwords of four keys, halves brought together: r[h][0] has the dims of tiles 0 to 3 of keys
-// 2 h and 2 h + 1, r[h][1] those of tiles 4 to 7.
-__device__ __forceinline__ void q4_v_halves(const u32x4& v, uint32_t (&r)[2][2]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    r[h][0] = __builtin_amdgcn_perm(v[2 * h + 1], v[2 * h], 0x05040100u);
-    r[h][1] = __builtin_amdgcn_perm(v[2 * h + 1], v[2 * h], 0x07060302u);
-  }
-}
-
-// Tile n's codes of keys 2 h and 2 h + 1 (odd n: times 16).
-template <int n>
-__device__ __forceinline__ uint32_t q4_v_codes(const uint32_t (&r)[2]) {
-  return q4_codes<(n & 1) != 0>(r[n >> 2] >> (8 * ((n >> 1) & 1)));
+  const half2_q4 a = q4_codes<false>(w), b = q4_codes<true>(w), c = q4_codes<false>(w >> 8), d = q4_codes<true>(w >> 8);
+  return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
 // Two values as a binary16 hi part and a lo part each. The values and the hi parts are pinned: the
-// compiler would otherwise take hi from the unrounded product y comes from in one place and from y
-// in the other, which differ by a last bit now and then.
+// compiler would otherwise take hi from the unrounded product a value comes from in one place and
+// from the value in the other, which differ by a last bit now and then (outputs up to 1e-5 off).
 __device__ __forceinline__ void q4_cut(float y0, float y1, uint32_t& hi, uint32_t& lo) {
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
   pin(y0);
   pin(y1);
-  hi = __builtin_bit_cast(uint32_t, h2{static_cast<_Float16>(y0), static_cast<_Float16>(y1)});
+  hi = __builtin_bit_cast(uint32_t, half2_q4{static_cast<_Float16>(y0), static_cast<_Float16>(y1)});
   pin(hi);
-  const h2 h = __builtin_bit_cast(h2, hi);
-  lo = __builtin_bit_cast(uint32_t, h2{static_cast<_Float16>(y0 - static_cast<float>(h.x)), static_cast<_Float16>(y1 - static_cast<float>(h.y))});
+  const half2_q4 h = __builtin_bit_cast(half2_q4, hi);
+  lo = __builtin_bit_cast(uint32_t, half2_q4{static_cast<_Float16>(__builtin_fmaf(static_cast<float>(h.x), -1.0f, y0)),
+                                             static_cast<_Float16>(__builtin_fmaf(static_cast<float>(h.y), -1.0f, y1))});
 }
 
-// Weights are 2^(room + x - m), x and m in log2, and x > m + kQ4Lazy moves m. As high as binary16
-// allows, since parts of weights below its smallest normal value lose bits: where one key
-// outweighs 4000 others, outputs were 1e-5 off with the maximum moved by more than 8 only (and
-// room 5), 2e-7 off like this.
+// Weights are 2^(kQ4Room + x - m), x and m in log2, and x > m + kQ4Lazy moves m: as high as
+// binary16 allows, since parts of weights below its smallest normal value lose bits.
 static constexpr float kQ4Lazy = 2.0f;
-static constexpr float kQ4Room = 11.0f;     // steps below 8 fit
-static constexpr float kQ4RoomBig = -4.0f;  // any step fits
+static constexpr float kQ4Room = 13.0f;
 
 // What one wave attends: NT tiles of 16 logical rows over the blocks [b0, b0 + nblk) of a page
-// table. rpos / rlo: the last and first key of this lane's column (rpos -1: no row).
+// table.
 template <int NT>
 struct Q4Wave {
-  float m[NT], l[NT];      // maximum (log2) and this lane's share of the sum
+  float m[NT], l[NT];      // maximum (log2) and sum
   floatx4 o[NT][8];        // unnormalised, dims 16 n + 4 g + i
 };
 
-template <int NT, int kPolicy>
+// The rows of a wave: this lane's column of each tile.
+template <int NT>
+struct Q4Rows {
+  bool has[NT];            // there is a row
+  int pos[NT], lo[NT];     // its last (-1: no row) and first key
+  float fac[NT];           // from products to log2 scores
+  int all_lo, all_pos;     // keys that every row of the wave sees,
+  int any_lo, any_pos;     // and from the first to the last that some row does
+};
+
+// A tile's q (this lane's dims 32 p + 8 g + 0 .. 7 of its column) as operands: hi and lo parts
+// scaled by a power of two; returns the factor from products to log2 scores.
+__device__ __forceinline__ float q4_cut_q(const float4 (&raw)[8], bool has, float scale_log2, half8 (&hi)[4], half8 (&lo)[4]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float4 a = raw[j];
+    top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
+  }
+  top = max_xor32(max_xor16(top));
+  const int ex = has && top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;  // top < 2^ex
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const float4 a = raw[2 * p], b = raw[2 * p + 1];
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = has ? __builtin_ldexpf(x[e], (e & 2) ? 9 - ex : 13 - ex) : 0.0f;
+      const _Float16 h = static_cast<_Float16>(v);
+      hi[p][e] = h;
+      lo[p][e] = static_cast<_Float16>(v - static_cast<float>(h));
+    }
+  }
+  return __builtin_ldexpf(scale_log2, ex - 13);
+}
+
+// kSlots: pairs of blocks a wave holds; each half (K, V) is loaded again as soon as it is used up.
+// q(t, p, part): the operand of tile t.
+template <int NT, int kSlots, bool kLong, int kPolicy, typename Q>
 __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict__ kc, const q4_t* __restrict__ vc,
                                           const uint32_t* __restrict__ pt, uint32_t b0, uint32_t nblk,
-                                          uint32_t bpp_shift, uint32_t kh, uint32_t hkv, const float4 (&qraw)[NT][8],
-                                          const bool (&has)[NT], const int (&rpos)[NT], const int (&rlo)[NT],
-                                          float scale_log2, int lane) {
+                                          uint32_t bpp_shift, uint32_t kh, uint32_t hkv, const Q4Rows<NT>& rows, int lane,
+                                          Q q) {
   const uint32_t bpp_mask = (1u << bpp_shift) - 1u;
   const size_t head_bytes = static_cast<size_t>(kQ4Block) << bpp_shift;
 
-  // Page ids, a lane per block, 64 blocks at a time and the next 64 on their way.
-  int pid = 0, pid_next = 0;
-  uint32_t batch = 0;
-  auto ids = [&](uint32_t k) -> int {
-    const uint32_t b = 64 * k + static_cast<uint32_t>(lane);
-    return b < nblk ? static_cast<int>(pt[(b0 + b) >> bpp_shift]) : 0;
+  // Page ids: kLong false, at most 64 blocks, a lane per block; else read a pair ahead of its use.
+  int pid = 0;
+  uint32_t ahead[2] = {0, 0};
+  auto page_at = [&](uint32_t b) -> uint32_t {
+    return pt[__builtin_amdgcn_readfirstlane((b0 + (b < nblk ? b : nblk - 1)) >> bpp_shift)];
   };
-  auto load = [&](Q4Regs& r, uint32_t b) {
+  struct Where {
+    size_t off;
+    bool valid;
+  };
+  auto where = [&](uint32_t b, int h) -> Where {
     const bool valid = b < nblk;
-    if (valid && (b >> 6) != batch) {  // uniform
-      pid = pid_next;
-      batch = b >> 6;
-      pid_next = ids(batch + 1);
+    uint32_t page;
+    if constexpr (kLong) {
+      page = ahead[h];
+      ahead[h] = page_at(b + 2);
+    } else {
+      page = static_cast<uint32_t>(__builtin_amdgcn_readlane(pid, static_cast<int>(b & 63)));
     }
-    const uint32_t page = static_cast<uint32_t>(__builtin_amdgcn_readlane(pid, static_cast<int>(b & 63)));
-    const size_t off = valid ? (static_cast<size_t>(page) * hkv + kh) * head_bytes + ((b0 + b) & bpp_mask) * static_cast<size_t>(kQ4Block) : 0;
-    q4_load<kPolicy>(r, kc + off, vc + off, valid, lane);
+    return {valid ? (static_cast<size_t>(page) * hkv + kh) * head_bytes + ((b0 + b) & bpp_mask) * static_cast<size_t>(kQ4Block) : 0, valid};
   };
-  Q4Regs s0[2], s1[2];
-  auto load_pair = [&](Q4Regs* r, uint32_t b) {
-    load(r[0], b);
-    load(r[1], b + 1);
+  Q4Half k[kSlots][2], v[kSlots][2];
+  Where at[kSlots][2];  // of the blocks whose V is to be loaded
+  auto load_k = [&](int s, uint32_t b) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      at[s][h] = where(b + h, h);
+      q4_load<kPolicy>(k[s][h], kc + at[s][h].off, at[s][h].valid, lane);
+    }
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto start = [&]() {
-    batch = 0;
-    pid = ids(0);
-    pid_next = nblk > 64 ? ids(1) : 0;
-    load_pair(s0, 0);
-    load_pair(s1, 2);
+  auto load_v = [&](int s) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) q4_load<kPolicy>(v[s][h], vc + at[s][h].off, at[s][h].valid, lane);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  if (nblk) start();
+  const int key_end = static_cast<int>((b0 + nblk) * 16);
+  floatx4 acc[NT][8];
+  uint32_t poison[NT];  // groups in which a row sees a step of NaN (slow runs)
+#pragma unroll
+  for (int t = 0; t < NT; ++t) poison[t] = 0;
 
-  // q as hi and lo parts, the factor from products to log2 scores.
-  half8 qh[NT][4], ql[NT][4];
-  float fac[NT];
-  int wmin = 0x7fffffff, wlo = 0;  // keys that every row of this wave sees: [wlo, wmin]
+  // One run over the blocks: all steps (kSlow false), or those from 1 up (scaled 2^-12), or the others,
+  // onto the first's results and with its maxima.
+  auto pass = [&](auto slow, bool small) {
+    constexpr bool kSlow = decltype(slow)::value;
+    if (nblk) {
+      if constexpr (kLong) {
+        ahead[0] = page_at(0);
+        ahead[1] = page_at(1);
+      } else {
+        pid = static_cast<uint32_t>(lane) < nblk ? static_cast<int>(pt[(b0 + lane) >> bpp_shift]) : 0;
+      }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float top = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float4 a = qraw[t][j];
-      top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
-    }
-    top = max_xor32(max_xor16(top));
-    const bool usable = has[t] && top > 0.0f && top < INFINITY;
-    const int ex = usable ? __builtin_amdgcn_frexp_expf(top) : 0;  // top < 2^ex
-    fac[t] = __builtin_ldexpf(scale_log2, ex - 13);
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const float4 a = qraw[t][2 * p], b = qraw[t][2 * p + 1];
-      const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = has[t] ? __builtin_ldexpf(x[e], 13 - ex) : 0.0f;
-        const float part = (e & 2) ? v * 0.0625f : v;
-        const _Float16 hi = static_cast<_Float16>(part);
-        qh[t][p][e] = hi;
-        ql[t][p][e] = static_cast<_Float16>(part - static_cast<float>(hi));
+      for (int s = 0; s < kSlots; ++s) {
+        load_k(s, 2 * s);
+        load_v(s);
       }
     }
-    int lo = has[t] ? rlo[t] : 0, hi = has[t] ? rpos[t] : 0x7fffffff;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-      lo = max(lo, __shfl_xor(lo, o));
-      hi = min(hi, __shfl_xor(hi, o));
-    }
-    wmin = min(wmin, __builtin_amdgcn_readfirstlane(hi));
-    wlo = max(wlo, __builtin_amdgcn_readfirstlane(lo));
-  }
-  const int key_end = static_cast<int>((b0 + nblk) * 16);
-
-  float room = kQ4Room;
-  for (;;) {
-    floatx4 acc[NT][8];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      w.m[t] = -INFINITY;
+      if (!small) w.m[t] = -INFINITY;
       w.l[t] = 0.0f;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) acc[t][n] = floatx4{0, 0, 0, 0};
+      for (int n = 0; n < 8; ++n) acc[t][n] = small ? acc[t][n] * 0x1p12f : floatx4{0, 0, 0, 0};
     }
-    auto compute = [&](auto masked, const Q4Regs* r, int key0) {
-      constexpr bool kMask = decltype(masked)::value;
-      half8 ka[2][4];
+    auto compute = [&](int s, uint32_t b, bool masked) {  // masked: uniform
+      const int key0 = static_cast<int>((b0 + b) * 16) + 4 * (lane >> 4);
+      u32x4 ph[NT], pl[NT];
+      floatx4 sc[NT][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) ka[h][p] = q4_k_codes(r[h].k[p]);
-      uint32_t vr[2][2][2];
-      q4_v_halves(r[0].v, vr[0]);
-      q4_v_halves(r[1].v, vr[1]);
-      auto v_tile = [&](auto n) -> half8 {
-        constexpr int N = decltype(n)::value;
-        return __builtin_bit_cast(half8, u32x4{q4_v_codes<N>(vr[0][0]), q4_v_codes<N>(vr[0][1]),
-                                               q4_v_codes<N>(vr[1][0]), q4_v_codes<N>(vr[1][1])});
-      };
+        for (int t = 0; t < NT; ++t) sc[t][h] = floatx4{0, 0, 0, 0};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const half8 ka = q4_k_codes(k[s][h].codes[p]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            floatx4 d = {0, 0, 0, 0};
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q(t, p, 0), d, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q(t, p, 1), d, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float step = static_cast<float>(__builtin_bit_cast(half8, k[s][h].steps[i >> 1])[(i & 1) * 4 + p]);
+              sc[t][h][i] = __builtin_fmaf(step, d[i], sc[t][h][i]);
+            }
+          }
+        }
+      }
+      load_k(s, b + 2 * kSlots);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float x[8];
         bool ok[8];
         float top = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          floatx4 sc = {0, 0, 0, 0};
+        for (int e = 0; e < 8; ++e) {
+          x[e] = sc[t][e >> 2][e & 3] * rows.fac[t];
+          ok[e] = true;
+        }
+        if (masked) {
 #pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            floatx4 d = {0, 0, 0, 0};
-            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[h][p], qh[t][p], d, 0, 0, 0);
-            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[h][p], ql[t][p], d, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[i] = __builtin_fmaf(q4_step(r[h].ks, i, p), d[i], sc[i]);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int e = h * 4 + i;
-            x[e] = sc[i] * fac[t];
-            if constexpr (kMask) {
-              const int key = key0 + h * 16 + 4 * (lane >> 4) + i;
-              ok[e] = (key >= rlo[t]) & (key <= rpos[t]) & (key < key_end);
-              x[e] = ok[e] ? x[e] : -INFINITY;
-            }
-            top = fmaxf(top, x[e]);
+          for (int e = 0; e < 8; ++e) {
+            const int key = key0 + (e >> 2) * 16 + (e & 3);
+            ok[e] = (key >= rows.lo[t]) & (key <= rows.pos[t]) & (key < key_end);
+            x[e] = ok[e] ? x[e] : -INFINITY;
           }
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
         if (__builtin_amdgcn_ballot_w64(top > w.m[t] + kQ4Lazy)) {
           const float mn = fmaxf(w.m[t], max_xor32(max_xor16(top)));
           const float corr = __builtin_amdgcn_exp2f(w.m[t] - fmaxf(mn, kLowest));
@@ -259,85 +258,183 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
 #pragma unroll
           for (int n = 0; n < 8; ++n) acc[t][n] *= corr;
         }
-        const float base = fmaxf(w.m[t], kLowest) - room;
-        float pr[8];
+        const float base = fmaxf(w.m[t], kLowest) - kQ4Room;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          pr[e] = __builtin_amdgcn_exp2f(x[e] - base);
-          w.l[t] += pr[e];
+          x[e] = __builtin_amdgcn_exp2f(x[e] - base);
+          w.l[t] += x[e];
         }
-        auto group = [&](auto pc) {
-          constexpr int p = decltype(pc)::value;
-          u32x4 hi, lo;
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            float y0 = pr[e] * q4_step(r[e >> 2].vs, e & 3, p), y1 = pr[e + 1] * q4_step(r[e >> 2].vs, (e & 3) + 1, p);
-            if constexpr (kMask) {
-              y0 = ok[e] ? y0 : 0.0f;
-              y1 = ok[e + 1] ? y1 : 0.0f;
+        for (int e = 0; e < 4; ++e) {
+          uint32_t hi, lo;
+          q4_cut(x[2 * e], x[2 * e + 1], hi, lo);
+          ph[t][e] = hi;
+          pl[t][e] = lo;
+        }
+        if constexpr (kSlow) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const float step = static_cast<float>(__builtin_bit_cast(half8, v[s][e >> 2].steps[p >> 1])[(p & 1) * 4 + (e & 3)]);
+              if (!(fabsf(step) < INFINITY) && ok[e]) poison[t] |= 1u << p;
             }
-            uint32_t a, b;
-            q4_cut(y0, y1, a, b);
-            hi[e / 2] = a;
-            lo[e / 2] = b;
-          }
-          const half8 ph = __builtin_bit_cast(half8, hi), pl = __builtin_bit_cast(half8, lo);
-          const half8 va = v_tile(std::integral_constant<int, 2 * p>{}), vb = v_tile(std::integral_constant<int, 2 * p + 1>{});
-          acc[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph, acc[t][2 * p], 0, 0, 0);
-          acc[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, ph, acc[t][2 * p + 1], 0, 0, 0);
-          acc[t][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl, acc[t][2 * p], 0, 0, 0);
-          acc[t][2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb, pl, acc[t][2 * p + 1], 0, 0, 0);
-        };
-        group(std::integral_constant<int, 0>{});
-        group(std::integral_constant<int, 1>{});
-        group(std::integral_constant<int, 2>{});
-        group(std::integral_constant<int, 3>{});
+        }
       }
-    };
-    auto pair = [&](const Q4Regs* r, uint32_t b) {
-      const int key0 = static_cast<int>((b0 + b) * 16);
-      if (key0 >= wlo && key0 + 31 <= wmin && key0 + 32 <= key_end)  // uniform
-        compute(std::false_type{}, r, key0);
-      else
-        compute(std::true_type{}, r, key0);
-    };
-    for (uint32_t b = 0; b < nblk; b += 4) {
-      pair(s0, b);
-      load_pair(s0, b + 4);
-      pair(s1, b + 2);
-      load_pair(s1, b + 6);
-    }
-    float bad = 0.0f;
+      if constexpr (kSlow) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            half8 st = __builtin_bit_cast(half8, v[s][h].steps[j]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float f = fabsf(static_cast<float>(st[e]));
+              const _Float16 big = st[e] * static_cast<_Float16>(0x1p-12f);
+              st[e] = small ? (f < 1.0f ? st[e] : static_cast<_Float16>(0.0f))
+                            : (f >= 1.0f && f < INFINITY ? big : static_cast<_Float16>(0.0f));
+            }
+            v[s][h].steps[j] = __builtin_bit_cast(u32x4, st);
+          }
+      }
+      if (masked) {  // keys no row sees
+        u32x2 seen[2];        // [block][keys 2 h, 2 h + 1]
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const int key = key0 + (e >> 2) * 16 + (e & 3);
+          const auto in = [&](int x) { return x >= rows.any_lo && x <= rows.any_pos; };
+          seen[e >> 2][(e >> 1) & 1] = (in(key) ? 0xffffu : 0u) | (in(key + 1) ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[s][h].steps[j >> 2][j & 3] &= seen[h][j & 1];
+      }
+      // V: halves of the four keys' dwords brought together, [block][keys 2 h, 2 h + 1][tiles 0-3, 4-7].
+      uint32_t vr[2][2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          vr[j][h][0] = __builtin_amdgcn_perm(v[s][j].codes[2 * h + 1], v[s][j].codes[2 * h], 0x05040100u);
+          vr[j][h][1] = __builtin_amdgcn_perm(v[s][j].codes[2 * h + 1], v[s][j].codes[2 * h], 0x07060302u);
+        }
+      auto tile = [&](auto nc) {
+        constexpr int n = decltype(nc)::value, p = n >> 1;
+        u32x4 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t word = vr[j][h][n >> 2];
+            const half2_q4 c = q4_codes<(n & 1) != 0>((n & 2) ? word >> 8 : word);
+            const half2_q4 st = __builtin_bit_cast(half2_q4, static_cast<uint32_t>(v[s][j].steps[p >> 1][(p & 1) * 2 + h]));
+            uint32_t product = __builtin_bit_cast(uint32_t, c * st);
+            pin(product);
+            hi[2 * j + h] = product;
+            lo[2 * j + h] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, st, -__builtin_bit_cast(half2_q4, product)));
+          }
+        const half8 vh = __builtin_bit_cast(half8, hi), vl = __builtin_bit_cast(half8, lo);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const half8 a = __builtin_bit_cast(half8, ph[t]), b2 = __builtin_bit_cast(half8, pl[t]);
+          acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, a, acc[t][n], 0, 0, 0);
+          acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, b2, acc[t][n], 0, 0, 0);
+          acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, a, acc[t][n], 0, 0, 0);
+        }
+      };
+      tile(std::integral_constant<int, 0>{});
+      tile(std::integral_constant<int, 1>{});
+      tile(std::integral_constant<int, 2>{});
+      tile(std::integral_constant<int, 3>{});
+      tile(std::integral_constant<int, 4>{});
+      tile(std::integral_constant<int, 5>{});
+      tile(std::integral_constant<int, 6>{});
+      tile(std::integral_constant<int, 7>{});
+      load_v(s);
+    };
+    for (uint32_t b = 0; b < nblk; b += 2 * kSlots) {
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) {
+        const uint32_t bs = b + 2 * s;
+        const int key0 = static_cast<int>((b0 + bs) * 16);
+        compute(s, bs, !(key0 >= rows.all_lo && key0 + 31 <= rows.all_pos && key0 + 32 <= key_end));
+      }
+    }
+  };
+  pass(std::false_type{}, false);
+  float bad = 0.0f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bad += acc[t][n][i] * 0.0f;
+  if (__builtin_amdgcn_ballot_w64(bad != 0.0f)) {  // an infinity or NaN
+    pass(std::true_type{}, false);
+    pass(std::true_type{}, true);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      uint32_t seen = poison[t];
+      seen |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(seen), 16));
+      seen |= static_cast<uint32_t>(__shfl_xor(static_cast<int>(seen), 32));
 #pragma unroll
       for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w.o[t][n][i] = acc[t][n][i] * (n & 1 ? 0.0625f : 1.0f);
-          bad += w.o[t][n][i] * 0.0f;
-        }
-    // An infinity or NaN: a step too large for the scale (or in the inputs). At most once.
-    if (room != kQ4Room || !__builtin_amdgcn_ballot_w64(bad != 0.0f)) break;
-    room = kQ4RoomBig;
-    start();
+        if (seen >> (n >> 1) & 1) acc[t][n] = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+    }
   }
-  // Weights relative to the maximum alike, whichever scale was taken.
-  const float unit = __builtin_amdgcn_exp2f(-room);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    w.l[t] = sum_xor32(sum_xor16(w.l[t])) * unit;
+    w.l[t] = sum_xor32(sum_xor16(w.l[t])) * __builtin_amdgcn_exp2f(-kQ4Room);
 #pragma unroll
-    for (int n = 0; n < 8; ++n) w.o[t][n] *= unit;
+    for (int n = 0; n < 8; ++n) w.o[t][n] = acc[t][n] * ((n & 1 ? 0.0625f : 1.0f) * __builtin_amdgcn_exp2f(-kQ4Room));
   }
 }
 
-// q of a logical row, this lane's dims 32 p + 8 g + 0 .. 7.
-__device__ __forceinline__ void q4_read_q(float4 (&raw)[8], const float* q, int g) {
+// This lane's part of a wave's rows: tile t's column is logical row lr0 + 16 t + c. Reads and
+// cuts q, a tile at a time: keep(t, hi, lo).
+template <int NT, typename Keep>
+__device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, uint32_t lr0, uint32_t r0, uint32_t nlog, uint32_t kh,
+                                        uint32_t G, uint32_t hq, const uint32_t* __restrict__ pos,
+                                        const float* __restrict__ q, uint32_t window, float scale_log2, int lane, Keep keep) {
+  const int c = lane & 15, g = lane >> 4;
+  rows.all_lo = 0;
+  rows.all_pos = 0x7fffffff;
+  rows.any_lo = 0x7fffffff;
+  rows.any_pos = -1;
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    raw[2 * p] = *reinterpret_cast<const float4*>(q + p * 32 + g * 8);
-    raw[2 * p + 1] = *reinterpret_cast<const float4*>(q + p * 32 + g * 8 + 4);
+  for (int t = 0; t < NT; ++t) {
+    const uint32_t lr = lr0 + t * 16 + c;
+    const bool has = lr < nlog;
+    const uint32_t lrc = has ? lr : 0;
+    const uint32_t rr = r0 + lrc / G, h = kh * G + lrc % G;
+    const int p = static_cast<int>(pos[rr]);
+    rows.has[t] = has;
+    rows.pos[t] = has ? p : -1;
+    rows.lo[t] = (window > 0 && p + 1 > static_cast<int>(window)) ? p + 1 - static_cast<int>(window) : 0;
+    const float* src = q + (static_cast<size_t>(rr) * hq + h) * kD + g * 8;
+    float4 raw[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      raw[2 * j] = *reinterpret_cast<const float4*>(src + j * 32);
+      raw[2 * j + 1] = *reinterpret_cast<const float4*>(src + j * 32 + 4);
+    }
+    half8 hi[4], lo[4];
+    rows.fac[t] = q4_cut_q(raw, has, scale_log2, hi, lo);
+    keep(t, hi, lo);
+    int lo_most = has ? rows.lo[t] : 0, lo_least = has ? rows.lo[t] : 0x7fffffff;
+    int pos_least = has ? p : 0x7fffffff, pos_most = has ? p : -1;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      lo_most = max(lo_most, __shfl_xor(lo_most, o));
+      lo_least = min(lo_least, __shfl_xor(lo_least, o));
+      pos_least = min(pos_least, __shfl_xor(pos_least, o));
+      pos_most = max(pos_most, __shfl_xor(pos_most, o));
+    }
+    rows.all_lo = max(rows.all_lo, __builtin_amdgcn_readfirstlane(lo_most));
+    rows.any_lo = min(rows.any_lo, __builtin_amdgcn_readfirstlane(lo_least));
+    rows.all_pos = min(rows.all_pos, __builtin_amdgcn_readfirstlane(pos_least));
+    rows.any_pos = max(rows.any_pos, __builtin_amdgcn_readfirstlane(pos_most));
   }
 }
 
@@ -362,23 +459,23 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
   const uint32_t wb0 = it.blk0 + nall * wave / kWideWaves;
   const uint32_t wb1 = it.blk0 + nall * (wave + 1) / kWideWaves;
 
-  int rpos[NT], rlo[NT];
-  bool has[NT];
-  float4 qraw[NT][8];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const uint32_t lr = t * 16 + c;
-    has[t] = lr < nlog;
-    const uint32_t lrc = has[t] ? lr : 0;
-    const uint32_t rr = it.r0 + lrc / G, h = kh * G + lrc % G;
-    const int p = static_cast<int>(pos[rr]);
-    rpos[t] = has[t] ? p : -1;
-    rlo[t] = (window > 0 && p + 1 > static_cast<int>(window)) ? p + 1 - static_cast<int>(window) : 0;
-    q4_read_q(qraw[t], q + (static_cast<size_t>(rr) * hq + h) * kD, g);
-  }
+  Q4Rows<NT> rows;
   Q4Wave<NT> w;
-  q4_attend<NT, kNontemporal>(w, kc, vc, pages + it.pt_off, wb0, wb1 - wb0, bpp_shift, kh, hkv, qraw, has, rpos, rlo,
-                              scale_log2, lane);
+  // q in LDS, in the space of the waves' results.
+  half8* const qs = reinterpret_cast<half8*>(&sh.o[0][0][0]);
+  static_assert(sizeof(sh.o) >= NT * 8 * 64 * sizeof(half8), "q fits");
+  q4_rows<NT>(rows, 0, it.r0, nlog, kh, G, hq, pos, q, window, scale_log2, lane, [&](int t, const half8* hi, const half8* lo) {
+    if (wave == t)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        qs[(t * 8 + p) * 64 + lane] = hi[p];
+        qs[(t * 8 + 4 + p) * 64 + lane] = lo[p];
+      }
+  });
+  __syncthreads();
+  q4_attend<NT, NT == 1 ? 2 : 1, false, kNontemporal>(w, kc, vc, pages + it.pt_off, wb0, wb1 - wb0, bpp_shift, kh, hkv, rows, lane,
+                                               [&](int t, int p, int part) { return qs[(t * 8 + part * 4 + p) * 64 + lane]; });
+  __syncthreads();  // every wave is done with q before any writes its result over it
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int lr = t * 16 + c;
@@ -386,7 +483,7 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
       sh.m[wave][lr] = w.m[t];
       sh.l[wave][lr] = w.l[t];
     }
-    if (has[t])
+    if (rows.has[t])
 #pragma unroll
       for (int n = 0; n < 8; ++n) sh.o[wave][lr][n * 4 + g] = __builtin_bit_cast(float4, w.o[t][n]);
   }
@@ -413,17 +510,20 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
   }, members);
 }
 
-// Prefill: a tile of 64 logical rows, 16 to each of 4 waves, over the item's blocks; the waves
-// read the blocks by themselves (the codes of a block are 2 KiB: they come from the CU's cache
-// for all but the first).
+// Prefill: a tile of kQ4TileRows logical rows, NT tiles of 16 to each of 4 waves, over the item's
+// blocks; the waves read the blocks by themselves (the codes of a block are 2 KiB: they come from
+// the CU's cache for all but the first). q lies in LDS, each wave's own.
 static constexpr int kQ4TileWaves = 4;
-static constexpr int kQ4TileRows = 64;
+static constexpr int kQ4WaveTiles = 2;
+static constexpr int kQ4TileRows = kQ4TileWaves * kQ4WaveTiles * 16;
 
 __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_prefill_q4(
     const PrefillItem* __restrict__ items, const uint32_t* __restrict__ pos, const uint32_t* __restrict__ pages,
     const q4_t* __restrict__ kc, const q4_t* __restrict__ vc, const float* __restrict__ q, float* __restrict__ out,
     uint32_t hq, uint32_t hkv, uint32_t bpp_shift, uint32_t window, float scale_log2, float* __restrict__ part_o,
     float2* __restrict__ part_ml, uint32_t* __restrict__ counters, uint32_t part_o_bytes, uint32_t part_ml_bytes) {
+  constexpr int NT = kQ4WaveTiles;
+  __shared__ half8 q_lds[kQ4TileWaves][NT * 8][64];
   const PrefillItem it = items[blockIdx.x / hkv];
   const uint32_t kh = blockIdx.x % hkv;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -431,47 +531,48 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
   const int c = lane & 15, g = lane >> 4;
   const uint32_t G = hq / hkv;
   const uint32_t nlog = it.nrows * G;  // at most kQ4TileRows
-  const uint32_t lr = wave * 16 + c;
-  const bool has[1] = {lr < nlog};
-  const uint32_t lrc = has[0] ? lr : 0;
-  const uint32_t rr = it.r0 + lrc / G, h = kh * G + lrc % G;
-  const int p = static_cast<int>(pos[rr]);
-  const int rpos[1] = {has[0] ? p : -1};
-  const int rlo[1] = {(window > 0 && p + 1 > static_cast<int>(window)) ? p + 1 - static_cast<int>(window) : 0};
-  float4 qraw[1][8];
-  q4_read_q(qraw[0], q + (static_cast<size_t>(rr) * hq + h) * kD, g);
-  // The blocks some row of this wave sees.
-  int first = has[0] ? rlo[0] : 0x7fffffff, last = rpos[0];
+  half8 (*const qs)[64] = q_lds[wave];
+  Q4Rows<NT> rows;
+  q4_rows<NT>(rows, wave * NT * 16, it.r0, nlog, kh, G, hq, pos, q, window, scale_log2, lane,
+              [&](int t, const half8* hi, const half8* lo) {
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    first = min(first, __shfl_xor(first, o));
-    last = max(last, __shfl_xor(last, o));
-  }
-  first = __builtin_amdgcn_readfirstlane(first);
-  last = __builtin_amdgcn_readfirstlane(last);
-  const uint32_t b0 = last < 0 ? it.blk0 : max(it.blk0, static_cast<uint32_t>(first) / 16);
-  const uint32_t b1 = last < 0 ? it.blk0 : min(it.blk1, static_cast<uint32_t>(last) / 16 + 1);
-  Q4Wave<1> w;
-  q4_attend<1, 0>(w, kc, vc, pages + it.pt_off, b0, b1 > b0 ? b1 - b0 : 0, bpp_shift, kh, hkv, qraw, has, rpos, rlo,
-                  scale_log2, lane);
+    for (int p = 0; p < 4; ++p) {
+      qs[t * 8 + p][lane] = hi[p];
+      qs[t * 8 + 4 + p][lane] = lo[p];
+    }
+  });
+  // The blocks some row of this wave sees.
+  const bool some = rows.any_pos >= 0;
+  const uint32_t b0 = some ? max(it.blk0, static_cast<uint32_t>(rows.any_lo) / 16) : it.blk0;
+  const uint32_t b1 = some ? min(it.blk1, static_cast<uint32_t>(rows.any_pos) / 16 + 1) : it.blk0;
+  Q4Wave<NT> w;
+  q4_attend<NT, 1, true, 0>(w, kc, vc, pages + it.pt_off, b0, b1 > b0 ? b1 - b0 : 0, bpp_shift, kh, hkv, rows, lane,
+                      [&](int t, int p, int part) { return qs[t * 8 + part * 4 + p][lane]; });
   const uint32_t nch = it.chunk_nch >> 16;
   if (nch <= 1) {
-    if (!has[0]) return;
-    float* o = out + (static_cast<size_t>(rr) * hq + h) * kD + g * 4;
-    const float inv = 1.0f / w.l[0];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) *reinterpret_cast<floatx4*>(o + n * 16) = w.o[0][n] * inv;
+    for (int t = 0; t < NT; ++t) {
+      if (!rows.has[t]) continue;
+      const uint32_t lr = (wave * NT + t) * 16 + c, rr = it.r0 + lr / G, h = kh * G + lr % G;
+      float* o = out + (static_cast<size_t>(rr) * hq + h) * kD + g * 4;
+      const float inv = 1.0f / w.l[t];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) *reinterpret_cast<floatx4*>(o + n * 16) = w.o[t][n] * inv;
+    }
     return;
   }
   // A tile split along keys: the hand-off of the other arenas' tiles (attn_prefill.hpp).
   const __amdgpu_buffer_rsrc_t ro = make_rsrc(part_o, part_o_bytes);
   const __amdgpu_buffer_rsrc_t rml = make_rsrc(part_ml, part_ml_bytes);
-  if (has[0]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (!rows.has[t]) continue;
+    const uint32_t lr = (wave * NT + t) * 16 + c;
     const size_t e = ((static_cast<size_t>(it.part_base) + (it.chunk_nch & 0xffffu)) * hkv + kh) * kQ4TileRows + lr;
 #pragma unroll
     for (int n = 0; n < 8; ++n)
-      st4_coherent(ro, static_cast<uint32_t>((e * kD + 16 * n + 4 * g) * 4), __builtin_bit_cast(float4, w.o[0][n]));
-    if (g == 0) st2_coherent(rml, static_cast<uint32_t>(e * 8), float2{w.m[0], w.l[0]});
+      st4_coherent(ro, static_cast<uint32_t>((e * kD + 16 * n + 4 * g) * 4), __builtin_bit_cast(float4, w.o[t][n]));
+    if (g == 0) st2_coherent(rml, static_cast<uint32_t>(e * 8), float2{w.m[t], w.l[t]});
   }
   __builtin_amdgcn_s_waitcnt(0);
   __shared__ uint32_t last_chunk;

@@ -17,7 +17,7 @@
 //   K: byte 16 l + 4 p: a dword of the 8 codes of key c, dims 32 p + 8 g + e, code e in the
 //      nibble (e / 2) + 4 (e % 2);
 //   V: byte 16 l + 4 i: a dword of the 8 codes of key 4 g + i, dims 16 n + c, code n in nibble n;
-//   steps: `[key][4 groups]` binary16.
+//   steps, binary16: K `[key][4 groups]`, V `[g][4 groups][4 keys]`.
 // Masks of 0x000f000f and 0x00f000f0 over a dword and over the dword shifted by 8 leave two codes
 // each in the halves of a register, a few bits from being a binary16 matrix operand.
 #pragma once
@@ -41,6 +41,9 @@ static constexpr float kQ4MaxStep = 65504.0f;
 // c, 16 + c, .. of key k.
 __host__ __device__ inline uint32_t q4_k_word(uint32_t c, uint32_t g, uint32_t p) { return (g * 16 + c) * 16 + p * 4; }
 __host__ __device__ inline uint32_t q4_v_word(uint32_t k, uint32_t c) { return ((k / 4) * 16 + c) * 16 + (k % 4) * 4; }
+// Index of the step of key k, group p, behind kQ4Steps.
+__host__ __device__ inline uint32_t q4_k_step(uint32_t k, uint32_t p) { return k * 4 + p; }
+__host__ __device__ inline uint32_t q4_v_step(uint32_t k, uint32_t p) { return (k / 4) * 16 + p * 4 + k % 4; }
 __host__ __device__ inline uint32_t q4_k_nibble(uint32_t e) { return e / 2 + 4 * (e % 2); }
 
 // A wave's 32-lane halves hold one group each: the group's step and this lane's code.
@@ -90,9 +93,9 @@ __device__ __forceinline__ void q4_store_k(float x0, float x1, uint32_t k, int l
     *reinterpret_cast<uint32_t*>(blk + q4_k_word(k, g, p + 2)) = c1;
   }
   if ((lane & 31) == 0) {
-    _Float16* st = reinterpret_cast<_Float16*>(blk + kQ4Steps) + k * 4 + p;
-    st[0] = s0;
-    st[2] = s1;
+    _Float16* st = reinterpret_cast<_Float16*>(blk + kQ4Steps);
+    st[q4_k_step(k, p)] = s0;
+    st[q4_k_step(k, p + 2)] = s1;
   }
 }
 
@@ -105,9 +108,9 @@ __device__ __forceinline__ void q4_store_v(float x0, float x1, uint32_t k, int l
   const uint32_t w = or_xor(or_xor((c0 << (4 * n)) | (c1 << (4 * n + 16)), 16), 32);
   if (lane < 16) *reinterpret_cast<uint32_t*>(blk + q4_v_word(k, lane)) = w;
   if ((lane & 31) == 0) {
-    _Float16* st = reinterpret_cast<_Float16*>(blk + kQ4Steps) + k * 4 + (lane >> 5);
-    st[0] = s0;
-    st[2] = s1;
+    _Float16* st = reinterpret_cast<_Float16*>(blk + kQ4Steps);
+    st[q4_v_step(k, lane >> 5)] = s0;
+    st[q4_v_step(k, (lane >> 5) + 2)] = s1;
   }
 }
 
@@ -149,7 +152,7 @@ __device__ __forceinline__ void kv_row_piece(const q4_t* kc, const q4_t* vc, boo
                                              uint32_t hkv, uint32_t page_shift, uint32_t ch, float* x) {
   const q4_t* blk = (is_k ? kc : vc) + q4_block_of(slot, kh, hkv, page_shift);
   const uint32_t key = slot & 15;
-  const float s = static_cast<float>(reinterpret_cast<const _Float16*>(blk + kQ4Steps)[key * 4 + ch / 4]);
+  const float s = static_cast<float>(reinterpret_cast<const _Float16*>(blk + kQ4Steps)[is_k ? q4_k_step(key, ch / 4) : q4_v_step(key, ch / 4)]);
   if (is_k) {
     const uint32_t w = *reinterpret_cast<const uint32_t*>(blk + q4_k_word(key, ch & 3, ch >> 2));
 #pragma unroll

@@ -607,7 +607,8 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_
     if (G > 16) use_prefill = max_rows * G > 16 && !must_fit;
   } else {
     size_t tiles = 0;
-    for (const Group& g : c->groups) tiles += (g.n * G + yx::kPrefillRows - 1) / yx::kPrefillRows;
+    const size_t per = q4 ? yx::kQ4TileRows : yx::kPrefillRows;
+    for (const Group& g : c->groups) tiles += (g.n * G + per - 1) / per;
     tiles *= hkv;
     use_prefill = max_rows * G > static_cast<size_t>(c->max_tiles) * 8 &&
                   tiles * 8 >= static_cast<size_t>(c->cus);
@@ -621,8 +622,7 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_
     plan.q4 = q4;
     // f32 tiles of 128 logical rows (option prefill_f32_waves: 4 takes 64, on f32 products).
     if (f32) plan.pf32_waves = c->pf32_waves ? static_cast<int>(c->pf32_waves) : 8;
-    static_assert(yx::kQ4TileRows == yx::kPrefillRows, "tiles of the 4-bit arena are cut as the binary16 arena's");
-    const size_t tile_rows = !f32 ? yx::kPrefillRows : plan.pf32_waves == 4 ? yx::kPf32SmallRows : yx::kPf32Rows;
+    const size_t tile_rows = q4 ? yx::kQ4TileRows : !f32 ? yx::kPrefillRows : plan.pf32_waves == 4 ? yx::kPf32SmallRows : yx::kPf32Rows;
     const uint32_t per = static_cast<uint32_t>(std::max<size_t>(1, tile_rows / G));
     // f32 partials hold the rows in use (a tile of few rows and many chunks).
     plan.part_rows = static_cast<uint32_t>(!f32 ? tile_rows : std::min<size_t>(tile_rows, max_rows * G));
@@ -2180,8 +2180,10 @@ static int page_io(yx_ctx* c, yx_kv* kv, size_t layer, const uint32_t* pages, si
       uint8_t* blk = arena + r / 16 * yx::kQ4Block;  // a head's keys fill whole blocks
       uint8_t* row = rows + r * yx::kQ4Row;
       const uint32_t key = static_cast<uint32_t>(r % 16);
-      uint8_t* st = blk + yx::kQ4Steps + key * 8;
-      std::memcpy(to_arena ? st : row + 64, to_arena ? row + 64 : st, 8);
+      for (uint32_t p = 0; p < 4; ++p) {
+        uint8_t* st = blk + yx::kQ4Steps + 2 * (is_k ? yx::q4_k_step(key, p) : yx::q4_v_step(key, p));
+        std::memcpy(to_arena ? st : row + 64 + 2 * p, to_arena ? row + 64 + 2 * p : st, 2);
+      }
       if (!to_arena) std::memset(row, 0, 64);
       for (uint32_t d = 0; d < 128; ++d) {
         const uint32_t word = is_k ? yx::q4_k_word(key, d / 8 % 4, d / 32) : yx::q4_v_word(key, d % 16);
