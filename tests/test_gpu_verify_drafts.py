@@ -145,6 +145,7 @@ def test_rows_without_a_distribution(hip, dist):
     x[off[0]] = -INF                       # nothing allowed at the first draft
     x[off[1] + 3] = np.nan                 # nor at the free row
     x[off[2], 17] = np.nan                 # NaN is masked
+    x.view(np.uint32)[off[4]:off[4] + 4, ::7] = 0x7f800001  # signalling ones too
     c["drafts"][6] = 17
     x[off[3] + 1, 4999] = INF              # takes all
     c["drafts"][10] = 4999

@@ -374,7 +374,7 @@ struct yx_ctx {
   // Rows of logits read in slices: the slices' sums and keys and the rows' arrival counters,
   // for logprobs_slots slices in all, allocated with the context too.
   DevBuf lp_keys, lp_parts, lp_counters;
-  DevBuf vd_parts, vd_stops, vd_sums, vd_counters;  // drafts verified: chunk sums, where each sequence stopped, arrivals
+  DevBuf vd_parts, vd_sums, vd_counters;  // drafts verified: chunk sums of rows and of residuals, arrivals
   uint64_t mm_kernel = 0, mm_k_parts = 0, mm_run_stages = 0;  // what the latest matmul ran (tests)
   // options
   long target_waves = 0;  // 0: one work item per CU
@@ -407,8 +407,7 @@ struct yx_ctx {
   uint64_t buffer_gens() const {
     uint64_t s = 0;
     for (const DevBuf* b : {&d_meta, &d_pages, &part_o, &part_ml, &counters, &io_a, &io_b, &io_c,
-                            &io_q, &am_keys, &am_counters, &mm_part, &mm_counters, &vd_parts, &vd_stops, &vd_sums,
-                            &vd_counters})
+                            &io_q, &am_keys, &am_counters, &mm_part, &mm_counters, &vd_parts, &vd_sums, &vd_counters})
       s += b->gen;
     return s;
   }
@@ -1971,7 +1970,7 @@ int yx_ctx_destroy(yx_ctx* c) {
   c->spare.clear();
   for (DevBuf* b : {&c->d_meta, &c->d_pages, &c->am_keys, &c->am_counters, &c->mm_part, &c->mm_counters,
                     &c->mt_part, &c->mt_counters, &c->lp_keys, &c->lp_parts, &c->lp_counters,
-                    &c->vd_parts, &c->vd_stops, &c->vd_sums, &c->vd_counters,
+                    &c->vd_parts, &c->vd_sums, &c->vd_counters,
                     &c->part_o, &c->part_ml, &c->counters,
                     &c->io_a, &c->io_b, &c->io_c, &c->io_q})
     b->release();
@@ -2889,11 +2888,9 @@ int yx_verify_drafts_dev(yx_ctx* c, const float* logits, size_t cols, size_t ld,
   const size_t part_bytes = part_rows * nch * sizeof(yx::VerifyPart), now = std::min<size_t>(seqs, yx::kVdSeqs);
   const size_t counter_bytes = yx::kVdSeqs * 4 * yx::kCounterStride;
   if ((rc = c->vd_parts.ensure(part_bytes, c->stream))) return rc;
-  if ((rc = c->vd_stops.ensure(yx::kVdSeqs * sizeof(yx::VerifyStop), c->stream))) return rc;
   if ((rc = c->vd_sums.ensure(now * nch * sizeof(double), c->stream))) return rc;
   if ((rc = c->vd_counters.ensure(counter_bytes, c->stream, true))) return rc;
   auto* parts = static_cast<yx::VerifyPart*>(c->vd_parts.p);
-  auto* stops = static_cast<yx::VerifyStop*>(c->vd_stops.p);
   auto* counters = static_cast<uint32_t*>(c->vd_counters.p);
   for (size_t i = 0; i + 1 < cuts.size(); ++i) {
     const size_t a = cuts[i], n = cuts[i + 1] - a, row0 = row_off[a], d0 = row0 - a;
@@ -2904,10 +2901,10 @@ int yx_verify_drafts_dev(yx_ctx* c, const float* logits, size_t cols, size_t ld,
                           temperature ? temperature + a : nullptr, nd ? accept_u + d0 : nullptr, pick_u + a, ld, draft_ld,
                           static_cast<uint32_t>(cols), static_cast<uint32_t>(nch)};
     hipLaunchKernelGGL(yx::verify_sums, dim3(static_cast<unsigned>(nch), static_cast<unsigned>(launch_rows(a, a + n))),
-                       dim3(yx::kVdThreads), 0, c->stream, vr, in, parts, part_bytes, stops, counters, accepted + a, next + a);
-    if (in.dlogits)
-      hipLaunchKernelGGL(yx::verify_residual, dim3(static_cast<unsigned>(nch), static_cast<unsigned>(n)), dim3(yx::kVdThreads), 0,
-                         c->stream, vr, in, parts, part_bytes, stops, static_cast<double*>(c->vd_sums.p), counters, next + a);
+                       dim3(yx::kVdSumThreads), 0, c->stream, vr, in, parts);
+    hipLaunchKernelGGL(yx::verify_pick, dim3(in.dlogits ? static_cast<unsigned>(nch) : 1u, static_cast<unsigned>(n)),
+                       dim3(yx::kVdThreads), 0, c->stream, vr, in, parts, static_cast<double*>(c->vd_sums.p), counters,
+                       accepted + a, next + a);
   }
   YX_HIP(hipGetLastError());
   return YX_OK;

@@ -15,12 +15,13 @@
 // polynomial of 12 terms here, about 20 operations a logit: at 64-bit rates 4 us for 80 rows of
 // 151936 logits, less than the 9 us that reading them takes.
 //
-// Launch 1: every chunk of 4096 logits (target and draft rows) gives its maximum M_c and
-// sum e^((l - M_c) / t); a sequence's last chunk to arrive adds them up, decides, and draws where
-// one row's chunk sums say enough (accepted all, certain drafts, temperature 0): the chunk by its
-// cumulative sum, then the token within it. Launch 2 (drafts with logits, sequences with a
-// rejected one): the residual's sum per chunk, the last to arrive draws from them. Chunk order
-// fixes every sum's order: the same answer every time.
+// Launch 1 reads every chunk of 4096 logits (target and draft rows): its maximum M_c and
+// sum e^((l - M_c) / t). Launch 2, a workgroup per sequence (per chunk and sequence where drafts
+// have logits): adds the chunks up and decides, every workgroup of a sequence by itself; then draws
+// where one row's chunk sums say enough (accepted all, certain drafts, temperature 0): the chunk by
+// its cumulative sum, then the token within it. Where they don't, each workgroup adds up its chunk
+// of the residual and the last of the sequence to arrive draws. Chunk order fixes every sum's
+// order: the same answer every time.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -31,9 +32,13 @@
 
 namespace yx {
 
-static constexpr int kVdThreads = 256;
-static constexpr int kVdQuads = 4;                                     // 16-byte loads a thread and chunk
-static constexpr uint32_t kVdChunk = kVdThreads * kVdQuads * 4;        // logits
+static constexpr int kVdSumThreads = 256, kVdSumQuads = 4;             // launch 1: 16-byte loads a thread
+// Launch 2: one 16-byte load a thread. Four times the logits in a quarter of the threads is four
+// times the code, which a launch this short fetches more slowly than it runs it (7 us a chunk of
+// both rows' weights).
+static constexpr int kVdThreads = 1024;
+static constexpr int kVdWaves = kVdThreads / 64;
+static constexpr uint32_t kVdChunk = kVdThreads * 4;                   // logits
 static constexpr uint32_t kVdMaxChunks = 1024;
 static constexpr uint32_t kVdSeqs = 256;                               // sequences of a launch
 
@@ -59,20 +64,15 @@ struct VerifyPart {  // a chunk: sum of weights relative to its maximum, that ma
   uint32_t at;
 };
 
-// Where a sequence stopped.
-struct VerifyStop {
-  double ip, iq;      // 1 / W of the row and of the draft's row
-  double c;           // log2(e) / temperature (-1: temperature 0)
-  float mp, mq;       // their maxima
-  uint32_t row, drow;
-  uint32_t drawn;     // the next token is drawn already
-};
-
-// 2^t, t <= 0, within 2^-50: 2^f by its series (|f| <= 1/2, the next term below 2^-51).
+// 2^t, t <= 0 (below -1000, and NaN: 2^-1000), within 2^-47: the whole part n of t goes into the
+// exponent, 2^f by its series (|f| <= 1/2: the first term left out is below 2^-47). 17 operations,
+// all at full rate: the rounding by a large addend instead of rndne, the exponent by an integer
+// addition instead of ldexp.
 __device__ __forceinline__ double vd_exp2(double t) {
-  t = fmax(t, -1100.0);  // (and NaN)
-  const double n = __builtin_rint(t), f = t - n;
-  constexpr double k[13] = {1.0,
+  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52: the sum's last bit is worth 1
+  t = fmax(t, -1000.0);
+  const double r = t + kWhole, f = t - (r - kWhole);
+  constexpr double k[12] = {1.0,
                             6.93147180559945286e-01,
                             2.40226506959100694e-01,
                             5.55041086648215762e-02,
@@ -83,12 +83,14 @@ __device__ __forceinline__ double vd_exp2(double t) {
                             1.32154867901443053e-06,
                             1.01780860092396960e-07,
                             7.05491162080112188e-09,
-                            4.44553827187081007e-10,
-                            2.56784359934881958e-11};  // ln(2)^i / i!
-  double p = k[12];
+                            4.44553827187081007e-10};  // ln(2)^i / i!
+  double p = k[11];
 #pragma unroll
-  for (int i = 11; i >= 0; --i) p = __builtin_fma(p, f, k[i]);
-  return __builtin_ldexp(p, static_cast<int>(n));
+  for (int i = 10; i >= 0; --i) p = __builtin_fma(p, f, k[i]);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, p);
+  const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, r));
+  const uint32_t hi = static_cast<uint32_t>(bits >> 32) + (n << 20);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | static_cast<uint32_t>(bits));
 }
 
 // Weight of a logit relative to the maximum m (above -inf), c = log2(e) / temperature.
@@ -103,59 +105,65 @@ __device__ __forceinline__ double vd_c(const VerifyIn& in, uint32_t seq) {
   return t > 0.0f ? 1.4426950408889634 / static_cast<double>(t) : -1.0;
 }
 
-// This thread's 16 logits of a chunk: quad i holds elements 4 (i * 256 + thread) of the chunk;
-// -inf past the row's end and for NaN.
-__device__ __forceinline__ void vd_load(f32x4 (&v)[kVdQuads], const float* row, uint32_t cols, uint32_t chunk) {
-  const uint32_t e0 = chunk * kVdChunk;
-  if (e0 + kVdChunk <= cols) {  // uniform
-#pragma unroll
-    for (int i = 0; i < kVdQuads; ++i)
-      v[i] = *reinterpret_cast<const f32x4_any*>(row + e0 + 4 * (i * kVdThreads + threadIdx.x));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVdQuads; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t e = e0 + 4 * (i * kVdThreads + threadIdx.x) + j;
-        v[i][j] = e < cols ? row[e] : -INFINITY;
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < kVdQuads; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[i][j] = v[i][j] == v[i][j] ? v[i][j] : -INFINITY;
+// This thread's 4 logits of a chunk; -inf past the row's end.
+__device__ __forceinline__ f32x4 vd_load(const float* row, uint32_t cols, uint32_t chunk) {
+  const uint32_t e = chunk * kVdChunk + 4 * threadIdx.x;
+  if (e + 4 <= cols) return *reinterpret_cast<const f32x4_any*>(row + e);
+  f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if (e < cols) v.x = row[e];
+  if (e + 1 < cols) v.y = row[e + 1];
+  if (e + 2 < cols) v.z = row[e + 2];
+  return v;
 }
 
 __device__ __forceinline__ double vd_shfl_xor(double x, int o) { return __shfl_xor(x, o); }
 
+static constexpr uint32_t kVdBatch = 64;  // drafts decided at once
+
 struct VerifyShared {
   double mass[kVdMaxChunks];
-  double sum[kVdQuads][4];  // [sub-block][wave]
-  double row_w[2 * 64];     // W of a batch's target and draft rows
-  float row_m[2 * 64];
-  uint32_t row_at[2 * 64];
-  double total;
-  float m[4];
-  uint32_t at[4];
-  uint32_t chunk, first, last_pos, flag;
-  VerifyStop stop;
+  double sum[kVdWaves];
+  double row_w[2 * kVdBatch + 2];  // W of a batch's target rows, then of its drafts'
+  float row_m[2 * kVdBatch + 2];
+  uint32_t row_at[kVdBatch + 1];
+  double before;
+  float m[kVdWaves];
+  uint32_t at[kVdWaves], last[kVdWaves];
+  uint32_t flag;
 };
+
+// Inclusive sums over the lanes of a wave.
+__device__ __forceinline__ double vd_scan(double x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
 
 // Sum over the workgroup, to all threads, in a fixed order.
 __device__ __forceinline__ double vd_sum(VerifyShared& sh, double x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x += vd_shfl_xor(x, o);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.sum[0][threadIdx.x >> 6] = x;
+  if ((threadIdx.x & 63) == 0) sh.sum[threadIdx.x >> 6] = x;
   __syncthreads();
-  return (sh.sum[0][0] + sh.sum[0][1]) + (sh.sum[0][2] + sh.sum[0][3]);
+  x = sh.sum[threadIdx.x & (kVdWaves - 1)];
+#pragma unroll
+  for (int o = kVdWaves / 2; o > 0; o >>= 1) x += vd_shfl_xor(x, o);
+  return x;
 }
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t vd_rsrc(void* p, size_t bytes) {
-  return make_rsrc(p, static_cast<uint32_t>(bytes));
+// Inclusive sums over the waves, of sh.sum (a sum per wave): lane i has that of waves 0 to i.
+__device__ __forceinline__ double vd_waves(const VerifyShared& sh, int lane) {
+  const double own = sh.sum[lane & (kVdWaves - 1)];
+  return vd_scan(lane < kVdWaves ? own : 0.0, lane);
 }
-__device__ __forceinline__ VerifyPart vd_part(__amdgpu_buffer_rsrc_t r, uint32_t i) {
-  return __builtin_bit_cast(VerifyPart, ld4_coherent(r, i * 16));
+// That of the waves before `wave`.
+__device__ __forceinline__ double vd_before(double waves, int wave) {
+  const double b = __shfl(waves, wave ? wave - 1 : 0);
+  return wave ? b : 0.0;
 }
 
 // What a draw weighs: p of a row, p without one token, or the residual of p and q.
@@ -174,272 +182,354 @@ struct VerifyDraw {
 };
 
 // This thread's weights of a chunk.
-__device__ __forceinline__ void vd_weights(double (&w)[kVdQuads][4], const VerifyDraw& d, uint32_t cols, uint32_t chunk) {
-  f32x4 a[kVdQuads], b[kVdQuads];
-  vd_load(a, d.x, cols, chunk);
-  if (d.y) vd_load(b, d.y, cols, chunk);
+__device__ __forceinline__ void vd_weights(double (&w)[4], const VerifyDraw& d, uint32_t cols, uint32_t chunk) {
+  const f32x4 a = vd_load(d.x, cols, chunk);
+  f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (d.y) b = vd_load(d.y, cols, chunk);
 #pragma unroll
-  for (int i = 0; i < kVdQuads; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w[i][j] = d.weight(a[i][j], d.y ? b[i][j] : 0.0f, chunk * kVdChunk + 4 * (i * kVdThreads + threadIdx.x) + j);
+  for (int j = 0; j < 4; ++j) w[j] = d.weight(a[j], b[j], chunk * kVdChunk + 4 * threadIdx.x + j);
 }
 
 __device__ __forceinline__ double vd_chunk_sum(VerifyShared& sh, const VerifyDraw& d, uint32_t cols, uint32_t chunk) {
-  double w[kVdQuads][4], s = 0.0;
+  double w[4];
   vd_weights(w, d, cols, chunk);
-#pragma unroll
-  for (int i = 0; i < kVdQuads; ++i) s += (w[i][0] + w[i][1]) + (w[i][2] + w[i][3]);
-  return vd_sum(sh, s);
+  return vd_sum(sh, (w[0] + w[1]) + (w[2] + w[3]));
+}
+
+// Of a wave whose lanes hold rising indexes: the first lane's that has one (YX_NO_TOKEN: none), and
+// the last lane's. (Ballots: LDS atomics of divergent lanes become loops over the lanes, 20 us a draw.)
+__device__ __forceinline__ uint32_t vd_first(uint32_t i) {
+  const uint64_t has = __builtin_amdgcn_ballot_w64(i != YX_NO_TOKEN);
+  return has ? static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(i), __builtin_ctzll(has))) : YX_NO_TOKEN;
+}
+__device__ __forceinline__ uint32_t vd_last(uint32_t i) {
+  const uint64_t has = __builtin_amdgcn_ballot_w64(i != YX_NO_TOKEN);
+  return has ? static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(i), 63 - __builtin_clzll(has))) : YX_NO_TOKEN;
+}
+
+// Of the workgroup, whose threads hold rising indexes: the first thread's that has one, else the
+// last of `last` (YX_NO_TOKEN: neither), to all threads.
+__device__ __forceinline__ uint32_t vd_choose(VerifyShared& sh, uint32_t first, uint32_t last) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  first = vd_first(first);
+  last = vd_last(last);
+  if (lane == 0) {
+    sh.at[wave] = first;
+    sh.last[wave] = last;
+  }
+  __syncthreads();
+  first = vd_first(lane < kVdWaves ? sh.at[lane] : YX_NO_TOKEN);
+  last = vd_last(lane < kVdWaves ? sh.last[lane] : YX_NO_TOKEN);
+  return first != YX_NO_TOKEN ? first : last;
 }
 
 // The token at v among the weights of d, whose chunk sums lie in sh.mass[0 .. nch): the first
 // whose cumulative sum exceeds v times the whole, the last with any weight where none does (v not
 // below 1); YX_NO_TOKEN where there is no weight. All threads call it and have the result.
 __device__ __forceinline__ uint32_t vd_draw(VerifyShared& sh, const VerifyDraw& d, uint32_t cols, uint32_t nch, float v) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double total = 0.0;
-    uint32_t last = YX_NO_TOKEN;
-    for (uint32_t c = 0; c < nch; ++c) {
-      total += sh.mass[c];
-      if (sh.mass[c] > 0.0) last = c;
-    }
-    const double target = static_cast<double>(v) * total;
-    uint32_t c = 0;
-    double before = 0.0;  // the sum of the chunks before c
-    if (last != YX_NO_TOKEN)
-      for (; c < last && !(sh.mass[c] > 0.0 && before + sh.mass[c] > target); ++c) before += sh.mass[c];
-    sh.chunk = last == YX_NO_TOKEN ? YX_NO_TOKEN : c;
-    sh.total = target - before;
-    sh.first = YX_NO_TOKEN;
-    sh.last_pos = 0;
-  }
-  __syncthreads();
-  const uint32_t chunk = sh.chunk;
-  if (chunk == YX_NO_TOKEN) return YX_NO_TOKEN;  // uniform
-  const double target = sh.total;                // within the chunk
-  double w[kVdQuads][4];
-  vd_weights(w, d, cols, chunk);
+  static_assert(kVdMaxChunks <= kVdThreads, "a thread per chunk");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double own[kVdQuads], upto[kVdQuads];  // a thread's sum of a sub-block of 1024, and that of the wave's lanes up to it
-#pragma unroll
-  for (int i = 0; i < kVdQuads; ++i) {
-    own[i] = (w[i][0] + w[i][1]) + (w[i][2] + w[i][3]);
-    double x = own[i];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
-    upto[i] = x;
-    if (lane == 63) sh.sum[i][wave] = x;
-  }
   __syncthreads();
-  double base = 0.0;
-#pragma unroll
-  for (int i = 0; i < kVdQuads; ++i) {
-    double before = base;
-    for (int k = 0; k < wave; ++k) before += sh.sum[i][k];
-    double sum = before + (upto[i] - own[i]);
-    uint32_t first = YX_NO_TOKEN, last = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t e = chunk * kVdChunk + 4 * (i * kVdThreads + threadIdx.x) + j;
-      sum += w[i][j];
-      if (w[i][j] > 0.0) {
-        last = e + 1;
-        if (sum > target && first == YX_NO_TOKEN) first = e;
-      }
-    }
-    if (first != YX_NO_TOKEN) atomicMin(&sh.first, first);
-    if (last) atomicMax(&sh.last_pos, last);
-    base += (sh.sum[i][0] + sh.sum[i][1]) + (sh.sum[i][2] + sh.sum[i][3]);
-  }
+  double mass = sh.mass[threadIdx.x & (kVdMaxChunks - 1)];
+  mass = threadIdx.x < nch ? mass : 0.0;
+  double upto = vd_scan(mass, lane);
+  if (lane == 63) sh.sum[wave] = upto;
   __syncthreads();
-  return sh.first != YX_NO_TOKEN ? sh.first : sh.last_pos - 1;
+  double waves = vd_waves(sh, lane);
+  upto += vd_before(waves, wave);
+  double target = static_cast<double>(v) * __shfl(waves, kVdWaves - 1);
+  const bool some = mass > 0.0;
+  const uint32_t chunk = vd_choose(sh, some && upto > target ? threadIdx.x : YX_NO_TOKEN, some ? threadIdx.x : YX_NO_TOKEN);
+  if (chunk == YX_NO_TOKEN) return chunk;  // uniform: no weight
+  if (threadIdx.x == chunk) sh.before = upto - mass;
+  double w[4];
+  vd_weights(w, d, cols, chunk);
+  const double own = (w[0] + w[1]) + (w[2] + w[3]);
+  upto = vd_scan(own, lane);
+  __syncthreads();  // (every wave has read the chunks' sums)
+  if (lane == 63) sh.sum[wave] = upto;
+  __syncthreads();
+  target -= sh.before;  // within the chunk
+  waves = vd_waves(sh, lane);
+  double sum = upto - own + vd_before(waves, wave);
+  uint32_t first = YX_NO_TOKEN, last = YX_NO_TOKEN;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t e = chunk * kVdChunk + 4 * threadIdx.x + j;
+    sum += w[j];
+    if (w[j] > 0.0) {
+      last = e;
+      if (sum > target && first == YX_NO_TOKEN) first = e;
+    }
+  }
+  return vd_choose(sh, first, last);
 }
 
 // Chunk masses of a row (relative to its maximum m) from its parts, into sh.mass.
-__device__ __forceinline__ void vd_masses(VerifyShared& sh, __amdgpu_buffer_rsrc_t parts, uint32_t row, uint32_t nch,
-                                          float m, double c) {
-  for (uint32_t i = threadIdx.x; i < nch; i += kVdThreads) {
-    const VerifyPart p = vd_part(parts, row * nch + i);
+__device__ __forceinline__ void vd_masses(VerifyShared& sh, const VerifyPart* __restrict__ parts, uint32_t nch, float m,
+                                          double c) {
+  if (const uint32_t i = threadIdx.x; i < nch) {
+    const VerifyPart p = parts[i];
     sh.mass[i] = p.m > -INFINITY ? p.s * vd_weight(p.m, m, c) : 0.0;
   }
 }
 
 // Launch 1. Grid: (chunks, target rows + draft rows). parts: a VerifyPart per (row, chunk),
-// target rows first; counters: one per sequence, zero on entry and left at zero.
-__global__ __launch_bounds__(kVdThreads) void verify_sums(VerifyRows rows, VerifyIn in, VerifyPart* __restrict__ parts,
-                                                          size_t part_bytes, VerifyStop* __restrict__ stops,
-                                                          uint32_t* __restrict__ counters,
-                                                          uint32_t* __restrict__ accepted, uint32_t* __restrict__ next) {
-  __shared__ VerifyShared sh;
+// target rows first.
+__global__ __launch_bounds__(kVdSumThreads) void verify_sums(VerifyRows rows, VerifyIn in, VerifyPart* __restrict__ parts) {
+  constexpr int kWaves = kVdSumThreads / 64;
+  static_assert(kVdSumThreads * kVdSumQuads * 4 == kVdChunk && kWaves == 4, "a chunk of logits a workgroup");
+  __shared__ float ms[kWaves];
+  __shared__ double ss[kWaves];
+  __shared__ uint32_t ns[kWaves];
   const uint32_t chunk = blockIdx.x, r = blockIdx.y, nrows = rows.off[rows.seqs];
   const bool draft = r >= nrows;
-  // The sequence of the row: target row off[s] + i; draft off[s] - s + i.
-  uint32_t lo = 0, hi = rows.seqs;  // off[lo] <= row < off[hi]
-  const uint32_t mine = draft ? r - nrows : r;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (rows.off[mid] - (draft ? mid : 0) <= mine) lo = mid;
-    else hi = mid;
-  }
-  const uint32_t seq = lo, row0 = rows.off[seq], k = rows.off[seq + 1] - row0 - 1, draft0 = row0 - seq;
-  const double c = vd_c(in, seq);
-  const __amdgpu_buffer_rsrc_t pr = vd_rsrc(parts, part_bytes);
+  const uint32_t mine = draft ? r - nrows : r, e0 = chunk * kVdChunk;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-
-  if (!draft || c >= 0.0) {  // uniform: a draft's own distribution does not count at temperature 0
-    f32x4 v[kVdQuads];
-    vd_load(v, draft ? in.dlogits + mine * in.dld : in.logits + mine * in.ld, in.cols, chunk);
-    float m = -INFINITY;
+  const float* row = draft ? in.dlogits + mine * in.dld : in.logits + mine * in.ld;
+  f32x4 v[kVdSumQuads];
 #pragma unroll
-    for (int i = 0; i < kVdQuads; ++i) m = fmaxf(m, fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w)));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if (lane == 0) sh.m[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sh.m[0], sh.m[1]), fmaxf(sh.m[2], sh.m[3]));
-    double s = 0.0;
-    uint32_t at = YX_NO_TOKEN;
-    if (c >= 0.0) {
-      if (m > -INFINITY)
-#pragma unroll
-        for (int i = 0; i < kVdQuads; ++i) {
-          double t[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) t[j] = vd_weight(v[i][j], m, c);
-          s += (t[0] + t[1]) + (t[2] + t[3]);
-        }
-      s = vd_sum(sh, s);
-    } else {  // the first of the largest
-#pragma unroll
-      for (int i = 0; i < kVdQuads; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (v[i][j] == m) at = min(at, chunk * kVdChunk + 4 * (i * kVdThreads + threadIdx.x) + j);
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) at = min(at, static_cast<uint32_t>(__shfl_xor(static_cast<int>(at), o)));
-      if (lane == 0) sh.at[wave] = at;
-      __syncthreads();
-      at = min(min(sh.at[0], sh.at[1]), min(sh.at[2], sh.at[3]));
+  for (int i = 0; i < kVdSumQuads; ++i) {
+    const uint32_t e = e0 + 4 * (i * kVdSumThreads + threadIdx.x);
+    v[i] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (e + 4 <= in.cols) {
+      v[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(row + e));
+    } else {
+      if (e < in.cols) v[i].x = row[e];
+      if (e + 1 < in.cols) v[i].y = row[e + 1];
+      if (e + 2 < in.cols) v[i].z = row[e + 2];
     }
-    if (threadIdx.x == 0) st4_coherent(pr, (r * in.nch + chunk) * 16, __builtin_bit_cast(float4, VerifyPart{s, m, at}));
   }
-  // Arrival (the memory order of the attention's split-K hand-off, attn_decode.hpp).
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    uint32_t* cnt = counters + static_cast<size_t>(seq) * kCounterStride;
-    const uint32_t all = in.nch * (k + 1 + (in.dlogits ? k : 0));
-    const uint32_t arrived = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    sh.flag = arrived == all - 1;
-    if (sh.flag) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // The sequence of the row: target row off[s] + i; draft off[s] - s + i. (Read as a lane per
+  // sequence while the logits are on their way.)
+  {
+    const uint32_t s = threadIdx.x;
+    const bool before = s < rows.seqs && rows.off[s] - (draft ? s : 0) <= mine;
+    const uint32_t n = __popcll(__builtin_amdgcn_ballot_w64(before));
+    if (lane == 0) ns[wave] = n;
   }
+  static_assert(kVdSeqs <= kVdSumThreads, "a thread per sequence");
   __syncthreads();
-  if (!sh.flag) return;
+  // (Of sequences without drafts, which share their draft offset with the next, the last.)
+  const uint32_t seq = __builtin_amdgcn_readfirstlane(ns[0] + ns[1] + ns[2] + ns[3]) - 1;
+  const double c = vd_c(in, seq);
+  if (draft && c < 0.0) return;  // uniform: a draft's own distribution does not count at temperature 0
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kVdSumQuads; ++i) m = fmaxf(m, fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w)));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (lane == 0) ms[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+  double s = 0.0;
+  uint32_t at = YX_NO_TOKEN;
+  const bool plain = c > 0x1p-100 && m > -INFINITY && m < INFINITY;  // masked tokens then add 2^-1000 at most
+  if (c < 0.0 || !plain) {
+    // Temperature 0: the first of the largest. A row of nothing, +inf, temperatures beyond 2^100: the exact form.
+#pragma unroll
+    for (int i = 0; i < 4 * kVdSumQuads; ++i) {
+      const float x = v[i / 4][i % 4];
+      if (c < 0.0) {
+        if (x == m && m > -INFINITY) at = min(at, e0 + 4 * (i / 4 * kVdSumThreads + threadIdx.x) + i % 4);
+      } else if (m == INFINITY) {
+        s += x == m ? 1.0 : 0.0;
+      } else if (m > -INFINITY) {
+        s += vd_weight(x, m, c);
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) at = min(at, static_cast<uint32_t>(__shfl_xor(static_cast<int>(at), o)));
+    if (lane == 0) ns[wave] = at;
+  } else {
+    const double md = static_cast<double>(m);
+#pragma unroll 1
+    for (int i = 0; i < kVdSumQuads; ++i) {
+      double t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = vd_exp2((static_cast<double>(v[0][j]) - md) * c);
+      s += (t[0] + t[1]) + (t[2] + t[3]);
+#pragma unroll
+      for (int j = 0; j + 1 < kVdSumQuads; ++j) v[j] = v[j + 1];  // (a loop a quarter as long)
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += vd_shfl_xor(s, o);
+  if (lane == 0) ss[wave] = s;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    parts[static_cast<size_t>(r) * in.nch + chunk] =
+        VerifyPart{(ss[0] + ss[1]) + (ss[2] + ss[3]), m, c < 0.0 ? min(min(ns[0], ns[1]), min(ns[2], ns[3])) : YX_NO_TOKEN};
+}
 
-  // The sequence's decision. A batch of up to 64 drafts: each wave adds up a row's chunks.
+// Launch 2. Grid: (chunks where drafts have logits, else 1; sequences). sums: a residual's sum per
+// (sequence, chunk); counters: one per sequence, zero on entry and left at zero.
+__global__ __launch_bounds__(kVdThreads) void verify_pick(VerifyRows rows, VerifyIn in, const VerifyPart* __restrict__ parts,
+                                                          double* __restrict__ sums, uint32_t* __restrict__ counters,
+                                                          uint32_t* __restrict__ accepted, uint32_t* __restrict__ next) {
+  __shared__ VerifyShared sh;
+  const uint32_t chunk = blockIdx.x, seq = blockIdx.y, nrows = rows.off[rows.seqs];
+  const uint32_t row0 = rows.off[seq], k = rows.off[seq + 1] - row0 - 1, draft0 = row0 - seq;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const double c = vd_c(in, seq);
+  const bool dist = in.dlogits != nullptr && c >= 0.0;
+  // The sequence's decision, up to 64 drafts at once: each wave adds up rows' chunks, two at a
+  // time on their way, while a thread per draft has its token, number and logits brought.
   uint32_t taken = 0;  // accepted
   bool stopped = false;
   double wp = 0.0, wq = 0.0;
   float mp = -INFINITY, mq = -INFINITY;
   uint32_t best = YX_NO_TOKEN;
-  for (uint32_t b = 0; b <= k && !stopped; b += 64) {  // uniform
-    const uint32_t n = min(64u, k + 1 - b);            // rows of this batch (the last may be the free one)
+  for (uint32_t b = 0; b <= k && !stopped; b += kVdBatch) {  // uniform
+    const uint32_t n = min(kVdBatch, k - b);                 // drafts of this batch
+    const uint32_t nt = min(n + 1, k + 1 - b), all = nt + (dist ? n : 0);  // target rows, the free one's among them at the end
+    uint32_t x = YX_NO_TOKEN;
+    float u = 0.0f, a = -INFINITY, y = -INFINITY;
+    if (threadIdx.x < n) {
+      x = in.drafts[draft0 + b + threadIdx.x];
+      u = in.u[draft0 + b + threadIdx.x];
+      if (x < in.cols) {
+        a = in.logits[(row0 + b + threadIdx.x) * in.ld + x];
+        if (dist) y = in.dlogits[(draft0 + b + threadIdx.x) * in.dld + x];
+      }
+    }
     __syncthreads();
-    for (uint32_t i = wave; i < 2 * n; i += 4) {
-      const bool q = i >= n;
-      const uint32_t j = b + (q ? i - n : i);
-      double w = 0.0;
-      float m = -INFINITY;
-      uint32_t at = YX_NO_TOKEN;
-      if (!q || (in.dlogits && j < k && c >= 0.0)) {
-        const uint32_t pr_row = q ? nrows + draft0 + j : row0 + j;
-        for (uint32_t h = lane; h < in.nch; h += 64) {
-          const VerifyPart p = vd_part(pr, pr_row * in.nch + h);
-          if (p.m > m) at = p.at;
-          if (c >= 0.0 && p.m > -INFINITY) {
-            const float mn = fmaxf(m, p.m);
-            w = (m > -INFINITY ? w * vd_weight(m, mn, c) : 0.0) + p.s * vd_weight(p.m, mn, c);
-          }
-          m = fmaxf(m, p.m);
+    for (uint32_t i0 = wave; i0 < all; i0 += 2 * kVdWaves) {
+      double w[2];
+      float m[2];
+      uint32_t at[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const uint32_t i = i0 + kVdWaves * g, pr_row = i < nt ? row0 + b + i : nrows + draft0 + b + (i - nt);
+        w[g] = 0.0;
+        m[g] = -INFINITY;
+        at[g] = YX_NO_TOKEN;
+        if (i >= all) continue;  // uniform
+        VerifyPart p{0.0, -INFINITY, YX_NO_TOKEN};
+        if (static_cast<uint32_t>(lane) < in.nch) p = parts[static_cast<size_t>(pr_row) * in.nch + lane];
+        w[g] = p.s;
+        m[g] = p.m;
+        at[g] = p.at;
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const uint32_t i = i0 + kVdWaves * g, pr_row = i < nt ? row0 + b + i : nrows + draft0 + b + (i - nt);
+        if (i >= all) continue;
+        for (uint32_t h = lane + 64; h < in.nch; h += 64) {  // more than 64 chunks
+          const VerifyPart p = parts[static_cast<size_t>(pr_row) * in.nch + h];
+          if (p.m > m[g]) at[g] = p.at;
+          const float mn = fmaxf(m[g], p.m);
+          if (c >= 0.0 && mn > -INFINITY)
+            w[g] = (m[g] > -INFINITY ? w[g] * vd_weight(m[g], mn, c) : 0.0) + (p.m > -INFINITY ? p.s * vd_weight(p.m, mn, c) : 0.0);
+          m[g] = mn;
         }
-        float top = m;
+        float top = m[g];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        if (m != top || top == -INFINITY) at = YX_NO_TOKEN;
-        w = m > -INFINITY ? w * vd_weight(m, top, c) : 0.0;
+        if (c >= 0.0) {
+          double s = m[g] > -INFINITY ? w[g] * vd_weight(m[g], top, c) : 0.0;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-          w += vd_shfl_xor(w, o);
-          at = min(at, static_cast<uint32_t>(__shfl_xor(static_cast<int>(at), o)));
+          for (int o = 32; o > 0; o >>= 1) s += vd_shfl_xor(s, o);
+          w[g] = s;
+        } else {
+          uint32_t f = m[g] == top && top > -INFINITY ? at[g] : YX_NO_TOKEN;
+#pragma unroll
+          for (int o = 32; o > 0; o >>= 1) f = min(f, static_cast<uint32_t>(__shfl_xor(static_cast<int>(f), o)));
+          at[g] = f;
         }
-        m = top;
-      }
-      if (lane == 0) {
-        sh.row_w[i] = w;
-        sh.row_m[i] = m;
-        sh.row_at[i] = at;
+        if (lane == 0) {
+          const uint32_t to = i < nt ? i : kVdBatch + 1 + (i - nt);
+          sh.row_w[to] = w[g];
+          sh.row_m[to] = top;
+          if (i < nt) sh.row_at[i] = at[g];
+        }
       }
     }
     __syncthreads();
-    for (uint32_t i = 0; i < n; ++i) {  // uniform
-      const uint32_t j = b + i;
-      wp = sh.row_w[i];
-      mp = sh.row_m[i];
-      best = sh.row_at[i];
-      wq = sh.row_w[n + i];
-      mq = sh.row_m[n + i];
-      if (j == k) break;
-      const uint32_t x = in.drafts[draft0 + j];
+    if (wave == 0) {
       bool ok = false;
-      if (c < 0.0) {
-        ok = x == best && best != YX_NO_TOKEN;
-      } else if (x < in.cols && mp > -INFINITY) {
-        const float a = in.logits[(row0 + j) * in.ld + x];
-        const double p = vd_weight(a, mp, c) / wp;
-        double q = 1.0;
-        if (in.dlogits) q = mq > -INFINITY ? vd_weight(in.dlogits[(draft0 + j) * in.dld + x], mq, c) / wq : 0.0;
-        ok = static_cast<double>(in.u[draft0 + j]) * q < p;
+      if (threadIdx.x < n) {
+        const uint32_t i = threadIdx.x;
+        const float m = sh.row_m[i];
+        if (c < 0.0) {
+          ok = x == sh.row_at[i] && x != YX_NO_TOKEN;
+        } else if (x < in.cols && m > -INFINITY) {
+          const double p = vd_weight(a, m, c) / sh.row_w[i];
+          double q = 1.0;
+          if (dist) {
+            const float md = sh.row_m[kVdBatch + 1 + i];
+            q = md > -INFINITY ? vd_weight(y, md, c) / sh.row_w[kVdBatch + 1 + i] : 0.0;
+          }
+          ok = static_cast<double>(u) * q < p;
+        }
       }
-      if (!ok) {
-        stopped = true;
-        break;
-      }
-      ++taken;
+      const uint64_t stand = __builtin_amdgcn_ballot_w64(ok);
+      const uint32_t first = ~stand ? static_cast<uint32_t>(__builtin_ctzll(~stand)) : 64u;
+      if (lane == 0) sh.flag = min(first, n);
     }
+    __syncthreads();
+    const uint32_t i = sh.flag;
+    taken = b + i;
+    stopped = i < n;
+    if (!stopped && taken < k) continue;  // the next batch
+    wp = sh.row_w[i];
+    mp = sh.row_m[i];
+    best = sh.row_at[i];
+    if (dist && stopped) {
+      wq = sh.row_w[kVdBatch + 1 + i];
+      mq = sh.row_m[kVdBatch + 1 + i];
+    }
+    break;
   }
   const uint32_t row = row0 + taken, drow = draft0 + taken;
-  const bool residual = stopped && in.dlogits != nullptr && c >= 0.0 && mp > -INFINITY && mq > -INFINITY;
-  if (threadIdx.x == 0) {
-    accepted[seq] = taken;
-    stops[seq] = VerifyStop{mp > -INFINITY ? 1.0 / wp : 0.0, mq > -INFINITY ? 1.0 / wq : 0.0, c, mp, mq, row, drow, residual ? 0u : 1u};
-  }
-  if (residual) return;
-  uint32_t token = best;  // temperature 0
-  if (c >= 0.0) {
-    token = YX_NO_TOKEN;
-    if (mp > -INFINITY) {
-      VerifyDraw d{in.logits + row * in.ld, nullptr, c, 1.0, 0.0, mp, mq, YX_NO_TOKEN};
+  if (chunk == 0 && threadIdx.x == 0) accepted[seq] = taken;
+  VerifyDraw d{in.logits + row * in.ld, nullptr, c, 1.0, 0.0, mp, mq, YX_NO_TOKEN};
+  const VerifyPart* const row_parts = parts + static_cast<size_t>(row) * in.nch;
+  uint32_t token = YX_NO_TOKEN;
+  if (stopped && dist && mp > -INFINITY && mq > -INFINITY) {
+    d.y = in.dlogits + drow * in.dld;
+    d.ip = 1.0 / wp;
+    d.iq = 1.0 / wq;
+    const double s = vd_chunk_sum(sh, d, in.cols, chunk);
+    double* const mine = sums + static_cast<size_t>(seq) * in.nch;
+    // Arrival (the memory order of the attention's split-K hand-off, attn_decode.hpp).
+    if (threadIdx.x == 0) {
+      __hip_atomic_store(mine + chunk, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __builtin_amdgcn_s_waitcnt(0);
+      uint32_t* cnt = counters + static_cast<size_t>(seq) * kCounterStride;
+      const uint32_t arrived = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sh.flag = arrived == in.nch - 1;
+      if (sh.flag) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!sh.flag) return;
+    if (const uint32_t i = threadIdx.x; i < in.nch)
+      sh.mass[i] = __hip_atomic_load(mine + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
+    if (token == YX_NO_TOKEN) {  // p nowhere above q: p itself
+      d.y = nullptr;
       __syncthreads();
-      vd_masses(sh, pr, row, in.nch, mp, c);
+      vd_masses(sh, row_parts, in.nch, mp, c);
+      token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
+    }
+  } else {
+    if (chunk != 0) return;
+    if (c < 0.0) {
+      token = best;  // temperature 0
+    } else if (mp > -INFINITY) {
       __syncthreads();
+      vd_masses(sh, row_parts, in.nch, mp, c);
       const uint32_t x = stopped ? in.drafts[drow] : YX_NO_TOKEN;
       if (stopped && in.dlogits == nullptr && x < in.cols) {
         // Without the rejected token: its chunk added up anew (taken away, it could leave only
         // rounding errors).
         d.without = x;
         const double s = vd_chunk_sum(sh, d, in.cols, x / kVdChunk);
-        __syncthreads();
         const double kept = sh.mass[x / kVdChunk];
         __syncthreads();
         if (threadIdx.x == 0) sh.mass[x / kVdChunk] = s;
         token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
         if (token == YX_NO_TOKEN) {  // nothing else has weight: p itself
-          __syncthreads();
           if (threadIdx.x == 0) sh.mass[x / kVdChunk] = kept;
           d.without = YX_NO_TOKEN;
           token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
@@ -448,41 +538,6 @@ __global__ __launch_bounds__(kVdThreads) void verify_sums(VerifyRows rows, Verif
         token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
       }
     }
-  }
-  if (threadIdx.x == 0) next[seq] = token;
-}
-
-// Launch 2. Grid: (chunks, sequences). sums: a residual's sum per (sequence, chunk).
-__global__ __launch_bounds__(kVdThreads) void verify_residual(VerifyRows rows, VerifyIn in, VerifyPart* __restrict__ parts,
-                                                              size_t part_bytes, const VerifyStop* __restrict__ stops,
-                                                              double* __restrict__ sums,
-                                                              uint32_t* __restrict__ counters,
-                                                              uint32_t* __restrict__ next) {
-  __shared__ VerifyShared sh;
-  const uint32_t chunk = blockIdx.x, seq = blockIdx.y;
-  const VerifyStop st = stops[seq];
-  if (st.drawn) return;  // uniform
-  VerifyDraw d{in.logits + st.row * in.ld, in.dlogits + st.drow * in.dld, st.c, st.ip, st.iq, st.mp, st.mq, YX_NO_TOKEN};
-  const double s = vd_chunk_sum(sh, d, in.cols, chunk);
-  double* mine = sums + static_cast<size_t>(seq) * in.nch;
-  if (threadIdx.x == 0) {
-    __hip_atomic_store(mine + chunk, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __builtin_amdgcn_s_waitcnt(0);
-    uint32_t* cnt = counters + static_cast<size_t>(seq) * kCounterStride;
-    const uint32_t arrived = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    sh.flag = arrived == in.nch - 1;
-    if (sh.flag) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (!sh.flag) return;
-  for (uint32_t i = threadIdx.x; i < in.nch; i += kVdThreads)
-    sh.mass[i] = __hip_atomic_load(mine + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  uint32_t token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
-  if (token == YX_NO_TOKEN) {  // p nowhere above q: p itself
-    d.y = nullptr;
-    __syncthreads();
-    vd_masses(sh, vd_rsrc(parts, part_bytes), st.row, in.nch, st.mp, st.c);
-    token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
   }
   if (threadIdx.x == 0) next[seq] = token;
 }
