@@ -116,7 +116,40 @@ __device__ __forceinline__ f32x4 vd_load(const float* row, uint32_t cols, uint32
   return v;
 }
 
-__device__ __forceinline__ double vd_shfl_xor(double x, int o) { return __shfl_xor(x, o); }
+// A lane's neighbour by a data-parallel-primitive control, 0 where it has none (or kRows leaves its
+// row of 16 out). These are register moves, where a shuffle goes through LDS (100 cycles a step).
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ double vd_dpp(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(b), kCtrl, kRows, 0xf, true));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), kCtrl, kRows, 0xf, true));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Inclusive sums over the lanes of a row of 16, and of the wave.
+__device__ __forceinline__ double vd_scan16(double x) {
+  x += vd_dpp<0x111>(x);  // row_shr:1, 2, 4, 8
+  x += vd_dpp<0x112>(x);
+  x += vd_dpp<0x114>(x);
+  x += vd_dpp<0x118>(x);
+  return x;
+}
+__device__ __forceinline__ double vd_scan(double x) {
+  x = vd_scan16(x);
+  x += vd_dpp<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  x += vd_dpp<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
+__device__ __forceinline__ double vd_lane(double x, int lane) {  // uniform lane
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b), lane));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The wave's sum.
+__device__ __forceinline__ double vd_wave_sum(double x) { return vd_lane(vd_scan(x), 63); }
 
 static constexpr uint32_t kVdBatch = 64;  // drafts decided at once
 
@@ -132,38 +165,14 @@ struct VerifyShared {
   uint32_t flag;
 };
 
-// Inclusive sums over the lanes of a wave.
-__device__ __forceinline__ double vd_scan(double x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
-
 // Sum over the workgroup, to all threads, in a fixed order.
 __device__ __forceinline__ double vd_sum(VerifyShared& sh, double x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += vd_shfl_xor(x, o);
+  static_assert(kVdWaves == 16, "the waves' sums are a row of lanes");
+  x = vd_wave_sum(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh.sum[threadIdx.x >> 6] = x;
   __syncthreads();
-  x = sh.sum[threadIdx.x & (kVdWaves - 1)];
-#pragma unroll
-  for (int o = kVdWaves / 2; o > 0; o >>= 1) x += vd_shfl_xor(x, o);
-  return x;
-}
-
-// Inclusive sums over the waves, of sh.sum (a sum per wave): lane i has that of waves 0 to i.
-__device__ __forceinline__ double vd_waves(const VerifyShared& sh, int lane) {
-  const double own = sh.sum[lane & (kVdWaves - 1)];
-  return vd_scan(lane < kVdWaves ? own : 0.0, lane);
-}
-// That of the waves before `wave`.
-__device__ __forceinline__ double vd_before(double waves, int wave) {
-  const double b = __shfl(waves, wave ? wave - 1 : 0);
-  return wave ? b : 0.0;
+  return vd_lane(vd_scan16(sh.sum[threadIdx.x & (kVdWaves - 1)]), kVdWaves - 1);
 }
 
 // What a draw weighs: p of a row, p without one token, or the residual of p and q.
@@ -181,19 +190,18 @@ struct VerifyDraw {
   }
 };
 
-// This thread's weights of a chunk.
-__device__ __forceinline__ void vd_weights(double (&w)[4], const VerifyDraw& d, uint32_t cols, uint32_t chunk) {
-  const f32x4 a = vd_load(d.x, cols, chunk);
-  f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (d.y) b = vd_load(d.y, cols, chunk);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = d.weight(a[j], b[j], chunk * kVdChunk + 4 * threadIdx.x + j);
+// This thread's logits of a chunk, and their weights.
+struct VerifyLogits {
+  f32x4 a, b;
+};
+__device__ __forceinline__ VerifyLogits vd_logits(const VerifyDraw& d, uint32_t cols, uint32_t chunk) {
+  VerifyLogits l{vd_load(d.x, cols, chunk), f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+  if (d.y) l.b = vd_load(d.y, cols, chunk);
+  return l;
 }
-
-__device__ __forceinline__ double vd_chunk_sum(VerifyShared& sh, const VerifyDraw& d, uint32_t cols, uint32_t chunk) {
-  double w[4];
-  vd_weights(w, d, cols, chunk);
-  return vd_sum(sh, (w[0] + w[1]) + (w[2] + w[3]));
+__device__ __forceinline__ void vd_weights(double (&w)[4], const VerifyDraw& d, const VerifyLogits& l, uint32_t chunk) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = d.weight(l.a[j], l.b[j], chunk * kVdChunk + 4 * threadIdx.x + j);
 }
 
 // Of a wave whose lanes hold rising indexes: the first lane's that has one (YX_NO_TOKEN: none), and
@@ -228,30 +236,30 @@ __device__ __forceinline__ uint32_t vd_choose(VerifyShared& sh, uint32_t first, 
 // below 1); YX_NO_TOKEN where there is no weight. All threads call it and have the result.
 __device__ __forceinline__ uint32_t vd_draw(VerifyShared& sh, const VerifyDraw& d, uint32_t cols, uint32_t nch, float v) {
   static_assert(kVdMaxChunks <= kVdThreads, "a thread per chunk");
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   __syncthreads();
   double mass = sh.mass[threadIdx.x & (kVdMaxChunks - 1)];
   mass = threadIdx.x < nch ? mass : 0.0;
-  double upto = vd_scan(mass, lane);
+  double upto = vd_scan(mass);
   if (lane == 63) sh.sum[wave] = upto;
   __syncthreads();
-  double waves = vd_waves(sh, lane);
-  upto += vd_before(waves, wave);
-  double target = static_cast<double>(v) * __shfl(waves, kVdWaves - 1);
+  double waves = vd_scan16(sh.sum[lane & (kVdWaves - 1)]);  // lane i: of waves 0 to i
+  if (wave) upto += vd_lane(waves, wave - 1);
+  double target = static_cast<double>(v) * vd_lane(waves, kVdWaves - 1);
   const bool some = mass > 0.0;
   const uint32_t chunk = vd_choose(sh, some && upto > target ? threadIdx.x : YX_NO_TOKEN, some ? threadIdx.x : YX_NO_TOKEN);
   if (chunk == YX_NO_TOKEN) return chunk;  // uniform: no weight
   if (threadIdx.x == chunk) sh.before = upto - mass;
   double w[4];
-  vd_weights(w, d, cols, chunk);
+  vd_weights(w, d, vd_logits(d, cols, chunk), chunk);
   const double own = (w[0] + w[1]) + (w[2] + w[3]);
-  upto = vd_scan(own, lane);
+  upto = vd_scan(own);
   __syncthreads();  // (every wave has read the chunks' sums)
   if (lane == 63) sh.sum[wave] = upto;
   __syncthreads();
   target -= sh.before;  // within the chunk
-  waves = vd_waves(sh, lane);
-  double sum = upto - own + vd_before(waves, wave);
+  waves = vd_scan16(sh.sum[lane & (kVdWaves - 1)]);
+  double sum = upto - own + (wave ? vd_lane(waves, wave - 1) : 0.0);
   uint32_t first = YX_NO_TOKEN, last = YX_NO_TOKEN;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -353,8 +361,7 @@ __global__ __launch_bounds__(kVdSumThreads) void verify_sums(VerifyRows rows, Ve
       for (int j = 0; j + 1 < kVdSumQuads; ++j) v[j] = v[j + 1];  // (a loop a quarter as long)
     }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += vd_shfl_xor(s, o);
+  s = vd_wave_sum(s);
   if (lane == 0) ss[wave] = s;
   __syncthreads();
   if (threadIdx.x == 0)
@@ -362,13 +369,14 @@ __global__ __launch_bounds__(kVdSumThreads) void verify_sums(VerifyRows rows, Ve
         VerifyPart{(ss[0] + ss[1]) + (ss[2] + ss[3]), m, c < 0.0 ? min(min(ns[0], ns[1]), min(ns[2], ns[3])) : YX_NO_TOKEN};
 }
 
-// Launch 2. Grid: (chunks where drafts have logits, else 1; sequences). sums: a residual's sum per
-// (sequence, chunk); counters: one per sequence, zero on entry and left at zero.
+// Launch 2. Grid: (shares of a sequence's chunks, `per` chunks each, where drafts have logits, else
+// 1; sequences). sums: a residual's sum per (sequence, chunk); counters: one per sequence, zero on
+// entry and left at zero.
 __global__ __launch_bounds__(kVdThreads) void verify_pick(VerifyRows rows, VerifyIn in, const VerifyPart* __restrict__ parts,
-                                                          double* __restrict__ sums, uint32_t* __restrict__ counters,
+                                                          uint32_t per, double* __restrict__ sums, uint32_t* __restrict__ counters,
                                                           uint32_t* __restrict__ accepted, uint32_t* __restrict__ next) {
   __shared__ VerifyShared sh;
-  const uint32_t chunk = blockIdx.x, seq = blockIdx.y, nrows = rows.off[rows.seqs];
+  const uint32_t share = blockIdx.x, seq = blockIdx.y, nrows = rows.off[rows.seqs];
   const uint32_t row0 = rows.off[seq], k = rows.off[seq + 1] - row0 - 1, draft0 = row0 - seq;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const double c = vd_c(in, seq);
@@ -427,10 +435,7 @@ __global__ __launch_bounds__(kVdThreads) void verify_pick(VerifyRows rows, Verif
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
         if (c >= 0.0) {
-          double s = m[g] > -INFINITY ? w[g] * vd_weight(m[g], top, c) : 0.0;
-#pragma unroll
-          for (int o = 32; o > 0; o >>= 1) s += vd_shfl_xor(s, o);
-          w[g] = s;
+          w[g] = vd_wave_sum(m[g] > -INFINITY ? w[g] * vd_weight(m[g], top, c) : 0.0);
         } else {
           uint32_t f = m[g] == top && top > -INFINITY ? at[g] : YX_NO_TOKEN;
 #pragma unroll
@@ -482,61 +487,67 @@ __global__ __launch_bounds__(kVdThreads) void verify_pick(VerifyRows rows, Verif
     break;
   }
   const uint32_t row = row0 + taken, drow = draft0 + taken;
-  if (chunk == 0 && threadIdx.x == 0) accepted[seq] = taken;
-  VerifyDraw d{in.logits + row * in.ld, nullptr, c, 1.0, 0.0, mp, mq, YX_NO_TOKEN};
-  const VerifyPart* const row_parts = parts + static_cast<size_t>(row) * in.nch;
-  uint32_t token = YX_NO_TOKEN;
-  if (stopped && dist && mp > -INFINITY && mq > -INFINITY) {
-    d.y = in.dlogits + drow * in.dld;
-    d.ip = 1.0 / wp;
-    d.iq = 1.0 / wq;
-    const double s = vd_chunk_sum(sh, d, in.cols, chunk);
+  if (share == 0 && threadIdx.x == 0) accepted[seq] = taken;
+  const bool residual = stopped && dist && mp > -INFINITY && mq > -INFINITY;
+  if (!residual && share != 0) return;  // uniform
+  uint32_t token = best;                // temperature 0
+  if (c >= 0.0) token = YX_NO_TOKEN;
+  if (c >= 0.0 && mp > -INFINITY) {
+    VerifyDraw d{in.logits + row * in.ld, nullptr, c, 1.0, 0.0, mp, mq, YX_NO_TOKEN};
+    const VerifyPart* const row_parts = parts + static_cast<size_t>(row) * in.nch;
+    if (residual) {
+      d.y = in.dlogits + drow * in.dld;
+      d.ip = 1.0 / wp;
+      d.iq = 1.0 / wq;
+    } else if (stopped && in.dlogits == nullptr) {
+      const uint32_t x = in.drafts[drow];
+      if (x < in.cols) d.without = x;
+    }
+    // The residual's sum in this chunk; or that of p without the rejected token in its chunk (added
+    // up anew: taken away, it could leave only rounding errors).
+    const bool without = d.without != YX_NO_TOKEN;
+    double s = 0.0;
     double* const mine = sums + static_cast<size_t>(seq) * in.nch;
-    // Arrival (the memory order of the attention's split-K hand-off, attn_decode.hpp).
-    if (threadIdx.x == 0) {
-      __hip_atomic_store(mine + chunk, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __builtin_amdgcn_s_waitcnt(0);
-      uint32_t* cnt = counters + static_cast<size_t>(seq) * kCounterStride;
-      const uint32_t arrived = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      sh.flag = arrived == in.nch - 1;
-      if (sh.flag) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!sh.flag) return;
-    if (const uint32_t i = threadIdx.x; i < in.nch)
-      sh.mass[i] = __hip_atomic_load(mine + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
-    if (token == YX_NO_TOKEN) {  // p nowhere above q: p itself
-      d.y = nullptr;
-      __syncthreads();
-      vd_masses(sh, row_parts, in.nch, mp, c);
-      token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
-    }
-  } else {
-    if (chunk != 0) return;
-    if (c < 0.0) {
-      token = best;  // temperature 0
-    } else if (mp > -INFINITY) {
-      __syncthreads();
-      vd_masses(sh, row_parts, in.nch, mp, c);
-      const uint32_t x = stopped ? in.drafts[drow] : YX_NO_TOKEN;
-      if (stopped && in.dlogits == nullptr && x < in.cols) {
-        // Without the rejected token: its chunk added up anew (taken away, it could leave only
-        // rounding errors).
-        d.without = x;
-        const double s = vd_chunk_sum(sh, d, in.cols, x / kVdChunk);
-        const double kept = sh.mass[x / kVdChunk];
-        __syncthreads();
-        if (threadIdx.x == 0) sh.mass[x / kVdChunk] = s;
-        token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
-        if (token == YX_NO_TOKEN) {  // nothing else has weight: p itself
-          if (threadIdx.x == 0) sh.mass[x / kVdChunk] = kept;
-          d.without = YX_NO_TOKEN;
-          token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
-        }
-      } else {
-        token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
+    if (residual || without) {
+      const uint32_t first = residual ? share * per : d.without / kVdChunk, end = residual ? min(in.nch, first + per) : first + 1;
+      VerifyLogits l = vd_logits(d, in.cols, first);
+#pragma unroll 1
+      for (uint32_t chunk = first; chunk < end; ++chunk) {
+        const VerifyLogits now = l;
+        if (chunk + 1 < end) l = vd_logits(d, in.cols, chunk + 1);
+        double w[4];
+        vd_weights(w, d, now, chunk);
+        s = vd_sum(sh, (w[0] + w[1]) + (w[2] + w[3]));
+        if (residual && threadIdx.x == 0) __hip_atomic_store(mine + chunk, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
+    }
+    if (residual) {
+      // Arrival (the memory order of the attention's split-K hand-off, attn_decode.hpp).
+      if (threadIdx.x == 0) {
+        __builtin_amdgcn_s_waitcnt(0);
+        uint32_t* cnt = counters + static_cast<size_t>(seq) * kCounterStride;
+        const uint32_t arrived = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh.flag = arrived == gridDim.x - 1;
+        if (sh.flag) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+      if (!sh.flag) return;
+      if (const uint32_t i = threadIdx.x; i < in.nch)
+        sh.mass[i] = __hip_atomic_load(mine + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+      vd_masses(sh, row_parts, in.nch, mp, c);
+      __syncthreads();
+      if (without && threadIdx.x == 0) sh.mass[d.without / kVdChunk] = s;
+    }
+#pragma unroll 1
+    for (int more = residual || without ? 1 : 0;; --more) {
+      token = vd_draw(sh, d, in.cols, in.nch, in.v[seq]);
+      if (token != YX_NO_TOKEN || more == 0) break;  // uniform
+      // Nothing is left (p nowhere above q, or the rejected token is all): p itself.
+      d.y = nullptr;
+      d.without = YX_NO_TOKEN;
+      __syncthreads();
+      vd_masses(sh, row_parts, in.nch, mp, c);
     }
   }
   if (threadIdx.x == 0) next[seq] = token;
