@@ -440,31 +440,35 @@ class HipBackend:
         `[seqs]` or None (1), pick_u `[seqs]`. Returns (accepted, next), uint32 `[seqs]`: ``out``,
         or new device tensors."""
         off = np.ascontiguousarray(row_off, np.uint32)
-        if off.ndim != 1 or len(off) < 1:
+        if off.ndim != 1 or off.size < 1:
             raise ValueError("row_off holds every sequence's first row and the end of the last")
-        seqs, rows = len(off) - 1, int(off[-1])
-        nd = rows - seqs
-        ld = logits.shape[1]
-        cols = ld if cols is None else cols
-        out = out if out is not None else tuple(self.tensor((seqs,), np.uint32) for _ in range(2))
-        if logits.shape[0] < rows:
+        seqs, rows = off.size - 1, int(off[-1])
+        nd, (have, ld) = rows - seqs, logits.shape
+        if have < rows:
             raise ValueError("fewer rows of logits than row_off names")
-        if nd > 0 and (drafts is None or accept_u is None):
-            raise ValueError("drafts without their tokens or numbers")
-        if draft_logits is not None and draft_logits.shape[0] < nd:
-            raise ValueError("fewer rows of draft logits than drafts")
         _need(logits, rows * ld * 4, "logits")
+        if nd > 0:
+            if drafts is None or accept_u is None:
+                raise ValueError("drafts without their tokens or numbers")
+            _need(drafts, nd * 4, "drafts")
+            _need(accept_u, nd * 4, "accept_u")
+        dl, dld = None, 0
         if draft_logits is not None:
-            _need(draft_logits, nd * draft_logits.shape[1] * 4, "draft_logits")
-        for t, n, what in ((drafts, nd, "drafts"), (accept_u, nd, "accept_u"), (pick_u, seqs, "pick_u"),
-                           (temperature, seqs, "temperature"), (out[0], seqs, "accepted"), (out[1], seqs, "next")):
-            if t is not None and n > 0:
-                _need(t, n * 4, what)
+            have, dld = draft_logits.shape
+            if have < nd:
+                raise ValueError("fewer rows of draft logits than drafts")
+            _need(draft_logits, nd * dld * 4, "draft_logits")
+            dl = draft_logits.ptr
+        _need(pick_u, seqs * 4, "pick_u")
+        if temperature is not None:
+            _need(temperature, seqs * 4, "temperature")
+        accepted, nxt = out or (self.tensor((seqs,), np.uint32), self.tensor((seqs,), np.uint32))
+        _need(accepted, seqs * 4, "accepted")
+        _need(nxt, seqs * 4, "next")
         check_hip(self.L.yx_verify_drafts_dev(
-            self.ctx, logits.ptr, cols, ld, ptr(off), seqs, drafts and drafts.ptr, draft_logits and draft_logits.ptr,
-            draft_logits.shape[1] if draft_logits is not None else 0, temperature and temperature.ptr,
-            accept_u and accept_u.ptr, pick_u.ptr, out[0].ptr, out[1].ptr))
-        return out
+            self.ctx, logits.ptr, ld if cols is None else cols, ld, off.ctypes.data, seqs, drafts and drafts.ptr, dl, dld,
+            temperature and temperature.ptr, accept_u and accept_u.ptr, pick_u.ptr, accepted.ptr, nxt.ptr))
+        return accepted, nxt
 
     def stat(self, key):
         """A counter of the context (yx_ctx_get_stat), e.g. "page_entries_sent"."""

@@ -54,16 +54,17 @@ __device__ __forceinline__ void q4_load(Q4Half& r, const q4_t* blk, bool valid, 
 // the difference is exact. (As they lie, read as subnormals code * 2^-24, they would need no
 // exponent, but the matrix unit aligns a subnormal's products by its nominal exponent and drops
 // up to 7 of their bits: outputs 6e-6 off after 600 keys and 1.3e-5 after 4000, against 3e-7.)
+// The exponent comes in a register: with two literals the and-or would be two instructions.
 template <bool kOdd>
-__device__ __forceinline__ half2_q4 q4_codes(uint32_t w) {
-  const half2_q4 c = __builtin_bit_cast(half2_q4, (w & (kOdd ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
+__device__ __forceinline__ half2_q4 q4_codes(uint32_t w, uint32_t exponent) {
+  const half2_q4 c = __builtin_bit_cast(half2_q4, (w & (kOdd ? 0x00f000f0u : 0x000f000fu)) | exponent);
   const _Float16 base = static_cast<_Float16>(kOdd ? 1152.0f : 1032.0f);
   return c - half2_q4{base, base};
 }
 
 // The codes of a K dword as a matrix operand (dims 32 p + 8 g + 0 .. 7; 2, 3, 6, 7 times 16).
-__device__ __forceinline__ half8 q4_k_codes(uint32_t w) {
-  const half2_q4 a = q4_codes<false>(w), b = q4_codes<true>(w), c = q4_codes<false>(w >> 8), d = q4_codes<true>(w >> 8);
+__device__ __forceinline__ half8 q4_k_codes(uint32_t w, uint32_t e) {
+  const half2_q4 a = q4_codes<false>(w, e), b = q4_codes<true>(w, e), c = q4_codes<false>(w >> 8, e), d = q4_codes<true>(w >> 8, e);
   return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
@@ -75,9 +76,10 @@ __device__ __forceinline__ void q4_cut(float y0, float y1, uint32_t& hi, uint32_
   pin(y1);
   hi = __builtin_bit_cast(uint32_t, half2_q4{static_cast<_Float16>(y0), static_cast<_Float16>(y1)});
   pin(hi);
-  const half2_q4 h = __builtin_bit_cast(half2_q4, hi);
-  lo = __builtin_bit_cast(uint32_t, half2_q4{static_cast<_Float16>(__builtin_fmaf(static_cast<float>(h.x), -1.0f, y0)),
-                                             static_cast<_Float16>(__builtin_fmaf(static_cast<float>(h.y), -1.0f, y1))});
+  float r0, r1;  // y - hi, the half read where it lies
+  __asm__("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(y0));
+  __asm__("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(y1));
+  lo = __builtin_bit_cast(uint32_t, half2_q4{static_cast<_Float16>(r0), static_cast<_Float16>(r1)});
 }
 
 // Weights are 2^(kQ4Room + x - m), x and m in log2, and x > m + kQ4Lazy moves m: as high as
@@ -103,6 +105,8 @@ struct Q4Rows {
   int any_lo, any_pos;     // and from the first to the last that some row does
 };
 
+// The scale's sign goes into q, and a scale of 0 becomes one without effect, so that the factor is
+// positive: the maximum may be looked for before it, and a masked -inf stays one.
 // A tile's q (this lane's dims 32 p + 8 g + 0 .. 7 of its column) as operands: hi and lo parts
 // scaled by a power of two; returns the factor from products to log2 scores.
 __device__ __forceinline__ float q4_cut_q(const float4 (&raw)[8], bool has, float scale_log2, half8 (&hi)[4], half8 (&lo)[4]) {
@@ -120,22 +124,23 @@ __device__ __forceinline__ float q4_cut_q(const float4 (&raw)[8], bool has, floa
     const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float v = has ? __builtin_ldexpf(x[e], (e & 2) ? 9 - ex : 13 - ex) : 0.0f;
+      const float v = has ? __builtin_ldexpf(scale_log2 < 0.0f ? -x[e] : x[e], (e & 2) ? 9 - ex : 13 - ex) : 0.0f;
       const _Float16 h = static_cast<_Float16>(v);
       hi[p][e] = h;
       lo[p][e] = static_cast<_Float16>(v - static_cast<float>(h));
     }
   }
-  return __builtin_ldexpf(scale_log2, ex - 13);
+  return __builtin_ldexpf(fmaxf(fabsf(scale_log2), 0x1p-90f), ex - 13);
 }
 
 // kSlots: pairs of blocks a wave holds; each half (K, V) is loaded again as soon as it is used up.
 // q(t, p, part): the operand of tile t.
-template <int NT, int kSlots, bool kLong, int kPolicy, typename Q>
+// begin(): the wave's q and rows, made ready while the first blocks are on their way.
+template <int NT, int kSlots, bool kLong, int kPolicy, typename Q, typename Begin>
 __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict__ kc, const q4_t* __restrict__ vc,
                                           const uint32_t* __restrict__ pt, uint32_t b0, uint32_t nblk,
                                           uint32_t bpp_shift, uint32_t kh, uint32_t hkv, const Q4Rows<NT>& rows, int lane,
-                                          Q q) {
+                                          Q q, Begin begin) {
   const uint32_t bpp_mask = (1u << bpp_shift) - 1u;
   const size_t head_bytes = static_cast<size_t>(kQ4Block) << bpp_shift;
 
@@ -176,6 +181,8 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
     __builtin_amdgcn_sched_barrier(0);
   };
   const int key_end = static_cast<int>((b0 + nblk) * 16);
+  uint32_t exponent = 0x64006400u;
+  __asm__("" : "+v"(exponent));
   floatx4 acc[NT][8];
   uint32_t poison[NT];  // groups in which a row sees a step of NaN (slow runs)
 #pragma unroll
@@ -198,6 +205,7 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
         load_v(s);
       }
     }
+    if constexpr (!kSlow) begin();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (!small) w.m[t] = -INFINITY;
@@ -205,17 +213,20 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
 #pragma unroll
       for (int n = 0; n < 8; ++n) acc[t][n] = small ? acc[t][n] * 0x1p12f : floatx4{0, 0, 0, 0};
     }
-    auto compute = [&](int s, uint32_t b, bool masked) {  // masked: uniform
+    // A pair of blocks; false: the maxima moved, once more (kSlots 1: so the loop's own path has one
+    // set of registers for the results; a branch around the scaling within it costs a move each).
+    auto compute = [&](int s, uint32_t b, bool masked) -> bool {  // masked: uniform
       const int key0 = static_cast<int>((b0 + b) * 16) + 4 * (lane >> 4);
       u32x4 ph[NT], pl[NT];
       floatx4 sc[NT][2];
+      float top[NT];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) sc[t][h] = floatx4{0, 0, 0, 0};
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const half8 ka = q4_k_codes(k[s][h].codes[p]);
+          const half8 ka = q4_k_codes(k[s][h].codes[p], exponent);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             floatx4 d = {0, 0, 0, 0};
@@ -229,39 +240,45 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
           }
         }
       }
-      load_k(s, b + 2 * kSlots);
+      if (masked) {
+        __asm__ volatile("");  // a branch, not 40 selects in every pair
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float x[8];
-        bool ok[8];
-        float top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = sc[t][e >> 2][e & 3] * rows.fac[t];
-          ok[e] = true;
-        }
-        if (masked) {
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int key = key0 + (e >> 2) * 16 + (e & 3);
-            ok[e] = (key >= rows.lo[t]) & (key <= rows.pos[t]) & (key < key_end);
-            x[e] = ok[e] ? x[e] : -INFINITY;
+            if (!((key >= rows.lo[t]) & (key <= rows.pos[t]) & (key < key_end))) sc[t][e >> 2][e & 3] = -INFINITY;
           }
-        }
+      }
+      bool moved = false;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
-        if (__builtin_amdgcn_ballot_w64(top > w.m[t] + kQ4Lazy)) {
-          const float mn = fmaxf(w.m[t], max_xor32(max_xor16(top)));
+      for (int t = 0; t < NT; ++t) {
+        top[t] = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top[t] = fmaxf(top[t], sc[t][e >> 2][e & 3]);
+        top[t] *= rows.fac[t];
+        moved |= top[t] > w.m[t] + kQ4Lazy;
+      }
+      if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float mn = fmaxf(w.m[t], max_xor32(max_xor16(top[t])));
           const float corr = __builtin_amdgcn_exp2f(w.m[t] - fmaxf(mn, kLowest));
           w.m[t] = mn;
           w.l[t] *= corr;
 #pragma unroll
           for (int n = 0; n < 8; ++n) acc[t][n] *= corr;
         }
-        const float base = fmaxf(w.m[t], kLowest) - kQ4Room;
+        if constexpr (kSlots == 1) return false;
+      }
+      load_k(s, b + 2 * kSlots);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float x[8];
+        const float base = kQ4Room - fmaxf(w.m[t], kLowest);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(x[e] - base);
+          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e >> 2][e & 3], rows.fac[t], base));
           w.l[t] += x[e];
         }
 #pragma unroll
@@ -277,7 +294,9 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
               const float step = static_cast<float>(__builtin_bit_cast(half8, v[s][e >> 2].steps[p >> 1])[(p & 1) * 4 + (e & 3)]);
-              if (!(fabsf(step) < INFINITY) && ok[e]) poison[t] |= 1u << p;
+              const int key = key0 + (e >> 2) * 16 + (e & 3);
+              const bool ok = (key >= rows.lo[t]) & (key <= rows.pos[t]) & (key < key_end);
+              if (!(fabsf(step) < INFINITY) && ok) poison[t] |= 1u << p;
             }
         }
       }
@@ -298,6 +317,7 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
           }
       }
       if (masked) {  // keys no row sees
+        __asm__ volatile("");
         u32x2 seen[2];        // [block][keys 2 h, 2 h + 1]
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -327,7 +347,7 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t word = vr[j][h][n >> 2];
-            const half2_q4 c = q4_codes<(n & 1) != 0>((n & 2) ? word >> 8 : word);
+            const half2_q4 c = q4_codes<(n & 1) != 0>((n & 2) ? word >> 8 : word, exponent);
             const half2_q4 st = __builtin_bit_cast(half2_q4, static_cast<uint32_t>(v[s][j].steps[p >> 1][(p & 1) * 2 + h]));
             uint32_t product = __builtin_bit_cast(uint32_t, c * st);
             pin(product);
@@ -352,13 +372,19 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
       tile(std::integral_constant<int, 6>{});
       tile(std::integral_constant<int, 7>{});
       load_v(s);
+      return true;
     };
-    for (uint32_t b = 0; b < nblk; b += 2 * kSlots) {
+    auto whole = [&](uint32_t b) {  // every row sees every key of the pair
+      const int key0 = static_cast<int>((b0 + b) * 16);
+      return key0 >= rows.all_lo && key0 + 31 <= rows.all_pos && key0 + 32 <= key_end;
+    };
+    if constexpr (kSlots == 1) {
+      for (uint32_t b = 0; b < nblk;)
+        if (compute(0, b, !whole(b))) b += 2;
+    } else {
+      for (uint32_t b = 0; b < nblk; b += 2 * kSlots) {
 #pragma unroll
-      for (int s = 0; s < kSlots; ++s) {
-        const uint32_t bs = b + 2 * s;
-        const int key0 = static_cast<int>((b0 + bs) * 16);
-        compute(s, bs, !(key0 >= rows.all_lo && key0 + 31 <= rows.all_pos && key0 + 32 <= key_end));
+        for (int s = 0; s < kSlots; ++s) compute(s, b + 2 * s, !whole(b + 2 * s));
       }
     }
   };
@@ -391,36 +417,51 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
   }
 }
 
-// This lane's part of a wave's rows: tile t's column is logical row lr0 + 16 t + c. Reads and
-// cuts q, a tile at a time: keep(t, hi, lo).
+// This lane's part of a wave's rows: tile t's column is logical row lr0 + 16 t + c. First the loads
+// of its position and q (dims 32 p + 8 g + 0 .. 7), unconditional, of a valid row.
+template <int NT>
+struct Q4Raw {
+  int pos[NT];
+  float4 q[NT][8];
+};
+template <int NT>
+__device__ __forceinline__ void q4_rows_load(Q4Raw<NT>& raw, uint32_t lr0, uint32_t r0, uint32_t nlog, uint32_t kh,
+                                             uint32_t G, uint32_t hq, const uint32_t* pos, const float* q, int lane) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const uint32_t lr = lr0 + t * 16 + (lane & 15), lrc = lr < nlog ? lr : 0;
+    const uint32_t rr = r0 + lrc / G, h = kh * G + lrc % G;
+    raw.pos[t] = static_cast<int>(pos[rr]);
+    const float* src = q + (static_cast<size_t>(rr) * hq + h) * kD + (lane >> 4) * 8;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      raw.q[t][2 * j] = *reinterpret_cast<const float4*>(src + j * 32);
+      raw.q[t][2 * j + 1] = *reinterpret_cast<const float4*>(src + j * 32 + 4);
+    }
+  }
+  // Issued here (q and pos are not declared __restrict__ and the empty asm may write memory), so
+  // that waiting for them waits for nothing issued after.
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Then the rows' keys, and q cut, a tile at a time: keep(t, hi, lo).
 template <int NT, typename Keep>
-__device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, uint32_t lr0, uint32_t r0, uint32_t nlog, uint32_t kh,
-                                        uint32_t G, uint32_t hq, const uint32_t* __restrict__ pos,
-                                        const float* __restrict__ q, uint32_t window, float scale_log2, int lane, Keep keep) {
-  const int c = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, const Q4Raw<NT>& raw, uint32_t lr0, uint32_t nlog,
+                                        uint32_t window, float scale_log2, int lane, Keep keep) {
   rows.all_lo = 0;
   rows.all_pos = 0x7fffffff;
   rows.any_lo = 0x7fffffff;
   rows.any_pos = -1;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const uint32_t lr = lr0 + t * 16 + c;
-    const bool has = lr < nlog;
-    const uint32_t lrc = has ? lr : 0;
-    const uint32_t rr = r0 + lrc / G, h = kh * G + lrc % G;
-    const int p = static_cast<int>(pos[rr]);
+    const bool has = lr0 + t * 16 + (lane & 15) < nlog;
+    const int p = raw.pos[t];
     rows.has[t] = has;
     rows.pos[t] = has ? p : -1;
     rows.lo[t] = (window > 0 && p + 1 > static_cast<int>(window)) ? p + 1 - static_cast<int>(window) : 0;
-    const float* src = q + (static_cast<size_t>(rr) * hq + h) * kD + g * 8;
-    float4 raw[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      raw[2 * j] = *reinterpret_cast<const float4*>(src + j * 32);
-      raw[2 * j + 1] = *reinterpret_cast<const float4*>(src + j * 32 + 4);
-    }
     half8 hi[4], lo[4];
-    rows.fac[t] = q4_cut_q(raw, has, scale_log2, hi, lo);
+    rows.fac[t] = q4_cut_q(raw.q[t], has, scale_log2, hi, lo);
     keep(t, hi, lo);
     int lo_most = has ? rows.lo[t] : 0, lo_least = has ? rows.lo[t] : 0x7fffffff;
     int pos_least = has ? p : 0x7fffffff, pos_most = has ? p : -1;
@@ -442,8 +483,8 @@ __device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, uint32_t lr0, uint32_t
 // 16-row-tile kernel, whose items, hand-off and merge these are.
 template <int NT>
 __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_decode_q4(
-    const AttnItem* __restrict__ items, const uint32_t* __restrict__ pos, const uint32_t* __restrict__ pages,
-    const q4_t* __restrict__ kc, const q4_t* __restrict__ vc, const float* __restrict__ q, float* __restrict__ out,
+    const AttnItem* __restrict__ items, const uint32_t* pos, const uint32_t* __restrict__ pages,
+    const q4_t* __restrict__ kc, const q4_t* __restrict__ vc, const float* q, float* __restrict__ out,
     float* __restrict__ part_o, float2* __restrict__ part_ml, uint32_t* __restrict__ counters, uint32_t part_o_bytes,
     uint32_t part_ml_bytes, uint32_t hq, uint32_t hkv, uint32_t bpp_shift, uint32_t window, float scale_log2,
     const SubRef* __restrict__ members, uint32_t by_item) {
@@ -464,17 +505,22 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
   // q in LDS, in the space of the waves' results.
   half8* const qs = reinterpret_cast<half8*>(&sh.o[0][0][0]);
   static_assert(sizeof(sh.o) >= NT * 8 * 64 * sizeof(half8), "q fits");
-  q4_rows<NT>(rows, 0, it.r0, nlog, kh, G, hq, pos, q, window, scale_log2, lane, [&](int t, const half8* hi, const half8* lo) {
-    if (wave == t)
+  Q4Raw<NT> raw;
+  q4_rows_load<NT>(raw, 0, it.r0, nlog, kh, G, hq, pos, q, lane);
+  q4_attend<NT, NT == 1 ? 2 : 1, false, kNontemporal>(
+      w, kc, vc, pages + it.pt_off, wb0, wb1 - wb0, bpp_shift, kh, hkv, rows, lane,
+      [&](int t, int p, int part) { return qs[(t * 8 + part * 4 + p) * 64 + lane]; },
+      [&]() {
+        q4_rows<NT>(rows, raw, 0, nlog, window, scale_log2, lane, [&](int t, const half8* hi, const half8* lo) {
+          if (wave == t)
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        qs[(t * 8 + p) * 64 + lane] = hi[p];
-        qs[(t * 8 + 4 + p) * 64 + lane] = lo[p];
-      }
-  });
-  __syncthreads();
-  q4_attend<NT, NT == 1 ? 2 : 1, false, kNontemporal>(w, kc, vc, pages + it.pt_off, wb0, wb1 - wb0, bpp_shift, kh, hkv, rows, lane,
-                                               [&](int t, int p, int part) { return qs[(t * 8 + part * 4 + p) * 64 + lane]; });
+            for (int p = 0; p < 4; ++p) {
+              qs[(t * 8 + p) * 64 + lane] = hi[p];
+              qs[(t * 8 + 4 + p) * 64 + lane] = lo[p];
+            }
+        });
+        lds_barrier();
+      });
   __syncthreads();  // every wave is done with q before any writes its result over it
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -518,8 +564,8 @@ static constexpr int kQ4WaveTiles = 2;
 static constexpr int kQ4TileRows = kQ4TileWaves * kQ4WaveTiles * 16;
 
 __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_prefill_q4(
-    const PrefillItem* __restrict__ items, const uint32_t* __restrict__ pos, const uint32_t* __restrict__ pages,
-    const q4_t* __restrict__ kc, const q4_t* __restrict__ vc, const float* __restrict__ q, float* __restrict__ out,
+    const PrefillItem* __restrict__ items, const uint32_t* pos, const uint32_t* __restrict__ pages,
+    const q4_t* __restrict__ kc, const q4_t* __restrict__ vc, const float* q, float* __restrict__ out,
     uint32_t hq, uint32_t hkv, uint32_t bpp_shift, uint32_t window, float scale_log2, float* __restrict__ part_o,
     float2* __restrict__ part_ml, uint32_t* __restrict__ counters, uint32_t part_o_bytes, uint32_t part_ml_bytes) {
   constexpr int NT = kQ4WaveTiles;
@@ -533,8 +579,9 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
   const uint32_t nlog = it.nrows * G;  // at most kQ4TileRows
   half8 (*const qs)[64] = q_lds[wave];
   Q4Rows<NT> rows;
-  q4_rows<NT>(rows, wave * NT * 16, it.r0, nlog, kh, G, hq, pos, q, window, scale_log2, lane,
-              [&](int t, const half8* hi, const half8* lo) {
+  Q4Raw<NT> raw;
+  q4_rows_load<NT>(raw, wave * NT * 16, it.r0, nlog, kh, G, hq, pos, q, lane);
+  q4_rows<NT>(rows, raw, wave * NT * 16, nlog, window, scale_log2, lane, [&](int t, const half8* hi, const half8* lo) {
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       qs[t * 8 + p][lane] = hi[p];
@@ -547,7 +594,7 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
   const uint32_t b1 = some ? min(it.blk1, static_cast<uint32_t>(rows.any_pos) / 16 + 1) : it.blk0;
   Q4Wave<NT> w;
   q4_attend<NT, 1, true, 0>(w, kc, vc, pages + it.pt_off, b0, b1 > b0 ? b1 - b0 : 0, bpp_shift, kh, hkv, rows, lane,
-                      [&](int t, int p, int part) { return qs[t * 8 + part * 4 + p][lane]; });
+                      [&](int t, int p, int part) { return qs[t * 8 + part * 4 + p][lane]; }, []() {});
   const uint32_t nch = it.chunk_nch >> 16;
   if (nch <= 1) {
 #pragma unroll
