@@ -133,10 +133,35 @@ __device__ __forceinline__ float q4_cut_q(const float4 (&raw)[8], bool has, floa
   return __builtin_ldexpf(fmaxf(fabsf(scale_log2), 0x1p-90f), ex - 13);
 }
 
+// Whether a result of the wave is an infinity or NaN.
+template <int NT>
+__device__ __forceinline__ bool q4_bad(const floatx4 (&acc)[NT][8]) {
+  float bad = 0.0f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bad += acc[t][n][i] * 0.0f;
+  return __builtin_amdgcn_ballot_w64(bad != 0.0f) != 0;
+}
+
+// The wave's results and sums, without the operands' powers of two.
+template <int NT>
+__device__ __forceinline__ void q4_done(Q4Wave<NT>& w, const floatx4 (&acc)[NT][8]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    w.l[t] = sum_xor32(sum_xor16(w.l[t])) * __builtin_amdgcn_exp2f(-kQ4Room);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) w.o[t][n] = acc[t][n] * ((n & 1 ? 0.0625f : 1.0f) * __builtin_amdgcn_exp2f(-kQ4Room));
+  }
+}
+
 // kSlots: pairs of blocks a wave holds; each half (K, V) is loaded again as soon as it is used up.
 // q(t, p, part): the operand of tile t.
 // begin(): the wave's q and rows, made ready while the first blocks are on their way.
-template <int NT, int kSlots, bool kLong, int kPolicy, typename Q, typename Begin>
+// kFast false: only the two runs of a wave whose fast one, made elsewhere, was not finite.
+template <int NT, int kSlots, bool kLong, int kPolicy, bool kFast, typename Q, typename Begin>
 __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict__ kc, const q4_t* __restrict__ vc,
                                           const uint32_t* __restrict__ pt, uint32_t b0, uint32_t nblk,
                                           uint32_t bpp_shift, uint32_t kh, uint32_t hkv, const Q4Rows<NT>& rows, int lane,
@@ -163,7 +188,7 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
     } else {
       page = static_cast<uint32_t>(__builtin_amdgcn_readlane(pid, static_cast<int>(b & 63)));
     }
-    return {valid ? (static_cast<size_t>(page) * hkv + kh) * head_bytes + ((b0 + b) & bpp_mask) * static_cast<size_t>(kQ4Block) : 0, valid};
+    return {(static_cast<size_t>(page) * hkv + kh) * head_bytes + ((b0 + b) & bpp_mask) * kQ4Block, valid};
   };
   Q4Half k[kSlots][2], v[kSlots][2];
   Where at[kSlots][2];  // of the blocks whose V is to be loaded
@@ -241,12 +266,13 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
         }
       }
       if (masked) {
-        __asm__ volatile("");  // a branch, not 40 selects in every pair
+        int first = key0;  // known here only: a branch, with no comparison of it in every pair
+        pin(first);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int key = key0 + (e >> 2) * 16 + (e & 3);
+            const int key = first + (e >> 2) * 16 + (e & 3);
             if (!((key >= rows.lo[t]) & (key <= rows.pos[t]) & (key < key_end))) sc[t][e >> 2][e & 3] = -INFINITY;
           }
       }
@@ -317,11 +343,12 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
           }
       }
       if (masked) {  // keys no row sees
-        __asm__ volatile("");
+        int first = key0;
+        pin(first);
         u32x2 seen[2];        // [block][keys 2 h, 2 h + 1]
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const int key = key0 + (e >> 2) * 16 + (e & 3);
+          const int key = first + (e >> 2) * 16 + (e & 3);
           const auto in = [&](int x) { return x >= rows.any_lo && x <= rows.any_pos; };
           seen[e >> 2][(e >> 1) & 1] = (in(key) ? 0xffffu : 0u) | (in(key + 1) ? 0xffff0000u : 0u);
         }
@@ -388,15 +415,8 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
       }
     }
   };
-  pass(std::false_type{}, false);
-  float bad = 0.0f;
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bad += acc[t][n][i] * 0.0f;
-  if (__builtin_amdgcn_ballot_w64(bad != 0.0f)) {  // an infinity or NaN
+  if constexpr (kFast) pass(std::false_type{}, false);
+  if (!kFast || q4_bad<NT>(acc)) {
     pass(std::true_type{}, false);
     pass(std::true_type{}, true);
 #pragma unroll
@@ -409,12 +429,7 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
         if (seen >> (n >> 1) & 1) acc[t][n] = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
     }
   }
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    w.l[t] = sum_xor32(sum_xor16(w.l[t])) * __builtin_amdgcn_exp2f(-kQ4Room);
-#pragma unroll
-    for (int n = 0; n < 8; ++n) w.o[t][n] = acc[t][n] * ((n & 1 ? 0.0625f : 1.0f) * __builtin_amdgcn_exp2f(-kQ4Room));
-  }
+  q4_done<NT>(w, acc);
 }
 
 // This lane's part of a wave's rows: tile t's column is logical row lr0 + 16 t + c. First the loads
@@ -507,7 +522,7 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
   static_assert(sizeof(sh.o) >= NT * 8 * 64 * sizeof(half8), "q fits");
   Q4Raw<NT> raw;
   q4_rows_load<NT>(raw, 0, it.r0, nlog, kh, G, hq, pos, q, lane);
-  q4_attend<NT, NT == 1 ? 2 : 1, false, kNontemporal>(
+  q4_attend<NT, NT == 1 ? 2 : 1, false, kNontemporal, true>(
       w, kc, vc, pages + it.pt_off, wb0, wb1 - wb0, bpp_shift, kh, hkv, rows, lane,
       [&](int t, int p, int part) { return qs[(t * 8 + part * 4 + p) * 64 + lane]; },
       [&]() {
@@ -557,11 +572,26 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
 }
 
 // Prefill: a tile of kQ4TileRows logical rows, NT tiles of 16 to each of 4 waves, over the item's
-// blocks; the waves read the blocks by themselves (the codes of a block are 2 KiB: they come from
-// the CU's cache for all but the first). q lies in LDS, each wave's own.
+// blocks. A pair of blocks is made into operands once for the four waves: K's codes (a dword of each
+// lane, group p by wave p) and V's hi and lo parts (tiles 2 w, 2 w + 1, which share group w's steps),
+// through LDS, two pairs deep with one barrier a pair. q is in registers.
 static constexpr int kQ4TileWaves = 4;
 static constexpr int kQ4WaveTiles = 2;
 static constexpr int kQ4TileRows = kQ4TileWaves * kQ4WaveTiles * 16;
+
+// A pair's operands.
+struct Q4Stage {
+  half8 k[2][4][64];       // [block][group][lane]
+  half8 v[8][2][64];       // [tile][hi, lo][lane]
+  u32x4 steps[2][8];       // K's, [block][two keys' four groups]
+};
+
+// What a wave loads of a pair to make its share of them.
+struct Q4Share {
+  u32x4 v[2];
+  u32x2 vsteps[2];
+  uint32_t k[2], ksteps;
+};
 
 __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_prefill_q4(
     const PrefillItem* __restrict__ items, const uint32_t* pos, const uint32_t* __restrict__ pages,
@@ -569,7 +599,8 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
     uint32_t hq, uint32_t hkv, uint32_t bpp_shift, uint32_t window, float scale_log2, float* __restrict__ part_o,
     float2* __restrict__ part_ml, uint32_t* __restrict__ counters, uint32_t part_o_bytes, uint32_t part_ml_bytes) {
   constexpr int NT = kQ4WaveTiles;
-  __shared__ half8 q_lds[kQ4TileWaves][NT * 8][64];
+  __shared__ Q4Stage stages[2];
+  __shared__ int seen_lo[kQ4TileWaves], seen_pos[kQ4TileWaves];
   const PrefillItem it = items[blockIdx.x / hkv];
   const uint32_t kh = blockIdx.x % hkv;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -577,24 +608,313 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
   const int c = lane & 15, g = lane >> 4;
   const uint32_t G = hq / hkv;
   const uint32_t nlog = it.nrows * G;  // at most kQ4TileRows
-  half8 (*const qs)[64] = q_lds[wave];
-  Q4Rows<NT> rows;
-  Q4Raw<NT> raw;
-  q4_rows_load<NT>(raw, wave * NT * 16, it.r0, nlog, kh, G, hq, pos, q, lane);
-  q4_rows<NT>(rows, raw, wave * NT * 16, nlog, window, scale_log2, lane, [&](int t, const half8* hi, const half8* lo) {
+  const uint32_t* const pt = pages + it.pt_off;
+  const uint32_t nblk = it.blk1 - it.blk0;
+  const uint32_t bpp_mask = (1u << bpp_shift) - 1u;
+  const size_t head_bytes = static_cast<size_t>(kQ4Block) << bpp_shift;
+
+  // Page ids are read a pair ahead of their use.
+  auto page_at = [&](uint32_t b) -> uint32_t {
+    return pt[__builtin_amdgcn_readfirstlane((it.blk0 + (b < nblk ? b : nblk - 1)) >> bpp_shift)];
+  };
+  uint32_t ahead[2] = {page_at(0), page_at(1)};
+  Q4Share share;
+  size_t off[2];  // of the pair being loaded
+  int bytes[2];
+  auto locate = [&](uint32_t b) {
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      qs[t * 8 + p][lane] = hi[p];
-      qs[t * 8 + 4 + p][lane] = lo[p];
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t page = ahead[h];
+      ahead[h] = page_at(b + h + 2);
+      const bool valid = b + h < nblk;
+      off[h] = (static_cast<size_t>(page) * hkv + kh) * head_bytes + ((it.blk0 + b + h) & bpp_mask) * kQ4Block;
+      bytes[h] = valid ? static_cast<int>(kQ4Block) : 0;
     }
-  });
-  // The blocks some row of this wave sees.
-  const bool some = rows.any_pos >= 0;
-  const uint32_t b0 = some ? max(it.blk0, static_cast<uint32_t>(rows.any_lo) / 16) : it.blk0;
-  const uint32_t b1 = some ? min(it.blk1, static_cast<uint32_t>(rows.any_pos) / 16 + 1) : it.blk0;
+  };
+  auto load_k = [&]() {
+    __amdgpu_buffer_rsrc_t rs[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      rs[h] = __builtin_amdgcn_make_buffer_rsrc(const_cast<q4_t*>(kc + off[h]), 0, bytes[h], 0x00020000);
+      share.k[h] = __builtin_amdgcn_raw_buffer_load_b32(rs[h], lane * 16, wave * 4, 0);
+    }
+    share.ksteps = __builtin_amdgcn_raw_buffer_load_b32((wave & 1) ? rs[1] : rs[0], static_cast<int>(kQ4Steps) + (lane & 31) * 4, 0, 0);
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<q4_t*>(vc + off[h]), 0, bytes[h], 0x00020000);
+      share.v[h] = __builtin_amdgcn_raw_buffer_load_b128(rs, lane * 16, 0, 0);
+      share.vsteps[h] = __builtin_amdgcn_raw_buffer_load_b64(rs, static_cast<int>(kQ4Steps) + g * 32, wave * 8, 0);
+    }
+  };
+  auto load = [&](uint32_t b) {
+    locate(b);
+    load_k();
+    load_v();
+  };
+  load(0);
+
+  Q4Rows<NT> rows;
+  half8 qa[NT][2][4];
+  {
+    Q4Raw<NT> raw;
+    q4_rows_load<NT>(raw, wave * NT * 16, it.r0, nlog, kh, G, hq, pos, q, lane);
+    q4_rows<NT>(rows, raw, wave * NT * 16, nlog, window, scale_log2, lane, [&](int t, const half8* hi, const half8* lo) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        qa[t][0][p] = hi[p];
+        qa[t][1][p] = lo[p];
+      }
+    });
+  }
+  if (lane == 0) {
+    seen_lo[wave] = rows.any_lo;
+    seen_pos[wave] = rows.any_pos;
+  }
+  lds_barrier();
+  int any_lo = seen_lo[0], any_pos = seen_pos[0];  // keys that some row of the tile sees
+#pragma unroll
+  for (int v = 1; v < kQ4TileWaves; ++v) {
+    any_lo = min(any_lo, seen_lo[v]);
+    any_pos = max(any_pos, seen_pos[v]);
+  }
+  any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+  any_pos = __builtin_amdgcn_readfirstlane(any_pos);
+
+  uint32_t exponent = 0x64006400u;
+  __asm__("" : "+v"(exponent));
+  const uint32_t byte_sel = 0x0c000c00u | static_cast<uint32_t>(wave) | static_cast<uint32_t>(wave + 4) << 16;
+  // This wave's share of a pair, made into operands: steps of keys no row sees cleared, then four
+  // pieces (K's two blocks, V's two tiles).
+  auto clear = [&](uint32_t b) {
+    const int first = static_cast<int>((it.blk0 + b) * 16);
+    if (first >= any_lo && first + 31 <= any_pos) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int key = first + h * 16 + 4 * g + 2 * j;
+        const auto in = [&](int x) { return x >= any_lo && x <= any_pos; };
+        share.vsteps[h][j] &= (in(key) ? 0xffffu : 0u) | (in(key + 1) ? 0xffff0000u : 0u);
+      }
+  };
+  auto make = [&](auto piece, Q4Stage& st) {
+    constexpr int kPiece = decltype(piece)::value;
+    if constexpr (kPiece < 2) {
+      st.k[kPiece][wave][lane] = q4_k_codes(share.k[kPiece], exponent);
+      if constexpr (kPiece == 0) reinterpret_cast<uint32_t*>(st.steps)[(wave & 1) * 32 + (lane & 31)] = share.ksteps;
+    } else {
+      constexpr int n = kPiece - 2;
+      u32x4 hi, lo;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t word = __builtin_amdgcn_perm(share.v[j][2 * h + 1], share.v[j][2 * h], byte_sel);
+          const half2_q4 x = q4_codes<n != 0>(word, exponent);
+          const half2_q4 step = __builtin_bit_cast(half2_q4, static_cast<uint32_t>(share.vsteps[j][h]));
+          uint32_t product = __builtin_bit_cast(uint32_t, x * step);
+          pin(product);
+          hi[2 * j + h] = product;
+          lo[2 * j + h] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, step, -__builtin_bit_cast(half2_q4, product)));
+        }
+      st.v[2 * wave + n][0][lane] = __builtin_bit_cast(half8, hi);
+      st.v[2 * wave + n][1][lane] = __builtin_bit_cast(half8, lo);
+    }
+  };
+  auto convert = [&](Q4Stage& st, uint32_t b) {
+    clear(b);
+    make(std::integral_constant<int, 0>{}, st);
+    make(std::integral_constant<int, 1>{}, st);
+    make(std::integral_constant<int, 2>{}, st);
+    make(std::integral_constant<int, 3>{}, st);
+  };
+
   Q4Wave<NT> w;
-  q4_attend<NT, 1, true, 0>(w, kc, vc, pages + it.pt_off, b0, b1 > b0 ? b1 - b0 : 0, bpp_shift, kh, hkv, rows, lane,
-                      [&](int t, int p, int part) { return qs[t * 8 + part * 4 + p][lane]; }, []() {});
+  floatx4 acc[NT][8];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    w.m[t] = -INFINITY;
+    w.l[t] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) acc[t][n] = floatx4{0, 0, 0, 0};
+  }
+  const int key_end = static_cast<int>(it.blk1 * 16);
+  u32x4 ph[NT], pl[NT];
+  float corr[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) corr[t] = 1.0f;
+  // A pair's weights; false: the maxima moved, the results are to be scaled by corr.
+  auto weights = [&](const Q4Stage& st, int first, bool masked) -> bool {
+    floatx4 sc[NT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const half8 steps[2] = {__builtin_bit_cast(half8, st.steps[h][2 * g]), __builtin_bit_cast(half8, st.steps[h][2 * g + 1])};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sc[t][h] = floatx4{0, 0, 0, 0};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const half8 ka = st.k[h][p][lane];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          floatx4 d = {0, 0, 0, 0};
+          d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qa[t][0][p], d, 0, 0, 0);
+          d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qa[t][1][p], d, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sc[t][h][i] = __builtin_fmaf(static_cast<float>(steps[i >> 1][(i & 1) * 4 + p]), d[i], sc[t][h][i]);
+        }
+      }
+    }
+    if (masked) {
+      int key0 = first + 4 * g;  // known here only: a branch, with no comparison of it in every pair
+      pin(key0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = key0 + (e >> 2) * 16 + (e & 3);
+          if (!((key >= rows.lo[t]) & (key <= rows.pos[t]) & (key < key_end))) sc[t][e >> 2][e & 3] = -INFINITY;
+        }
+    }
+    float top[NT];
+    bool moved = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      top[t] = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top[t] = fmaxf(top[t], sc[t][e >> 2][e & 3]);
+      top[t] *= rows.fac[t];
+      moved |= top[t] > w.m[t] + kQ4Lazy;
+    }
+    if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float mn = fmaxf(w.m[t], max_xor32(max_xor16(top[t])));
+        corr[t] = __builtin_amdgcn_exp2f(w.m[t] - fmaxf(mn, kLowest));
+        w.m[t] = mn;
+        w.l[t] *= corr[t];
+      }
+      return false;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float x[8];
+      const float base = kQ4Room - fmaxf(w.m[t], kLowest);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e >> 2][e & 3], rows.fac[t], base));
+        w.l[t] += x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t hi, lo;
+        q4_cut(x[2 * e], x[2 * e + 1], hi, lo);
+        ph[t][e] = hi;
+        pl[t][e] = lo;
+      }
+    }
+    return true;
+  };
+  convert(stages[0], 0);
+  load(2);
+  lds_barrier();
+  // The pairs some row of this wave sees; for the tile's others it makes operands alone.
+  const bool some = rows.any_pos >= 0;
+  const uint32_t b0 = some ? max(it.blk0, static_cast<uint32_t>(rows.any_lo) / 16) - it.blk0 : nblk;
+  const uint32_t b1 = some ? min(it.blk1, max(it.blk0, static_cast<uint32_t>(rows.any_pos) / 16 + 1)) - it.blk0 : 0;
+  const uint32_t p0 = min(b0, nblk) / 2 * 2;
+  uint32_t b = 0;
+  auto others = [&](uint32_t end) {
+    for (; b < end; b += 2) {
+      convert(stages[((b >> 1) & 1) ^ 1], b + 2);
+      load(b + 4);
+      lds_barrier();
+    }
+  };
+  auto priority = [&]() {
+    const uint32_t left = nblk - b;
+    if (left > 96) __builtin_amdgcn_s_setprio(3);
+    else if (left > 32) __builtin_amdgcn_s_setprio(2);
+    else if (left > 8) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(0);
+  };
+  priority();
+  others(p0);
+  // Where the maxima move, the inner loop ends, the results are scaled and the pair is looked at once
+  // more: so the inner loop has one set of registers for the results, with no moves.
+  for (bool moved = b < b1; moved;) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int n = 0; n < 8; ++n) acc[t][n] *= corr[t];
+    moved = false;
+    while (b < b1) {
+      const Q4Stage& st = stages[(b >> 1) & 1];
+      const int first = static_cast<int>((it.blk0 + b) * 16);
+      moved = !weights(st, first, !(first >= rows.all_lo && first + 31 <= rows.all_pos && first + 32 <= key_end));
+      if (moved) break;
+        clear(b + 2);
+      Q4Stage& next = stages[((b >> 1) & 1) ^ 1];
+      // V's operands are read a tile ahead, the next pair's are made in the shadow of the products.
+      half8 vh = st.v[0][0][lane], vl = st.v[0][1][lane];
+      auto tile = [&](auto nc) {
+        constexpr int n = decltype(nc)::value;
+        __builtin_amdgcn_sched_barrier(0);
+        const half8 h = vh, l = vl;
+        if constexpr (n < 7) {
+          vh = st.v[n + 1][0][lane];
+          vl = st.v[n + 1][1][lane];
+        }
+        if constexpr ((n & 1) == 0) make(std::integral_constant<int, n / 2>{}, next);
+        if constexpr (n == 1) locate(b + 4);
+        if constexpr (n == 3) load_k();
+        if constexpr (n == 7) load_v();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, __builtin_bit_cast(half8, ph[t]), acc[t][n], 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, __builtin_bit_cast(half8, pl[t]), acc[t][n], 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l, __builtin_bit_cast(half8, ph[t]), acc[t][n], 0, 0, 0);
+      };
+      tile(std::integral_constant<int, 0>{});
+      tile(std::integral_constant<int, 1>{});
+      tile(std::integral_constant<int, 2>{});
+      tile(std::integral_constant<int, 3>{});
+      tile(std::integral_constant<int, 4>{});
+      tile(std::integral_constant<int, 5>{});
+      tile(std::integral_constant<int, 6>{});
+      tile(std::integral_constant<int, 7>{});
+      __builtin_amdgcn_sched_barrier(0);
+      lds_barrier();
+      b += 2;
+      priority();
+    }
+  }
+  others(nblk);
+  if (q4_bad<NT>(acc)) {  // again, a tile at a time with q in LDS (the operands' space is free)
+    half8 (*const qs)[64] = reinterpret_cast<half8 (*)[64]>(stages) + wave * 8;
+    static_assert(sizeof(stages) >= kQ4TileWaves * 8 * sizeof(*qs), "q fits");
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        qs[p][lane] = qa[t][0][p];
+        qs[4 + p][lane] = qa[t][1][p];
+      }
+      const Q4Rows<1> row = {{rows.has[t]}, {rows.pos[t]}, {rows.lo[t]}, {rows.fac[t]}, rows.all_lo, rows.all_pos, rows.any_lo, rows.any_pos};
+      Q4Wave<1> one;
+      q4_attend<1, 1, true, 0, false>(one, kc, vc, pt, it.blk0 + b0, b1 > b0 ? b1 - b0 : 0, bpp_shift, kh, hkv, row, lane,
+                                      [&](int, int p, int part) { return qs[part * 4 + p][lane]; }, []() {});
+      w.m[t] = one.m[0];
+      w.l[t] = one.l[0];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) w.o[t][n] = one.o[0][n];
+    }
+  } else {
+    q4_done<NT>(w, acc);
+  }
   const uint32_t nch = it.chunk_nch >> 16;
   if (nch <= 1) {
 #pragma unroll
