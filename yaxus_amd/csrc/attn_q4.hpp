@@ -105,11 +105,11 @@ struct Q4Rows {
   int any_lo, any_pos;     // and from the first to the last that some row does
 };
 
-// The scale's sign goes into q, and a scale of 0 becomes one without effect, so that the factor is
-// positive: the maximum may be looked for before it, and a masked -inf stays one.
 // A tile's q (this lane's dims 32 p + 8 g + 0 .. 7 of its column) as operands: hi and lo parts
-// scaled by a power of two; returns the factor from products to log2 scores.
-__device__ __forceinline__ float q4_cut_q(const float4 (&raw)[8], bool has, float scale_log2, half8 (&hi)[4], half8 (&lo)[4]) {
+// scaled by a power of two; returns the factor from products to log2 scores. The scale's sign goes
+// into q, and a scale of 0 becomes one without effect, so that the factor is positive: the maximum
+// may be looked for before it, and a masked -inf stays one.
+__device__ __forceinline__ float q4_cut_q(float4 (&raw)[8], float scale_log2, u32x4 (&hi)[4], u32x4 (&lo)[4]) {
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -117,19 +117,25 @@ __device__ __forceinline__ float q4_cut_q(const float4 (&raw)[8], bool has, floa
     top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))));
   }
   top = max_xor32(max_xor16(top));
-  const int ex = has && top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;  // top < 2^ex
+  const int ex = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;  // top < 2^ex
+  if (scale_log2 < 0.0f) {
+    __asm__ volatile("");  // a branch: no select per value
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const float4 a = raw[2 * p], b = raw[2 * p + 1];
-    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = has ? __builtin_ldexpf(scale_log2 < 0.0f ? -x[e] : x[e], (e & 2) ? 9 - ex : 13 - ex) : 0.0f;
-      const _Float16 h = static_cast<_Float16>(v);
-      hi[p][e] = h;
-      lo[p][e] = static_cast<_Float16>(v - static_cast<float>(h));
-    }
+    for (int j = 0; j < 8; ++j) raw[j] = float4{-raw[j].x, -raw[j].y, -raw[j].z, -raw[j].w};
   }
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float4 a = raw[2 * p + j];
+      uint32_t h0, l0, h1, l1;  // elements 2, 3 meet codes 16 times as large
+      q4_cut(__builtin_ldexpf(a.x, 13 - ex), __builtin_ldexpf(a.y, 13 - ex), h0, l0);
+      q4_cut(__builtin_ldexpf(a.z, 9 - ex), __builtin_ldexpf(a.w, 9 - ex), h1, l1);
+      hi[p][2 * j] = h0;
+      hi[p][2 * j + 1] = h1;
+      lo[p][2 * j] = l0;
+      lo[p][2 * j + 1] = l1;
+    }
   return __builtin_ldexpf(fmaxf(fabsf(scale_log2), 0x1p-90f), ex - 13);
 }
 
@@ -460,14 +466,20 @@ __device__ __forceinline__ void q4_rows_load(Q4Raw<NT>& raw, uint32_t lr0, uint3
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Then the rows' keys, and q cut, a tile at a time: keep(t, hi, lo).
+// The least value of a row of 16 lanes, in each of them.
+__device__ __forceinline__ int row16_min(int v) {
+  v = min(v, __builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false));   // lanes 1, 0, 3, 2
+  v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false));   // 2, 3, 0, 1
+  v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xf, 0xf, false));  // mirrored in eights
+  return min(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xf, 0xf, false));  // in the row
+}
+
+// Then the rows' keys, and q cut, a tile at a time: keep(t, hi, lo). A column without a row has the
+// item's first row's q and sees no key.
 template <int NT, typename Keep>
-__device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, const Q4Raw<NT>& raw, uint32_t lr0, uint32_t nlog,
+__device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, Q4Raw<NT>& raw, uint32_t lr0, uint32_t nlog,
                                         uint32_t window, float scale_log2, int lane, Keep keep) {
-  rows.all_lo = 0;
-  rows.all_pos = 0x7fffffff;
-  rows.any_lo = 0x7fffffff;
-  rows.any_pos = -1;
+  int all_lo = 0, all_pos = 0x7fffffff, any_lo = 0x7fffffff, any_pos = -1;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const bool has = lr0 + t * 16 + (lane & 15) < nlog;
@@ -475,23 +487,20 @@ __device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, const Q4Raw<NT>& raw, 
     rows.has[t] = has;
     rows.pos[t] = has ? p : -1;
     rows.lo[t] = (window > 0 && p + 1 > static_cast<int>(window)) ? p + 1 - static_cast<int>(window) : 0;
-    half8 hi[4], lo[4];
-    rows.fac[t] = q4_cut_q(raw.q[t], has, scale_log2, hi, lo);
+    u32x4 hi[4], lo[4];
+    rows.fac[t] = q4_cut_q(raw.q[t], scale_log2, hi, lo);
     keep(t, hi, lo);
-    int lo_most = has ? rows.lo[t] : 0, lo_least = has ? rows.lo[t] : 0x7fffffff;
-    int pos_least = has ? p : 0x7fffffff, pos_most = has ? p : -1;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-      lo_most = max(lo_most, __shfl_xor(lo_most, o));
-      lo_least = min(lo_least, __shfl_xor(lo_least, o));
-      pos_least = min(pos_least, __shfl_xor(pos_least, o));
-      pos_most = max(pos_most, __shfl_xor(pos_most, o));
+    if (has) {
+      all_lo = max(all_lo, rows.lo[t]);
+      any_lo = min(any_lo, rows.lo[t]);
+      all_pos = min(all_pos, p);
+      any_pos = max(any_pos, p);
     }
-    rows.all_lo = max(rows.all_lo, __builtin_amdgcn_readfirstlane(lo_most));
-    rows.any_lo = min(rows.any_lo, __builtin_amdgcn_readfirstlane(lo_least));
-    rows.all_pos = min(rows.all_pos, __builtin_amdgcn_readfirstlane(pos_least));
-    rows.any_pos = max(rows.any_pos, __builtin_amdgcn_readfirstlane(pos_most));
   }
+  rows.all_lo = -__builtin_amdgcn_readfirstlane(row16_min(-all_lo));
+  rows.any_lo = __builtin_amdgcn_readfirstlane(row16_min(any_lo));
+  rows.all_pos = __builtin_amdgcn_readfirstlane(row16_min(all_pos));
+  rows.any_pos = -__builtin_amdgcn_readfirstlane(row16_min(-any_pos));
 }
 
 // Decode and verify: a work item's blocks dealt evenly over 8 waves, as the binary16 arena's
@@ -526,12 +535,12 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
       w, kc, vc, pages + it.pt_off, wb0, wb1 - wb0, bpp_shift, kh, hkv, rows, lane,
       [&](int t, int p, int part) { return qs[(t * 8 + part * 4 + p) * 64 + lane]; },
       [&]() {
-        q4_rows<NT>(rows, raw, 0, nlog, window, scale_log2, lane, [&](int t, const half8* hi, const half8* lo) {
+        q4_rows<NT>(rows, raw, 0, nlog, window, scale_log2, lane, [&](int t, const u32x4* hi, const u32x4* lo) {
           if (wave == t)
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-              qs[(t * 8 + p) * 64 + lane] = hi[p];
-              qs[(t * 8 + 4 + p) * 64 + lane] = lo[p];
+              qs[(t * 8 + p) * 64 + lane] = __builtin_bit_cast(half8, hi[p]);
+              qs[(t * 8 + 4 + p) * 64 + lane] = __builtin_bit_cast(half8, lo[p]);
             }
         });
         lds_barrier();
@@ -660,11 +669,11 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
   {
     Q4Raw<NT> raw;
     q4_rows_load<NT>(raw, wave * NT * 16, it.r0, nlog, kh, G, hq, pos, q, lane);
-    q4_rows<NT>(rows, raw, wave * NT * 16, nlog, window, scale_log2, lane, [&](int t, const half8* hi, const half8* lo) {
+    q4_rows<NT>(rows, raw, wave * NT * 16, nlog, window, scale_log2, lane, [&](int t, const u32x4* hi, const u32x4* lo) {
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        qa[t][0][p] = hi[p];
-        qa[t][1][p] = lo[p];
+        qa[t][0][p] = __builtin_bit_cast(half8, hi[p]);
+        qa[t][1][p] = __builtin_bit_cast(half8, lo[p]);
       }
     });
   }

@@ -246,6 +246,9 @@ void* g_scratch_ptr[kMaxDevices] = {};
 // recorded there at the hand-over), so calls on different streams do not overlap on
 // the scratch.
 using PlanKey = std::tuple<size_t, size_t, size_t, int, size_t>;  // (window, hq, hkv, dtype, page)
+// With the dtype: a 4-bit arena's plan whose partials fit the scratch of the entry point that
+// allocates nothing (other arenas' plans serve both).
+constexpr int kFitScratch = 0x100;
 struct ScratchOwner {
   const yx_ctx* ctx = nullptr;
   hipStream_t stream = nullptr;
@@ -540,10 +543,12 @@ static constexpr uint32_t kFanIn = 32;  // chunks per group the automatic split 
 // f32: the f32 arena's plan: its prefill kernel's items for passes with many rows per
 // sequence (as for f16), else its split-K decode kernel's (16 logical rows per item).
 // page_size: the arena's (shared prefixes are found by page ids).
-int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_t page_size,
+int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t page_size,
                AttnPlan** out) {
+  const int dtype = form & ~kFitScratch;
+  const bool fit = (form & kFitScratch) != 0;
   const bool f32 = dtype == YX_DTYPE_F32, q4 = dtype == YX_DTYPE_Q4;
-  auto key = std::make_tuple(window, hq, hkv, dtype, page_size);
+  auto key = std::make_tuple(window, hq, hkv, form, page_size);
   auto it = c->plans.find(key);
   if (it != c->plans.end()) {
     *out = &it->second;
@@ -563,6 +568,7 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_
   // after 32768 50.1 / 101.1, 1 x 128 after 32768 218.1 / 103.6, 2 x 64 after 16384
   // 81.5 / 70.7.
   bool use_prefill, must_fit = false;
+  double q4_decode_us = 0;  // 4-bit arena: estimate of the pass as decode items
   if (c->prefill_min_rows > 0) {
     use_prefill = max_rows >= static_cast<uint32_t>(c->prefill_min_rows);
   } else if (f32) {
@@ -604,9 +610,34 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_
     // item holds: such a pass is refused, whichever kernel would be faster.
     must_fit = decode_us <= 95.0 + 2.4 * max_keys / 1024.0;
     if (G > 16) use_prefill = max_rows * G > 16 && !must_fit;
+  } else if (q4) {
+    // The 4-bit arena: one decode item (32 logical rows, 8 waves with a share of its blocks each)
+    // per CU takes 14 us and 1.6 ns per pair of blocks over all items; prefill tiles 10 us and 2.1
+    // per pair of the split chosen below. The kernel with the smaller estimate runs. Measured (B x rows after ctx,
+    // 16/4 heads, decode / prefill us): 1 x 256 after 0 17 / 26, 1 x 128 after 4096 33 / 68, 1 x 64
+    // after 32768 65 / 181, 16 x 16 after 4096 44 / 70, 16 x 24 61 / 75, 16 x 64 122 / 108, 4 x 256
+    // after 2000 79 / 73, 16 x 128 after 1000 111 / 74, 1 x 2048 after 0 108 / 77, 1 x 1024 after
+    // 8000 252 / 185; 32/8 heads, 64 x 64 after 64 258 / 48, 2 x 64 after 16384 152 / 133.
+    use_prefill = max_rows * G > 32;
+    if (use_prefill) {
+      double items = 0, pairs = 0;
+      const uint32_t rows_per_item = static_cast<uint32_t>(32 / G);  // 0: no decode item holds a row
+      for (const Group& g : c->groups) {
+        if (!rows_per_item) break;
+        const double of_group = (g.n + rows_per_item - 1) / rows_per_item;
+        double keys = 0;
+        for (uint32_t i = g.r0; i < g.r0 + g.n; ++i) {
+          const uint64_t all = static_cast<uint64_t>(c->pos[i]) + 1;
+          keys += static_cast<double>(window > 0 ? std::min<uint64_t>(all, window) : all);
+        }
+        items += of_group;
+        pairs += of_group * keys / g.n / 32;
+      }
+      q4_decode_us = rows_per_item ? 14 * std::max(1.0, items * hkv / c->cus) + 1.6e-3 * pairs * hkv : 1e30;
+    }
   } else {
     size_t tiles = 0;
-    const size_t per = q4 ? yx::kQ4TileRows : yx::kPrefillRows;
+    const size_t per = yx::kPrefillRows;
     for (const Group& g : c->groups) tiles += (g.n * G + per - 1) / per;
     tiles *= hkv;
     use_prefill = max_rows * G > static_cast<size_t>(c->max_tiles) * 8 &&
@@ -666,22 +697,26 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_
     // 46 -> 36; 2 x 483 rows after 904 and 11780, 16/4: 127 (129 with kSplitPairs 12, 133
     // with 3 and more chunks). With kSplitPairs 8 and kAlone 0.8, 7 x 281 after 934-1796
     // split in vain (72 -> 81) and so did 2 x 277 after 344-5912 (9% slower); kTail 1 picks
-    // as many chunks again.
+    // as many chunks again. 4-bit tiles start in 5 us, 3 of their pairs, and have chunks down to 8
+    // pairs (8 x 128 rows after 1000-4000, window 512: 51 -> 43 us; 1 x 512 after 0 41 -> 39 as tiles);
+    // the last chunk merges at about half a pair a chunk (64 chunks of 2 x 64 rows after 32768: 180 us,
+    // 67 as decode items).
     if (c->prefill_split) {
-      constexpr double kTail = 0.5, kAlone = 0.9;
+      constexpr double kTail = 0.5;
+      const double kAlone = q4 ? 0.8 : 0.9;
       constexpr uint32_t kMinChunkPairs = 16;
       const bool parts8 = f32 && plan.pf32_waves == 8;
-      const uint32_t kFixedPairs = parts8 ? 3 : 7, kSplitPairs = parts8 ? 4 : 12;
-      const uint32_t min_chunk = parts8 ? 8 : kMinChunkPairs;
+      const uint32_t kFixedPairs = q4 || parts8 ? 3 : 7, kSplitPairs = q4 || parts8 ? 4 : 12;
+      const uint32_t min_chunk = q4 || parts8 ? 8 : kMinChunkPairs;
       // A chunk's own cost in a tile of nch, in pairs.
-      auto split_cost = [&](uint32_t nch) { return nch <= 1 ? 0 : kSplitPairs + (parts8 ? nch / 3 : 0); };
+      auto split_cost = [&](uint32_t nch) { return nch <= 1 ? 0 : kSplitPairs + (q4 ? nch / 2 : parts8 ? nch / 3 : 0); };
       uint64_t total = 0;
       for (const yx::PrefillItem& w : plan.pitems) total += (w.blk1 - w.blk0 + 1) / 2 + 4;
       total *= hkv;
       // Workgroup slots: two per CU (4-wave tiles), one (8-wave f32 tiles).
       const uint32_t per_cu = f32 && plan.pf32_waves == 8 ? 1 : 2;
       const uint64_t slots2 = per_cu * static_cast<uint64_t>(c->cus);
-      const uint32_t avg = static_cast<uint32_t>(std::max<uint64_t>(kMinChunkPairs, (total + slots2 - 1) / slots2));
+      const uint32_t avg = static_cast<uint32_t>(std::max<uint64_t>(q4 ? min_chunk : kMinChunkPairs, (total + slots2 - 1) / slots2));
       struct Split {
         uint32_t pairs, over;  // chunks of about `pairs`, for tiles of more than `over` (0: none)
       };
@@ -746,7 +781,7 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_
         auto consider = [&](const Split& sp) {
           const double below = (whole && chosen_parts == 0 ? 0.94 : 0.98) * best_t;
           const double t = estimate(sp, below);
-          if (t < below && (parts * part_bytes <= scratch || plain_parts * part_bytes > scratch) &&
+          if (t < below && (parts * part_bytes <= scratch || (q4 ? !fit : plain_parts * part_bytes > scratch)) &&
               parts * part_bytes <= (size_t{1} << 30)) {
             best = sp;
             best_t = t;
@@ -778,6 +813,11 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int dtype, size_
         }
       }
       if (must_fit && chosen_parts * part_bytes > scratch) use_prefill = false;
+      if (fit && chosen_parts * part_bytes > scratch) {
+        best = Split{0, 0};
+        best_t = estimate(best, 1e30);
+      }
+      if (q4 && c->prefill_min_rows == 0 && q4_decode_us < 10 + 2.1 * best_t) use_prefill = false;
       std::vector<yx::PrefillItem> split;
       uint32_t nslot = 0, ncnt = 0;
       for (const yx::PrefillItem& w : plan.pitems) {
@@ -1337,11 +1377,12 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
   if (c->rows == 0) return YX_OK;
   if (!out || (!q && !qkv)) return fail(YX_ERR_INVALID, "null q or out");
   AttnPlan* plan;
-  if (c->capturing && !c->plans.count(std::make_tuple(window, hq, hkv, kv->dtype, kv->page)))
+  const int form = kv->dtype | (noalloc && kv->q4 ? kFitScratch : 0);
+  const auto key = std::make_tuple(window, hq, hkv, form, kv->page);
+  if (c->capturing && !c->plans.count(key))
     return fail(YX_ERR_INVALID, "run the call once before capturing it (its work list is uploaded then)");
-  if ((rc = build_plan(c, window, hq, hkv, kv->dtype, kv->page, &plan))) return rc;
+  if ((rc = build_plan(c, window, hq, hkv, form, kv->page, &plan))) return rc;
   {
-    const auto key = std::make_tuple(window, hq, hkv, kv->dtype, kv->page);
     if (std::find(c->used_keys.begin(), c->used_keys.end(), key) == c->used_keys.end())
       c->used_keys.push_back(key);
   }
@@ -1360,7 +1401,7 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
   if (noalloc) {
     ScratchMap m;
     if ((rc = scratch_map(c, pml_need, po_need, cnt_need, &m))) return rc;
-    if ((rc = scratch_take(c, std::make_tuple(window, hq, hkv, kv->dtype, kv->page), plan, &m))) return rc;
+    if ((rc = scratch_take(c, key, plan, &m))) return rc;
     d_items = m.items;
     d_members = plan->members.empty() ? nullptr : static_cast<const yx::SubRef*>(m.members);
     po = static_cast<float*>(m.part_o);
