@@ -602,6 +602,16 @@ struct Q4Share {
   uint32_t k[2], ksteps;
 };
 
+// Of two waves of a SIMD the older goes first and leaves the other to run alone at the end (512 rows
+// after 24000 keys: 225 and 295 us). A wave with fewer blocks left gives way, so both end close to
+// each other (265 and 280).
+__device__ __forceinline__ void q4_priority(uint32_t left) {
+  if (left > 96) __builtin_amdgcn_s_setprio(3);
+  else if (left > 32) __builtin_amdgcn_s_setprio(2);
+  else if (left > 8) __builtin_amdgcn_s_setprio(1);
+  else __builtin_amdgcn_s_setprio(0);
+}
+
 __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_prefill_q4(
     const PrefillItem* __restrict__ items, const uint32_t* pos, const uint32_t* __restrict__ pages,
     const q4_t* __restrict__ kc, const q4_t* __restrict__ vc, const float* q, float* __restrict__ out,
@@ -842,14 +852,7 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
       lds_barrier();
     }
   };
-  auto priority = [&]() {
-    const uint32_t left = nblk - b;
-    if (left > 96) __builtin_amdgcn_s_setprio(3);
-    else if (left > 32) __builtin_amdgcn_s_setprio(2);
-    else if (left > 8) __builtin_amdgcn_s_setprio(1);
-    else __builtin_amdgcn_s_setprio(0);
-  };
-  priority();
+  q4_priority(nblk);
   others(p0);
   // Where the maxima move, the inner loop ends, the results are scaled and the pair is looked at once
   // more: so the inner loop has one set of registers for the results, with no moves.
@@ -898,7 +901,7 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
       __builtin_amdgcn_sched_barrier(0);
       lds_barrier();
       b += 2;
-      priority();
+      q4_priority(nblk - b);
     }
   }
   others(nblk);
