@@ -21,7 +21,8 @@
  * take device pointers and are asynchronous (yx_sync waits).
  *
  * The arena layout is private: per layer, K and V are `[page][kv_head][page_size][128]`
- * IEEE binary16, so one (page, kv head) is one contiguous block. head_dim is 128 (the
+ * IEEE binary16 (or f32, or 4-bit codes with steps, 72 bytes a head vector: yx_kv_create's
+ * dtype), so one (page, kv head) is one contiguous block. head_dim is 128 (the
  * reference GPU kernels are written for 128 as well: yaxus-backend-gpu lib.rs:72).
  */
 #ifndef YAXUS_HIP_H
@@ -67,14 +68,14 @@ int yx_sync(yx_ctx* ctx);
  * "prefill_min_rows" (rows of one sequence from which the prefill kernel is used; 0,
  * the default: automatic, the prefill kernel when a sequence has more (row, q head)
  * pairs than one decode work item holds and the pass makes at least one prefill tile
- * per 8 CUs; on the f32 arena, the kernel with the smaller time estimated from the
- * keys its decode items would read, the longest context and the pass's products),
+ * per 8 CUs; on the f32 and the 4-bit arena, the kernel with the smaller time estimated
+ * from the keys its decode items would read, the longest context and the pass's products),
  * "attn_decode_shape" (0, the default: automatic. Passes of more than 8 logical rows per
  * work item use the kernel with 16-row tiles and a fixed split of blocks over its waves;
  * so do one-tile passes whose work items split evenly over the waves or hold more than
  * 64 blocks; other one-tile passes use the kernel whose waves share a queue of blocks.
  * 1: the kernels with 8-row tiles and a fixed split only. 2: the 16-row-tile kernel for
- * every decode pass). "attn_cascade" (1, the default: consecutive groups of a one-tile
+ * every decode pass. f32 and 4-bit arenas have a kernel of 16-row tiles alone). "attn_cascade" (1, the default: consecutive groups of a one-tile
  * decode pass whose page tables start with the same pages, e.g. forks of one prompt,
  * attend those shared keys once for all their rows and merge that result into each
  * row's own; 0: every group reads its whole context). "attn_xcd_prefix" (1, the default:

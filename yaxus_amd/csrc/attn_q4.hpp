@@ -504,7 +504,12 @@ __device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, Q4Raw<NT>& raw, uint32
 }
 
 // Decode and verify: a work item's blocks dealt evenly over 8 waves, as the binary16 arena's
-// 16-row-tile kernel, whose items, hand-off and merge these are.
+// 16-row-tile kernel, whose items, hand-off and merge these are. q lies in LDS, since its parts of two
+// tiles are 64 registers, and is cut while the first blocks are on their way.
+// 16 x 4096 keys, 16/4 heads: 15.4 us, of which 2.3 to q and the first blocks, 0.9 q's cut, 6.5 the blocks (four
+// pairs a wave, two waves a SIMD: about 300 vector instructions a pair bind them, not the 2.4 TB/s), 2 until
+// the slowest wave's results are in LDS, 1.2 the hand-off. 4 x 131072, 32/8 heads: 145 us, 4.2 TB/s. Two
+// tiles (16 x 5 rows): 27.8 us.
 template <int NT>
 __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_decode_q4(
     const AttnItem* __restrict__ items, const uint32_t* pos, const uint32_t* __restrict__ pages,
@@ -584,6 +589,9 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
 // blocks. A pair of blocks is made into operands once for the four waves: K's codes (a dword of each
 // lane, group p by wave p) and V's hi and lo parts (tiles 2 w, 2 w + 1, which share group w's steps),
 // through LDS, two pairs deep with one barrier a pair. q is in registers.
+// 512 rows after 24000 keys, 20/4 heads: 318 us (each wave by itself converting, q in LDS: 360). What bounds it is
+// the waves' own order of instructions: 80 matrix instructions (1280 cycles), 256 vector and 28 LDS
+// ones a pair take a wave 4000 cycles alone and two of a SIMD 5000 each. Four tiles a wave spill.
 static constexpr int kQ4TileWaves = 4;
 static constexpr int kQ4WaveTiles = 2;
 static constexpr int kQ4TileRows = kQ4TileWaves * kQ4WaveTiles * 16;

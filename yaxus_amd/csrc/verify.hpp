@@ -16,12 +16,16 @@
 // 151936 logits, less than the 9 us that reading them takes.
 //
 // Launch 1 reads every chunk of 4096 logits (target and draft rows): its maximum M_c and
-// sum e^((l - M_c) / t). Launch 2, a workgroup per sequence (per chunk and sequence where drafts
-// have logits): adds the chunks up and decides, every workgroup of a sequence by itself; then draws
-// where one row's chunk sums say enough (accepted all, certain drafts, temperature 0): the chunk by
-// its cumulative sum, then the token within it. Where they don't, each workgroup adds up its chunk
-// of the residual and the last of the sequence to arrive draws. Chunk order fixes every sum's
-// order: the same answer every time.
+// sum e^((l - M_c) / t). Launch 2, a workgroup per sequence (where drafts have logits several, each
+// with an equal share of the chunks, at most one a CU over all sequences): adds the chunks up and decides,
+// every workgroup of a sequence by itself; then draws where one row's chunk sums say enough (accepted
+// all, certain drafts, temperature 0): the chunk by its cumulative sum, then the token within it. Where
+// they don't, each workgroup adds up its chunks of the residual and the last of the sequence to
+// arrive draws. Chunk order fixes every sum's order: the same answer every time.
+//
+// Measured: launch 1 is bound by reading (249 rows of 151936: 38 us, 4.0 TB/s), launch 2 by its chain of
+// trips to memory (sums, decision, residual, arrival, draw): 12 us for one sequence of 5 drafts, 18 for 16 of 4, 9
+// where no residual of two rows is drawn from.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
