@@ -284,6 +284,27 @@ def test_sizes_of_values_in_tiles(hip, kscale, qscale, vscale, scale):
         sc.kv.destroy()
 
 
+@pytest.mark.parametrize("qscale,scale", [(1e-20, 0.0), (1e-30, 1e-25), (1e-42, None)])
+@pytest.mark.parametrize("rows", [1, 66])
+def test_scores_too_small_for_f32(hip, qscale, scale, rows):
+    """The factor from products to scores is below f32's range: every key weighs the same, and masked
+    keys nothing."""
+    sc = Q4Scenario(hip, 70, 16, 1)
+    try:
+        seqs = [sc.cache.new_seq() for _ in range(2)]
+        sc.fill(dict(zip(seqs, [300, 33])))
+        sc.begin([(s, rows) for s in seqs])
+        k, v = sc.new_kv_rows()
+        q = sc.draw(2 * rows, 4 * D) * np.float32(qscale)
+        hip.set_option("prefill_min_rows", 2)
+        got = hip.attend_append(sc.kv, 0, k, v, q, 4, window=100, scale=scale)
+        sc.keep(k, v)
+        sc.check(got, q, 4, window=100, scale=scale)
+    finally:
+        hip.set_option("prefill_min_rows", 0)
+        sc.kv.destroy()
+
+
 @pytest.mark.parametrize("priors,rows,hq,hkv,page,window", [
     ([17, 0], [1, 40], 32, 1, 16, None),               # 4 rows a tile; a tile of one row
     ([1000], [131], 1, 1, 16, 9),                      # 128 rows a tile, each wave its own keys

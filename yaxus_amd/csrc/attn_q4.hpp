@@ -136,7 +136,9 @@ __device__ __forceinline__ float q4_cut_q(float4 (&raw)[8], float scale_log2, u3
       lo[p][2 * j] = l0;
       lo[p][2 * j + 1] = l1;
     }
-  return __builtin_ldexpf(fmaxf(fabsf(scale_log2), 0x1p-90f), ex - 13);
+  // Never 0, which a masked -inf would make NaN (products are below 2^40: 2^-126 times them is nothing).
+  const float size = fabsf(scale_log2) < 0x1p-90f ? 0x1p-90f : fabsf(scale_log2), fac = __builtin_ldexpf(size, ex - 13);
+  return fac < 0x1p-126f ? 0x1p-126f : fac;
 }
 
 // Whether a result of the wave is an infinity or NaN.

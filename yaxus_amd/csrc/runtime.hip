@@ -2935,15 +2935,16 @@ int yx_verify_drafts_dev(yx_ctx* c, const float* logits, size_t cols, size_t ld,
     return draft_logits ? 2 * t - (b - a) : t;
   };
   const size_t most = std::min(kMostRows, (size_t{1} << 28) / nch - 1);
-  std::vector<size_t> cuts{0};
-  size_t part_rows = 0;
-  while (cuts.back() < seqs) {
-    const size_t a = cuts.back();
+  const auto launch_end = [&](size_t a) {
     size_t b = a + 1;
-    if (launch_rows(a, b) > most) return fail(YX_ERR_UNSUPPORTED, "too many drafts of one sequence");
     while (b < seqs && b - a < yx::kVdSeqs && launch_rows(a, b + 1) <= most) ++b;
+    return b;
+  };
+  size_t part_rows = 0;
+  for (size_t a = 0, b; a < seqs; a = b) {
+    b = launch_end(a);
+    if (launch_rows(a, a + 1) > most) return fail(YX_ERR_UNSUPPORTED, "too many drafts of one sequence");
     part_rows = std::max(part_rows, launch_rows(a, b));
-    cuts.push_back(b);
   }
   int rc = c->set_device();
   if (rc) return rc;
@@ -2954,8 +2955,9 @@ int yx_verify_drafts_dev(yx_ctx* c, const float* logits, size_t cols, size_t ld,
   if ((rc = c->vd_counters.ensure(counter_bytes, c->stream, true))) return rc;
   auto* parts = static_cast<yx::VerifyPart*>(c->vd_parts.p);
   auto* counters = static_cast<uint32_t*>(c->vd_counters.p);
-  for (size_t i = 0; i + 1 < cuts.size(); ++i) {
-    const size_t a = cuts[i], n = cuts[i + 1] - a, row0 = row_off[a], d0 = row0 - a;
+  for (size_t a = 0, n; a < seqs; a += n) {
+    n = launch_end(a) - a;
+    const size_t row0 = row_off[a], d0 = row0 - a;
     yx::VerifyRows vr{};
     vr.seqs = static_cast<uint32_t>(n);
     for (size_t s = 0; s <= n; ++s) vr.off[s] = row_off[a + s] - row_off[a];
