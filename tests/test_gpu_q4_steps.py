@@ -168,7 +168,7 @@ def test_a_layer_as_the_model_calls_it(hip, rows):
 
 
 @pytest.mark.parametrize("priors,rows,window", [
-    ([700, 33, 5], 1, 0), ([700, 33], 6, 0), ([3000, 100], 1, 64), ([40, 900], 130, 0), ([6000], 40, 0), ([9000], 500, 0)])
+    ([700, 33, 5], 1, 0), ([700, 33], 6, 0), ([3000, 100], 1, 64), ([40, 900], 130, 0), ([6000], 40, 0), ([4000], 250, 0)])
 def test_the_call_that_allocates_nothing(hip, priors, rows, window):
     """The bits of the allocating call where both split alike, and correct in any case; twice in a row."""
     hq, hkv = 8, 2
@@ -328,6 +328,28 @@ def test_tiles(hip, priors, rows, hq, hkv, page, window):
         assert np.array_equal(bits(hip.attend(sc.kv, 0, q, hq, window=window)), bits(got))
     finally:
         hip.set_option("prefill_min_rows", 0)
+        sc.kv.destroy()
+
+
+@pytest.mark.parametrize("lens,rows,hq,hkv,window", [
+    ([70 + 3 * i for i in range(140)], 1, 8, 4, None),       # two items to a CU, four waves each
+    ([5 * i for i in range(70)], 4, 32, 8, None),            # of two tiles
+    ([900 + i for i in range(66)], 2, 16, 8, 300),
+    ([4200 + i for i in range(33)], 1, 8, 8, None),          # items too long for four waves' page ids
+])
+def test_many_sequences(hip, lens, rows, hq, hkv, window):
+    sc = Q4Scenario(hip, sum(-(-(n + rows) // 16) for n in lens) + 4, 16, hkv, pool_seed=2)
+    try:
+        seqs = [sc.cache.new_seq() for _ in lens]
+        sc.fill({s: n for s, n in zip(seqs, lens) if n}, chunk=1 << 15)
+        sc.begin([(s, rows) for s in seqs])
+        k, v = sc.new_kv_rows()
+        q = sc.draw(len(sc.meta.pos), hq * D)
+        got = hip.attend_append(sc.kv, 0, k, v, q, hq, window=window)
+        sc.keep(k, v)
+        sc.check(got, q, hq, window)
+        assert np.array_equal(bits(hip.attend(sc.kv, 0, q, hq, window=window)), bits(got))
+    finally:
         sc.kv.destroy()
 
 

@@ -505,21 +505,29 @@ __device__ __forceinline__ void q4_rows(Q4Rows<NT>& rows, Q4Raw<NT>& raw, uint32
   rows.any_pos = -__builtin_amdgcn_readfirstlane(row16_min(-any_pos));
 }
 
-// Decode and verify: a work item's blocks dealt evenly over 8 waves, as the binary16 arena's
-// 16-row-tile kernel, whose items, hand-off and merge these are. q lies in LDS, since its parts of two
+// Decode and verify: a work item's blocks dealt evenly over W waves: 8, one item to a CU, or 4, two
+// (build_plan chooses). Items, hand-off and merge are those of the binary16 arena's 16-row-tile kernel. q lies in LDS, since its parts of two
 // tiles are 64 registers, and is cut while the first blocks are on their way.
 // 16 x 4096 keys, 16/4 heads: 15.4 us, of which 2.3 to q and the first blocks, 0.9 q's cut, 6.5 the blocks (four
 // pairs a wave, two waves a SIMD: about 300 vector instructions a pair bind them, not the 2.4 TB/s), 2 until
 // the slowest wave's results are in LDS, 1.2 the hand-off. 4 x 131072, 32/8 heads: 145 us, 4.2 TB/s. Two
 // tiles (16 x 5 rows): 27.8 us.
-template <int NT>
-__global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_decode_q4(
+template <int NT, int W>
+struct Q4Shared {
+  float m[W][NT * 16];
+  float l[W][NT * 16];
+  float4 o[W][NT * 16][kD / 4];
+  uint32_t last;
+};
+
+template <int NT, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_decode_q4(
     const AttnItem* __restrict__ items, const uint32_t* pos, const uint32_t* __restrict__ pages,
     const q4_t* __restrict__ kc, const q4_t* __restrict__ vc, const float* q, float* __restrict__ out,
     float* __restrict__ part_o, float2* __restrict__ part_ml, uint32_t* __restrict__ counters, uint32_t part_o_bytes,
     uint32_t part_ml_bytes, uint32_t hq, uint32_t hkv, uint32_t bpp_shift, uint32_t window, float scale_log2,
     const SubRef* __restrict__ members, uint32_t by_item) {
-  __shared__ WideShared<NT, false> sh;
+  __shared__ Q4Shared<NT, W> sh;
   const AttnItem it = items[by_item ? blockIdx.y : blockIdx.x];
   const uint32_t kh = by_item ? blockIdx.x : blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -528,8 +536,8 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
   const uint32_t G = hq / hkv;
   const uint32_t nlog = it.nrows * G;  // at most NT * 16
   const uint32_t nall = it.blk1 - it.blk0;
-  const uint32_t wb0 = it.blk0 + nall * wave / kWideWaves;
-  const uint32_t wb1 = it.blk0 + nall * (wave + 1) / kWideWaves;
+  const uint32_t wb0 = it.blk0 + nall * wave / W;
+  const uint32_t wb1 = it.blk0 + nall * (wave + 1) / W;
 
   Q4Rows<NT> rows;
   Q4Wave<NT> w;
@@ -565,17 +573,17 @@ __global__ __launch_bounds__(64 * kWideWaves) __attribute__((amdgpu_waves_per_eu
       for (int n = 0; n < 8; ++n) sh.o[wave][lr][n * 4 + g] = __builtin_bit_cast(float4, w.o[t][n]);
   }
   __syncthreads();
-  finish_item<64 * kWideWaves, NT * 16, true>(it, kh, G, hq, hkv, nlog, out, part_o, part_ml, counters, part_o_bytes,
+  finish_item<64 * W, NT * 16, true>(it, kh, G, hq, hkv, nlog, out, part_o, part_ml, counters, part_o_bytes,
                                               part_ml_bytes, sh.last,
                                               [&](uint32_t lr, uint32_t qi, float& mt, float& lt, float4& o) {
     mt = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < kWideWaves; ++v) mt = fmaxf(mt, sh.m[v][lr]);
+    for (int v = 0; v < W; ++v) mt = fmaxf(mt, sh.m[v][lr]);
     lt = 0.0f;
     o = float4{0, 0, 0, 0};
     const float mf = fmaxf(mt, kLowest);
 #pragma unroll
-    for (int v = 0; v < kWideWaves; ++v) {
+    for (int v = 0; v < W; ++v) {
       const float wt = __builtin_amdgcn_exp2f(sh.m[v][lr] - mf);  // 0 for an empty wave
       lt += sh.l[v][lr] * wt;
       const float4 ow = sh.o[v][lr][qi];

@@ -182,6 +182,7 @@ struct AttnPlan {
   bool wide = false;  // 16-row tiles (the wide kernel) instead of 8-row ones
   bool f32 = false;   // the f32-arena kernel
   bool q4 = false;    // the 4-bit-arena kernels
+  int q4_waves = yx::kWideWaves;  // of their decode items: 8, or 4
   int pf32_waves = 8;  // f32 prefill tiles: 8 waves (128 logical rows) or 4 (64)
   std::vector<yx::AttnItem> items;
   DevBuf d_items;
@@ -1300,6 +1301,23 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
   }
   plan.f32 = f32;
   plan.q4 = q4;
+  // 4-bit items of two rounds, or of more than one where it ends earlier: of 4 waves, two items to a
+  // CU. An item's blocks then take twice as long, but its start and hand-off lie beside the other's
+  // blocks. Measured (8 waves / 4): 256 x 1 row after 1000, 16/4 heads, 59.7 / 43.8 us, 512 after 100-500
+  // 76.6 / 44.7, 64 x 2 after 100-3000, 32/8 heads, 35.1 / 27.9, 128 x 5 after 100-600 35.0 / 21.6, 134 x 1 after 1230,
+  // 2 KV heads (268 items), 35.0 / 24.5; not 48 after 60-12000 (300 items) 26.5 / 28.9, 64 after 500-1500
+  // (280) 18.0 / 18.5.
+  if (q4 && plan.items.size() * hkv > static_cast<size_t>(c->cus)) {
+    bool fits = true;  // a wave's page ids its 64 lanes
+    for (const yx::AttnItem& w : plan.items) fits &= w.blk1 - w.blk0 <= 64 * 4;
+    auto busiest = [&](uint32_t times, size_t slots) {
+      deal.clear();
+      for (const yx::AttnItem& w : plan.items) deal.add(times * (w.blk1 - w.blk0) + kStartBlocks, 1);
+      return deal.busiest(slots);
+    };
+    if (fits && (plan.items.size() * hkv >= 2 * static_cast<size_t>(c->cus) || busiest(2, 2 * head_slots) < busiest(1, head_slots)))
+      plan.q4_waves = 4;
+  }
   plan.balanced = !f32 && !q4 && nt == 1 && c->decode_shape == 0;
   for (const yx::AttnItem& w : plan.items)
     if (w.blk1 - w.blk0 > 4 * yx::kBalQuads) plan.balanced = false;
@@ -1515,8 +1533,11 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
                        vnew, c->dev_slot, kv->kf(layer),
                        kv->vf(layer), po_bytes, pml_bytes, H, HK, P, W, scale_log2, mem, by_item);
   } else if (plan->q4) {
-    auto* kern = plan->nt <= 2 ? yx::paged_attn_decode_q4<1> : yx::paged_attn_decode_q4<2>;
-    hipLaunchKernelGGL(kern, grid, dim3(64 * yx::kWideWaves), 0, c->stream, items, pos, pages, kv->kq(layer),
+    const bool narrow = plan->q4_waves == 4;
+    auto* kern = plan->nt <= 2 ? (narrow ? yx::paged_attn_decode_q4<1, 4> : yx::paged_attn_decode_q4<1, 8>)
+                               : (narrow ? yx::paged_attn_decode_q4<2, 4> : yx::paged_attn_decode_q4<2, 8>);
+    static_assert(yx::kWideWaves == 8, "the other kernel's items");
+    hipLaunchKernelGGL(kern, grid, dim3(64 * plan->q4_waves), 0, c->stream, items, pos, pages, kv->kq(layer),
                        kv->vq(layer), q, out, po, pml, cnt, po_bytes, pml_bytes, H, HK, P, W, scale_log2, mem, by_item);
   } else if (plan->balanced && !plan->wide) {
 #define YX_LAUNCH_BAL(QKV, UB, KN, VN, IN)                                                          \
