@@ -612,13 +612,13 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
     must_fit = decode_us <= 95.0 + 2.4 * max_keys / 1024.0;
     if (G > 16) use_prefill = max_rows * G > 16 && !must_fit;
   } else if (q4) {
-    // The 4-bit arena: one decode item (32 logical rows, 8 waves with a share of its blocks each)
-    // per CU takes 14 us and 1.6 ns per pair of blocks over all items; prefill tiles 10 us and 2.1
-    // per pair of the split chosen below. The kernel with the smaller estimate runs. Measured (B x rows after ctx,
-    // 16/4 heads, decode / prefill us): 1 x 256 after 0 17 / 26, 1 x 128 after 4096 33 / 68, 1 x 64
-    // after 32768 65 / 181, 16 x 16 after 4096 44 / 70, 16 x 24 61 / 75, 16 x 64 122 / 108, 4 x 256
-    // after 2000 79 / 73, 16 x 128 after 1000 111 / 74, 1 x 2048 after 0 108 / 77, 1 x 1024 after
-    // 8000 252 / 185; 32/8 heads, 64 x 64 after 64 258 / 48, 2 x 64 after 16384 152 / 133.
+    // The 4-bit arena: decode items (32 logical rows each) take 14 us, or 7 for each of several per CU,
+    // and 1.7 ns per pair of blocks over all items; prefill tiles 10 us and 2.1 per pair of the split
+    // chosen below. The kernel with the smaller estimate runs. Measured (B x rows after ctx, 16/4 heads,
+    // decode / prefill us): 1 x 512 after 0 21 / 40, 1 x 128 after 4096 33 / 68, 1 x 64 after 32768 66 / 181,
+    // 64 x 16 after 1000 40 / 63, 16 x 24 after 4096 61 / 75, 16 x 64 124 / 109, 4 x 256 after 2000 64 / 74, 16 x
+    // 128 after 1000 75 / 74, 1 x 1024 after 8000 252 / 187; 32/8 heads, 64 x 64 after 64 114 / 48, 2 x 64 after
+    // 16384 152 / 134.
     use_prefill = max_rows * G > 32;
     if (use_prefill) {
       double items = 0, pairs = 0;
@@ -634,7 +634,7 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
         items += of_group;
         pairs += of_group * keys / g.n / 32;
       }
-      q4_decode_us = rows_per_item ? 14 * std::max(1.0, items * hkv / c->cus) + 1.6e-3 * pairs * hkv : 1e30;
+      q4_decode_us = rows_per_item ? std::max(14.0, 7 * items * hkv / c->cus) + 1.7e-3 * pairs * hkv : 1e30;
     }
   } else {
     size_t tiles = 0;
