@@ -98,7 +98,7 @@ def test_any_split_of_the_keys(hip, chunk):
         sc.kv.destroy()
 
 
-@pytest.mark.parametrize("forks,prefix,rows,hq", [(6, 700, 1, 4), (16, 1024, 1, 16), (5, 300, 2, 4)])
+@pytest.mark.parametrize("forks,prefix,rows,hq", [(6, 700, 1, 4), (16, 1024, 1, 16), (5, 300, 2, 4), (40, 520, 1, 32)])
 def test_forks_of_a_prompt(hip, forks, prefix, rows, hq):
     sc = Q4Scenario(hip, 400, 16, hq // 4, pool_seed=2)
     try:
