@@ -792,7 +792,7 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
         consider(Split{0, 0});
         // 4-bit tiles: the shortest chunks that one round of slots holds. Their pairs are short
         // next to a start, so a second round's few items cost more than kTail says (512 rows
-        // after 24000 keys, 24/4 heads: 411 us without this choice, 360 with it).
+        // after 24000 keys, 20/4 heads: 411 us without this choice, 360 with it).
         if (q4) {
           const size_t slots = std::max<size_t>(1, slots2 / hkv);
           auto items_of = [&](uint32_t n) {
