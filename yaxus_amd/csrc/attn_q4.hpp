@@ -15,6 +15,7 @@
 // size does not matter; the cuts keep ~2^-22. A binary16 holds V's parts (and 16 times them) below
 // 4096: a wave whose result is not finite runs again, once for the steps from 1 up, scaled down,
 // and once for the others, with steps of NaN (or infinite) left out and noted where a row sees them.
+// So does a wave with scores beyond 2^16, whose weights need another form (q4_is_far).
 // Steps of keys that no row of the wave sees are cleared at once. So a masked key never has an
 // effect, whatever it holds.
 //
@@ -141,17 +142,37 @@ __device__ __forceinline__ float q4_cut_q(float4 (&raw)[8], float scale_log2, u3
   return fac < 0x1p-126f ? 0x1p-126f : fac;
 }
 
-// Whether a result of the wave is an infinity or NaN.
+// Scores this large need the second form below. 2^(x + (kQ4Room - m)) is one multiply-add a score,
+// with a sum in brackets that is rounded, and x exact where m is a rounded product: up to 2^16 both
+// are off by 2^-8, so weights stay below 2^(kQ4Room + kQ4Lazy + 2^-7), in binary16's range; from
+// 2^26 on kQ4Room would round to 16 or to nothing. (Scores of ordinary models are some hundreds.)
+static constexpr float kQ4Far = 0x1p16f;
+__device__ __forceinline__ bool q4_is_far(float m) { return fabsf(m) > kQ4Far && m > -INFINITY; }
+
+// A weight in the slow runs: a row's is made by the same form in every wave. Where the maximum is
+// far, the product is rounded as the maximum's was, so their difference is exact near it and at most
+// kQ4Lazy whatever their size.
+__device__ __forceinline__ float q4_slow_weight(float score, float fac, float m) {
+  float x = score * fac;
+  pin(x);  // no multiply-add with the difference
+  const float far = (x - fmaxf(m, kLowest)) + kQ4Room, near = __builtin_fmaf(score, fac, kQ4Room - fmaxf(m, kLowest));
+  return __builtin_amdgcn_exp2f(q4_is_far(m) ? far : near);
+}
+
+// Whether the wave runs again: a result is an infinity or NaN, or a row's maximum is far.
 template <int NT>
-__device__ __forceinline__ bool q4_bad(const floatx4 (&acc)[NT][8]) {
+__device__ __forceinline__ bool q4_again(const floatx4 (&acc)[NT][8], const float (&m)[NT]) {
   float bad = 0.0f;
+  bool far = false;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < NT; ++t) {
+    far |= q4_is_far(m[t]);
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) bad += acc[t][n][i] * 0.0f;
-  return __builtin_amdgcn_ballot_w64(bad != 0.0f) != 0;
+  }
+  return __builtin_amdgcn_ballot_w64(far | (bad != 0.0f)) != 0;
 }
 
 // The wave's results and sums, without the operands' powers of two.
@@ -168,7 +189,7 @@ __device__ __forceinline__ void q4_done(Q4Wave<NT>& w, const floatx4 (&acc)[NT][
 // kSlots: pairs of blocks a wave holds; each half (K, V) is loaded again as soon as it is used up.
 // q(t, p, part): the operand of tile t.
 // begin(): the wave's q and rows, made ready while the first blocks are on their way.
-// kFast false: only the two runs of a wave whose fast one, made elsewhere, was not finite.
+// kFast false: only the two runs of a wave whose fast one, made elsewhere, does not do (q4_again).
 template <int NT, int kSlots, bool kLong, int kPolicy, bool kFast, typename Q, typename Begin>
 __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict__ kc, const q4_t* __restrict__ vc,
                                           const uint32_t* __restrict__ pt, uint32_t b0, uint32_t nblk,
@@ -312,7 +333,8 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
         const float base = kQ4Room - fmaxf(w.m[t], kLowest);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e >> 2][e & 3], rows.fac[t], base));
+          if constexpr (kSlow) x[e] = q4_slow_weight(sc[t][e >> 2][e & 3], rows.fac[t], w.m[t]);
+          else x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e >> 2][e & 3], rows.fac[t], base));
           w.l[t] += x[e];
         }
 #pragma unroll
@@ -424,7 +446,7 @@ __device__ __forceinline__ void q4_attend(Q4Wave<NT>& w, const q4_t* __restrict_
     }
   };
   if constexpr (kFast) pass(std::false_type{}, false);
-  if (!kFast || q4_bad<NT>(acc)) {
+  if (!kFast || q4_again<NT>(acc, w.m)) {
     pass(std::true_type{}, false);
     pass(std::true_type{}, true);
 #pragma unroll
@@ -923,7 +945,7 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
     }
   }
   others(nblk);
-  if (q4_bad<NT>(acc)) {  // again, a tile at a time with q in LDS (the operands' space is free)
+  if (q4_again<NT>(acc, w.m)) {  // again, a tile at a time with q in LDS (the operands' space is free)
     half8 (*const qs)[64] = reinterpret_cast<half8 (*)[64]>(stages) + wave * 8;
     static_assert(sizeof(stages) >= kQ4TileWaves * 8 * sizeof(*qs), "q fits");
 #pragma unroll
