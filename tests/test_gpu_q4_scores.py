@@ -1,5 +1,6 @@
-"""4-bit arena: rows whose scores are far below or above zero, up to f32's range; decode items of one
-and two tiles, of eight and four waves, and tiles, whole and split."""
+"""4-bit arena: rows whose scores are far below or above zero, up to f32's range, and factors from
+products to scores at its lower end; decode items of one and two tiles, of eight and four waves,
+and tiles, whole and split."""
 
 import numpy as np
 import pytest
@@ -116,5 +117,21 @@ def test_one_key_leads(hip, how, kscale, qscale):
                 else:
                     assert np.abs(got[r, h]).max() <= np.abs(vh).max() * (1 + 2.0 ** -12)
         assert clear > 0.9 * p.n * p.hq
+    finally:
+        p.sc.kv.destroy()
+
+
+@pytest.mark.parametrize("qscale,scale", [
+    (2.0 ** 100, 0.0), (2.0 ** 120, 0.0), (2.0 ** 120, -0.0), (2.0 ** 100, 1e-31), (2.0 ** 100, -1e-31), (2.0 ** 124, 4e-39),
+    (2.0 ** 40, 1e-31), (2.0 ** 90, 1e-40)])
+@pytest.mark.parametrize("how", HOW)
+def test_scales_near_zero(hip, how, qscale, scale):
+    """A scale of 0: every key weighs the same, whatever q. Small ones: the scores they make."""
+    rng = np.random.default_rng(5)
+    p = Pass(hip, how, lambda t, hkv: rng.standard_normal((t, hkv, D)))
+    try:
+        q = (qscale * np.clip(rng.standard_normal((p.n, p.hq, D)), -4, 4)).astype(np.float32)
+        got = p.attend(q, scale)
+        p.sc.check(got.reshape(p.n, -1), q, p.hq, scale=float(np.float32(scale)))
     finally:
         p.sc.kv.destroy()

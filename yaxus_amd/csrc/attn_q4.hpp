@@ -108,7 +108,7 @@ struct Q4Rows {
 
 // A tile's q (this lane's dims 32 p + 8 g + 0 .. 7 of its column) as operands: hi and lo parts
 // scaled by a power of two; returns the factor from products to log2 scores. The scale's sign goes
-// into q, and a scale of 0 becomes one without effect, so that the factor is positive: the maximum
+// into q, and a factor of 0 becomes one without effect, so that it is positive: the maximum
 // may be looked for before it, and a masked -inf stays one.
 __device__ __forceinline__ float q4_cut_q(float4 (&raw)[8], float scale_log2, u32x4 (&hi)[4], u32x4 (&lo)[4]) {
   float top = 0.0f;
@@ -137,8 +137,9 @@ __device__ __forceinline__ float q4_cut_q(float4 (&raw)[8], float scale_log2, u3
       lo[p][2 * j] = l0;
       lo[p][2 * j + 1] = l1;
     }
-  // Never 0, which a masked -inf would make NaN (products are below 2^40: 2^-126 times them is nothing).
-  const float size = fabsf(scale_log2) < 0x1p-90f ? 0x1p-90f : fabsf(scale_log2), fac = __builtin_ldexpf(size, ex - 13);
+  // At least 2^-126, never 0, which a masked -inf would make NaN: products are below 2^40, so such a
+  // score is 2^-86 at most, as good as 0. A scale of 0 is that whatever q's size.
+  const float fac = scale_log2 == 0.0f ? 0.0f : __builtin_ldexpf(fabsf(scale_log2), ex - 13);
   return fac < 0x1p-126f ? 0x1p-126f : fac;
 }
 
