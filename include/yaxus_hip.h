@@ -288,13 +288,14 @@ int yx_logprobs_rows_dev(yx_ctx* ctx, const float* logits, size_t rows, size_t c
  * q the draft row's, draft x is accepted while accept_u q(x) < p(x); next[s] is the first token
  * whose cumulative weight, in index order, exceeds pick_u[s] times all weights, of max(p - q, 0)
  * at the first rejected draft (of p where that is nowhere positive), or of the last row's p when
- * every draft stands: accepted[s] of them. Uniform numbers from [0, 1); all comparisons and sums
- * in 64 bits, the same answer every time.
+ * every draft stands: accepted[s] of them. Uniform numbers from [0, 1), 0 among them. Weights are
+ * within 2^-47, comparisons and sums in 64 bits, the same answer every time.
  * draft_logits null: the drafts were certain (copied, not drawn), q(x) = 1. temperature null: 1
  * everywhere; a temperature of 0 (or below, or NaN): p is 1 at the first of the largest logits,
  * and q does not matter. Logits of -inf, and NaN, are masked tokens: probability 0, never
  * accepted, never drawn; +inf takes all of its row. A target row of nothing else accepts nothing
- * and gives YX_NO_TOKEN; a draft row of nothing else counts as q = 0. A draft of `cols` or more is
+ * and gives YX_NO_TOKEN; a draft row of nothing else counts as q = 0. A token less than 2^-1000
+ * times as likely as its row's most likely has probability 0 too. A draft of `cols` or more is
  * rejected. At most 4194304 columns. Everything but row_off lies on the device; accepted and next
  * `[seqs]` overlap neither the inputs nor each other. A captured call keeps its row_off. */
 int yx_verify_drafts_dev(yx_ctx* ctx, const float* logits, size_t cols, size_t ld, const uint32_t* row_off,

@@ -97,10 +97,12 @@ __device__ __forceinline__ double vd_exp2(double t) {
   return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | static_cast<uint32_t>(bits));
 }
 
-// Weight of a logit relative to the maximum m (above -inf), c = log2(e) / temperature.
+// Weight of a logit relative to the maximum m (above -inf), c = log2(e) / temperature. Below 2^-1000
+// there is none: a token far below, beside +inf, of -inf or NaN (the differences -inf and NaN) is
+// never accepted or drawn, at numbers of 0 either.
 __device__ __forceinline__ double vd_weight(float x, float m, double c) {
-  const double w = vd_exp2((static_cast<double>(x) - static_cast<double>(m)) * c);
-  return x == m ? 1.0 : x > -INFINITY ? w : 0.0;  // (a NaN: 0)
+  const double t = (static_cast<double>(x) - static_cast<double>(m)) * c, w = vd_exp2(t);
+  return x == m ? 1.0 : t >= -1000.0 ? w : 0.0;
 }
 
 // log2(e) / temperature; -1 for temperature 0 (and below, and NaN).
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(kVdSumThreads) void verify_sums(VerifyRows rows, Ve
   m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
   double s = 0.0;
   uint32_t at = YX_NO_TOKEN;
-  const bool plain = c > 0x1p-100 && m > -INFINITY && m < INFINITY;  // masked tokens then add 2^-1000 at most
+  const bool plain = c > 0x1p-100 && m > -INFINITY && m < INFINITY;  // tokens without weight then add 2^-1000 each, nothing beside 1
   if (c < 0.0 || !plain) {
     // Temperature 0: the first of the largest. A row of nothing, +inf, temperatures beyond 2^100: the exact form.
 #pragma unroll
