@@ -247,8 +247,8 @@ void* g_scratch_ptr[kMaxDevices] = {};
 // recorded there at the hand-over), so calls on different streams do not overlap on
 // the scratch.
 using PlanKey = std::tuple<size_t, size_t, size_t, int, size_t>;  // (window, hq, hkv, dtype, page)
-// With the dtype: a 4-bit arena's plan whose partials fit the scratch of the entry point that
-// allocates nothing (other arenas' plans serve both).
+// With the dtype: a 4-bit arena's plan for the entry point that allocates nothing, whose partials fit
+// its scratch wherever tiles or decode items can be cut so (other arenas' plans serve both).
 constexpr int kFitScratch = 0x100;
 struct ScratchOwner {
   const yx_ctx* ctx = nullptr;
@@ -424,6 +424,20 @@ struct yx_ctx {
 
 namespace {
 
+// Logical rows of a plan's partial slot: the kernel's tile rows.
+size_t partial_rows(const AttnPlan& p) {
+  return p.prefill ? p.part_rows : p.wide ? static_cast<size_t>((p.nt + 1) / 2) * 16 : static_cast<size_t>(p.nt) * 8;
+}
+
+// Whether the scratch holds a plan's partials, arrival counters and lists.
+bool fits_scratch(const AttnPlan& p, size_t hkv) {
+  auto r256 = [](size_t b) { return (b + 255) & ~static_cast<size_t>(255); };
+  const size_t rows = p.slots * hkv * partial_rows(p);
+  return p.counters * hkv * 4 * yx::kCounterStride <= kScratchCounterBytes &&
+         r256(p.item_bytes()) + r256(p.members.size() * sizeof(yx::SubRef)) <= kScratchListBytes &&
+         kScratchCounterBytes + kScratchListBytes + r256(rows * sizeof(float2)) + r256(rows * yx::kD * sizeof(float)) <= kScratchBytes;
+}
+
 // Regions of the device's scratch for one no-alloc call; refuses sizes beyond it.
 int scratch_map(yx_ctx* c, size_t part_ml, size_t part_o, size_t counters, ScratchMap* m) {
   char* base = static_cast<char*>(g_scratch_ptr[c->device]);
@@ -570,6 +584,22 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
   // 81.5 / 70.7.
   bool use_prefill, must_fit = false;
   double q4_decode_us = 0;  // 4-bit arena: estimate of the pass as decode items
+  AttnPlan tiles_plan;      // and its tiles, where decode items are the faster choice but may not do
+  bool have_tiles = false;
+  auto take_tiles = [&](AttnPlan&& tiles) {
+    c->split_tiles += tiles.counters;
+    ++c->prefill_plans;
+    // Longest first: the GPU hands work items to CUs in order as they free up, so
+    // this bounds the busiest CU near the average (contexts differ a lot in a pass).
+    std::stable_sort(tiles.pitems.begin(), tiles.pitems.end(),
+                     [](const yx::PrefillItem& a, const yx::PrefillItem& b) {
+                       return a.blk1 - a.blk0 > b.blk1 - b.blk0;
+                     });
+    auto& p = c->plans[key];
+    p = std::move(tiles);
+    *out = &p;
+    return YX_OK;
+  };
   if (c->prefill_min_rows > 0) {
     use_prefill = max_rows >= static_cast<uint32_t>(c->prefill_min_rows);
   } else if (f32) {
@@ -843,20 +873,11 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
       plan.pitems = std::move(split);
       plan.slots = nslot;
       plan.counters = ncnt;
-      if (use_prefill) c->split_tiles += ncnt;
     }
-    if (use_prefill) {
-      ++c->prefill_plans;
-      // Longest first: the GPU hands work items to CUs in order as they free up, so
-      // this bounds the busiest CU near the average (contexts differ a lot in a pass).
-      std::stable_sort(plan.pitems.begin(), plan.pitems.end(),
-                       [](const yx::PrefillItem& a, const yx::PrefillItem& b) {
-                         return a.blk1 - a.blk0 > b.blk1 - b.blk0;
-                       });
-      auto& p = c->plans[key];
-      p = std::move(plan);
-      *out = &p;
-      return YX_OK;
+    if (use_prefill) return take_tiles(std::move(plan));
+    if (q4) {
+      tiles_plan = std::move(plan);
+      have_tiles = true;
     }
   }
   size_t nt = (max_rows * G + 7) / 8;
@@ -1179,8 +1200,10 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
     const Casc& cc = cascs[ci];
     const uint32_t nq = (cc.blocks + 3) / 4;
     const uint32_t cq = chunk_quads(nq, cb);
-    if (cq * 4 > 64 * waves)  // each wave's page ids fit its 64 lanes
+    if (cq * 4 > 64 * waves) {  // each wave's page ids fit its 64 lanes
+      if (have_tiles) return take_tiles(std::move(tiles_plan));
       return fail(YX_ERR_UNSUPPORTED, "shared prefix too long for 256 chunks of the widest work item");
+    }
     const uint32_t nch = (nq + cq - 1) / cq;
     casc_base[ci] = static_cast<uint32_t>(slot);
     casc_nch[ci] = nch;
@@ -1217,8 +1240,10 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
     // kMaxChunks of them.
     const uint32_t nq = (s.b1 - s.b0 + 3) / 4;
     const uint32_t cq = chunk_quads(nq, cb);
-    if (cq * 4 > 64 * waves)
+    if (cq * 4 > 64 * waves) {
+      if (have_tiles) return take_tiles(std::move(tiles_plan));
       return fail(YX_ERR_UNSUPPORTED, "context too long for 256 chunks of the widest work item");
+    }
     const uint32_t nch = (nq + cq - 1) / cq;
     for (uint32_t ch = 0; ch < nch; ++ch) {
       yx::AttnItem w{};
@@ -1344,6 +1369,8 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
   plan.slots = slot;
   plan.counters = subs.size();
   if (plan.items.size() > 0x7fffffff) return fail(YX_ERR_UNSUPPORTED, "too many work items");
+  // (16 x 16 rows after 131072 keys, 16/4 heads: 39 MB of decode items' partials.)
+  if (fit && have_tiles && !fits_scratch(plan, hkv)) return take_tiles(std::move(tiles_plan));
   c->decode_items = plan.items.size() * hkv;
   auto& p = c->plans[key];
   p = std::move(plan);
@@ -1407,10 +1434,7 @@ int attention_impl(yx_ctx* c, yx_kv* kv, size_t layer, const float* q, float* ou
     if (std::find(c->used_keys.begin(), c->used_keys.end(), key) == c->used_keys.end())
       c->used_keys.push_back(key);
   }
-  // Logical rows per partial slot: the kernel's tile rows.
-  const size_t rps = plan->prefill ? plan->part_rows
-                    : plan->wide    ? static_cast<size_t>((plan->nt + 1) / 2) * 16
-                                    : static_cast<size_t>(plan->nt) * 8;
+  const size_t rps = partial_rows(*plan);
   const size_t po_need = plan->slots * hkv * rps * 128 * 4, pml_need = plan->slots * hkv * rps * 8;
   const size_t cnt_need = plan->counters * hkv * 4 * yx::kCounterStride;
   const void* d_items;
