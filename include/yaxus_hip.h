@@ -192,7 +192,10 @@ int yx_attention_qkv_dev(yx_ctx* ctx, yx_kv* kv, size_t layer, const float* qkv,
 /* attend (backend-cpu lib.rs:389-427; ATTN_SPLIT + ATTN_COMBINE, shaders.rs:1466-1637):
  * causal GQA attention of q `[rows][hq][128]` f32 over each row's keys `[lo, pos]`,
  * lo = pos + 1 - window when window > 0 and pos + 1 > window, else 0. out is
- * `[rows][hq][128]` f32. `scale` multiplies q.k (the reference uses 1/sqrt(128)). */
+ * `[rows][hq][128]` f32. `scale` multiplies q.k (the reference uses 1/sqrt(128)).
+ * Decode items hold at most 32 q heads per KV head (16 of an f32 arena) and a pass of more that
+ * would run as such is refused with YX_ERR_UNSUPPORTED; prefill tiles hold 64 (128 of an f32 or a 4-bit
+ * arena; the latter takes them for such passes of any length). */
 int yx_attention(yx_ctx* ctx, yx_kv* kv, size_t layer, const float* q, float* out, size_t hq,
                  size_t hkv, size_t window, float scale);
 int yx_attention_dev(yx_ctx* ctx, yx_kv* kv, size_t layer, const float* q, float* out,
@@ -218,7 +221,9 @@ int yx_attention_append_dev(yx_ctx* ctx, yx_kv* kv, size_t layer, const float* k
  * yx_pass_begin put on the device when the previous pass made the same call (a decode
  * loop's steady state), else it is sent once per pass into the scratch's list region
  * from the pass's pinned staging. A pass whose work lists or partials do not fit is
- * refused with YX_ERR_UNSUPPORTED. Every call on a GPU shares that GPU's scratch: when a
+ * refused with YX_ERR_UNSUPPORTED (one over a 4-bit arena only after a choice of tiles or
+ * decode items, and of their split, that aims at fitting and may differ from
+ * yx_attention_append_dev's). Every call on a GPU shares that GPU's scratch: when a
  * call comes from another context than the last one, its stream first waits for the
  * other context's stream (an event, no allocation), so contexts take turns; under graph
  * capture such a hand-over cannot be recorded and is refused (make one eager call

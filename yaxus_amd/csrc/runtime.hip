@@ -885,8 +885,9 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
   nt = std::max<size_t>(1, std::min<size_t>(nt, static_cast<size_t>(cap)));
   nt = std::max<size_t>(nt, (G + 7) / 8);  // one row's q heads always fit one work item
   if (f32 && nt > 2) return fail(YX_ERR_UNSUPPORTED, "f32 arena: more than 16 query heads per KV head");
+  // Two tiles of 16 rows are the most a decode item's kernel has.
+  if (nt > 4) return fail(YX_ERR_UNSUPPORTED, "decode items: more than 32 query heads per KV head");
   const size_t rows_per_sub = nt * 8 / G;
-  if (rows_per_sub == 0) return fail(YX_ERR_UNSUPPORTED, "more than 32 query heads per KV head");
 
   struct Sub {
     uint32_t r0, n, pt_off, dev_off, b0, b1;
