@@ -97,7 +97,9 @@ int yx_ctx_set_option(yx_ctx* ctx, const char* key, long value);
  * yx_pass_begin uploaded), "page_runs_sent" (runs of consecutive entries they formed)
  * "prefill_split_tiles" (prefill tiles split along keys in the work lists built) and
  * "prefill_plans" (work lists built as prefill tiles rather than decode items); "decode_items",
- * the items, of all heads, of the latest list of decode items. And of its
+ * the items, of all heads, of the latest list of decode items, "decode_prefixes", the shared
+ * prefixes in it, and "decode_q4_waves", the waves of an item (8 or 4) of the latest such list over a
+ * 4-bit arena. And of its
  * latest yx_matmul_bf16_dev or yx_linear_bf16_dev: "matmul_kernel" (0 none yet, 1 the kernel of 16 x 16 tiles, 2 the
  * one that streams the weight, 3 to 6 LDS tiles of 128 x 256, 128 x 128, 64 x 128, 64 x 64; of
  * yx_linear_bf16_dev also 7, tiles of 96 x 128, and 8, the kernel of few rows), "matmul_k_parts"

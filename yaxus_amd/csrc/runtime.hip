@@ -344,6 +344,8 @@ struct yx_ctx {
   uint64_t pages_sent = 0, runs_sent = 0;        // page-table entries and runs uploaded (tests)
   uint64_t split_tiles = 0;                       // prefill tiles split along keys (tests)
   uint64_t decode_items = 0;                      // items, of all heads, of the latest list of decode items (tests)
+  uint64_t decode_q4_waves = 0;                   // waves an item of the latest such list over a 4-bit arena (tests)
+  uint64_t decode_prefixes = 0;                   // shared prefixes of the latest list of decode items (tests)
   uint64_t prefill_plans = 0;                     // work lists built as prefill tiles (tests)
   bool have_pass = false;
   std::map<PlanKey, AttnPlan> plans;
@@ -1373,6 +1375,8 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
   // (16 x 16 rows after 131072 keys, 16/4 heads: 39 MB of decode items' partials.)
   if (fit && have_tiles && !fits_scratch(plan, hkv)) return take_tiles(std::move(tiles_plan));
   c->decode_items = plan.items.size() * hkv;
+  c->decode_prefixes = cascs.size();
+  if (q4) c->decode_q4_waves = static_cast<uint64_t>(plan.q4_waves);
   auto& p = c->plans[key];
   p = std::move(plan);
   p.cascades = cascs.size();
@@ -2539,6 +2543,10 @@ int yx_ctx_get_stat(yx_ctx* c, const char* key, uint64_t* out) {
     *out = c->prefill_plans;
   else if (!std::strcmp(key, "decode_items"))
     *out = c->decode_items;
+  else if (!std::strcmp(key, "decode_q4_waves"))
+    *out = c->decode_q4_waves;
+  else if (!std::strcmp(key, "decode_prefixes"))
+    *out = c->decode_prefixes;
   else if (!std::strcmp(key, "matmul_kernel"))
     *out = c->mm_kernel;
   else if (!std::strcmp(key, "matmul_k_parts"))
