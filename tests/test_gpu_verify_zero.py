@@ -59,3 +59,31 @@ def test_where_weights_end(hip):
             assert [int(a[0]) for a in c.got()] == ([1, 3] if has else [0, 30])
         finally:
             c.free()
+
+
+@pytest.mark.parametrize("dist", [True, False])
+def test_two_contexts_at_once(hip, dist):
+    """Workgroups of a sequence hand over through a context's own sums and counters: two streams side
+    by side give each call's answers."""
+    from tests.test_gpu_verify_drafts import Call, case
+    from yaxus_amd.backend import HipBackend
+    sides = []
+    try:
+        for seed, counts in ((21, [5, 3, 0, 7]), (22, [2] * 40)):
+            own = HipBackend(0)
+            sides.append((own, Call(own, **case(counts, 30011, seed=seed, dist=dist, noise=1.5))))
+        for own, c in sides:
+            c.run()  # each its scratch
+            own.sync()
+        want = [[a.tolist() for a in c.want()] for _, c in sides]
+        for _ in range(6):
+            for _ in range(4):
+                for _, c in sides:
+                    c.run()
+            for (own, c), w in zip(sides, want):
+                own.sync()
+                assert [a.tolist() for a in c.got()] == w
+    finally:
+        for own, c in sides:
+            c.free()
+            own.close()
