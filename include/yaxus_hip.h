@@ -119,7 +119,8 @@ int yx_ctx_get_stat(yx_ctx* ctx, const char* key, uint64_t* out);
  * prefill_f32_waves of yx_ctx_set_option describe;
  * at most 16 q heads per KV head; write_rows as its own launch) or YX_DTYPE_Q4 (no counterpart
  * in the reference: 72 bytes per head vector, see yx_kv_rows_dev for what it keeps; attention at
- * f32's precision on the values it holds, write_rows as its own launch). */
+ * f32's precision on the values it holds, to about 2^-38 where V is so small; write_rows as its own
+ * launch). */
 int yx_kv_create(yx_ctx* ctx, size_t layers, size_t pages, size_t page_size, size_t hkv,
                  size_t head_dim, int dtype, yx_kv** out);
 int yx_kv_destroy(yx_ctx* ctx, yx_kv* kv);

@@ -57,7 +57,7 @@ def attend(q, k, v, first, last, scale):
     a key at most, a weight times step is cut 2^-21: (keys + 16) 2^-24 of sum w |v|. That cut is
     also absolute, half of binary16's smallest number: with weights scaled to 2^11 (2^-4 where a
     step of V reaches 8) against a largest weight of 1 and codes to 8, 2^-25 8 / 2^11 = 2^-33
-    (2^-18, of values that reach 64) a key.
+    (2^-18, of values that reach 64) a key. (The kernels scale to 2^13 whatever V: 2^-38 |v| a key.)
     """
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
     group = q.shape[1] // k.shape[1]

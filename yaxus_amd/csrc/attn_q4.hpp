@@ -16,6 +16,8 @@
 // 4096: a wave whose result is not finite runs again, once for the steps from 1 up, scaled down,
 // and once for the others, with steps of NaN (or infinite) left out and noted where a row sees them.
 // So does a wave with scores beyond 2^16, whose weights need another form (q4_is_far).
+// Outputs are 3-4e-7 off 64 bits (1500 keys), also of small V down to 1e-5, whose products with codes
+// are subnormal binary16 numbers, of which the matrix unit drops bits: 7e-7 at 3e-6, 2-4e-6 at 1e-6.
 // Steps of keys that no row of the wave sees are cleared at once. So a masked key never has an
 // effect, whatever it holds.
 //
@@ -908,7 +910,7 @@ __global__ __launch_bounds__(64 * kQ4TileWaves) __attribute__((amdgpu_waves_per_
       const int first = static_cast<int>((it.blk0 + b) * 16);
       moved = !weights(st, first, !(first >= rows.all_lo && first + 31 <= rows.all_pos && first + 32 <= key_end));
       if (moved) break;
-        clear(b + 2);
+      clear(b + 2);
       Q4Stage& next = stages[((b >> 1) & 1) ^ 1];
       // V's operands are read a tile ahead, the next pair's are made in the shadow of the products.
       half8 vh = st.v[0][0][lane], vl = st.v[0][1][lane];

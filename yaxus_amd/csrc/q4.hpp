@@ -8,7 +8,8 @@
 // whichever its sign (N(0, 1): 7.6% of the values' root mean square; with a magnitude of at most
 // 7 on both sides 8.7%). A group of zeros, or below binary16's smallest: step 0, codes 8. A
 // group that holds an infinity or NaN: step NaN, codes 8, so each of its values reads NaN and
-// no code ever stands for anything but a small whole number.
+// no code ever stands for anything but a small whole number. (Groups, signed step and offset 8 are those
+// of the published block format Q4_0; ties, limits and byte order are this arena's.)
 //
 // A head vector is 72 bytes (64 of codes, 4 steps; 256 in binary16). Arena layout per layer:
 // `[page][kv_head][block of 16 keys]`, 1152 bytes a block, codes first, steps at 1024. Both

@@ -647,10 +647,11 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
     // The 4-bit arena: decode items (32 logical rows each) take 14 us, or 7 for each of several per CU,
     // and 1.7 ns per pair of blocks over all items; prefill tiles 10 us and 2.1 per pair of the split
     // chosen below. The kernel with the smaller estimate runs. Measured (B x rows after ctx, 16/4 heads,
-    // decode / prefill us): 1 x 512 after 0 21 / 40, 1 x 128 after 4096 33 / 68, 1 x 64 after 32768 66 / 181,
-    // 64 x 16 after 1000 40 / 63, 16 x 24 after 4096 61 / 75, 16 x 64 124 / 109, 4 x 256 after 2000 64 / 74, 16 x
-    // 128 after 1000 75 / 74, 1 x 1024 after 8000 252 / 187; 32/8 heads, 64 x 64 after 64 114 / 48, 2 x 64 after
-    // 16384 152 / 134.
+    // decode / prefill us): 1 x 512 after 0 22 / 40, 1 x 128 after 4096 34 / 67, 1 x 64 after 32768 65 / 178,
+    // 64 x 16 after 1000 40 / 61, 16 x 24 after 4096 60 / 74, 16 x 64 122 / 108, 16 x 128 after 1000 76 / 75,
+    // 1 x 1024 after 8000 244 / 185; 32/8 heads, 64 x 64 after 64 114 / 48, 2 x 64 after 16384 149 / 133. The
+    // estimate takes the slower kernel, tiles, for 4 x 256 after 2000 64 / 73, 1 x 2048 after 0 70 / 78 and 128 x 9
+    // after 600 50 / 55.
     use_prefill = max_rows * G > 32;
     if (use_prefill) {
       double items = 0, pairs = 0;
@@ -1087,7 +1088,8 @@ int build_plan(yx_ctx* c, size_t window, size_t hq, size_t hkv, int form, size_t
   };
   // A 4-bit arena's blocks take a quarter of the time and its items' start as long: 80 blocks (48 of
   // 60-12000 keys 28.8 -> 26.5 us, 64 of 500-1500 22.7 -> 18.0, 64 x 2 rows after 100-3000, 32/8 heads,
-  // 37.9 -> 34.7; 19 of 280-5543, 16/8, 21.3 -> 22.2).
+  // 37.9 -> 34.7; slower: 19 of 280-5543, 16/8, 21.3 -> 22.2). The search counts items of eight waves;
+  // whether they have four is decided for the list it made.
   const uint32_t kStartBlocks = q4 ? 80 : 16;
   const size_t head_slots = std::max<size_t>(1, static_cast<size_t>(c->cus) / hkv);
   auto estimate = [&](size_t cbk, double cutoff) {

@@ -11,7 +11,7 @@
 //
 // The draw's answer is a whole number that hangs on the order of cumulative sums, so weights and
 // sums are 64-bit: with 150 thousand tokens of similar weight, f32's rounding (2^-24 of the whole)
-// would cross the border of one in 50 draws, 64 bits' that of one in 10^10. e^x in 64 bits is a
+// would cross the border of one in 50 draws, weights within 2^-47 that of one in 4 x 10^8. e^x in 64 bits is a
 // polynomial of 12 terms here, about 20 operations a logit: at 64-bit rates 4 us for 80 rows of
 // 151936 logits, less than the 9 us that reading them takes.
 //
