@@ -24,11 +24,11 @@ HOW = {
 class Pass:
     """Sequences of `how`, K by make_k(rows), and a pass of their new rows."""
 
-    def __init__(self, hip, how, make_k):
+    def __init__(self, hip, how, make_k, vscale=1):
         self.priors, self.rows, self.hq, self.hkv, self.min_rows, self.split = HOW[how]
         self.hip, self.make_k = hip, make_k
         pages = sum(-(-(n + self.rows) // 16) for n in self.priors) + 4
-        self.sc = Q4Scenario(hip, pages, 16, self.hkv, pool_seed=3)
+        self.sc = Q4Scenario(hip, pages, 16, self.hkv, pool_seed=3, vscale=vscale)
         seqs = [self.sc.cache.new_seq() for _ in self.priors]
         self.append(list(zip(seqs, self.priors)))
         self.append([(s, self.rows) for s in seqs])
@@ -37,7 +37,7 @@ class Pass:
     def append(self, items):
         self.sc.begin(items)
         t = len(self.sc.meta.pos)
-        k, v = self.make_k(t, self.hkv).astype(np.float32), self.sc.draw(t, self.hkv, D)
+        k, v = self.make_k(t, self.hkv).astype(np.float32), self.sc.draw(t, self.hkv, D) * self.sc.vscale
         self.hip.append(self.sc.kv, 0, k, v)
         self.sc.keep(k, v)
 
@@ -117,6 +117,39 @@ def test_one_key_leads(hip, how, kscale, qscale):
                 else:
                     assert np.abs(got[r, h]).max() <= np.abs(vh).max() * (1 + 2.0 ** -12)
         assert clear > 0.9 * p.n * p.hq
+    finally:
+        p.sc.kv.destroy()
+
+
+@pytest.mark.parametrize("kscale,vscale", [(1, 1), (3e4, 1), (1, 3e5)])
+@pytest.mark.parametrize("how", HOW)
+def test_rows_of_all_sizes_beside_each_other(hip, how, kscale, vscale):
+    """Rows of a tile whose scores are ordinary beside such that are far: the first within the oracle's
+    bound, the others as in test_one_key_leads (V's parts cut 2^-21 too where its steps are large)."""
+    rng = np.random.default_rng(6)
+    p = Pass(hip, how, lambda t, hkv: kscale * rng.standard_normal((t, hkv, D)), vscale)
+    try:
+        size_of = rng.choice([1e-2, 1.0, 1e6, 1e12], (p.n, p.hq, 1)) / kscale
+        q = (size_of * rng.standard_normal((p.n, p.hq, D))).astype(np.float32)
+        got = p.attend(q)
+        assert np.isfinite(got).all()
+        seen = set()
+        for r in range(p.n):
+            k, v = p.seen(r)
+            want, bound = q4.attend(q[r:r + 1], k, v, [0], [len(k) - 1], SCALE)
+            for h in range(p.hq):
+                err = np.abs(got[r, h] - want[0, h])
+                if size_of[r, h] * kscale < 10:
+                    assert (err <= bound[0, h]).all(), (r, h)
+                    seen.add("ordinary")
+                    continue
+                kh, vh, qh = k[:, h * p.hkv // p.hq], v[:, h * p.hkv // p.hq], q[r, h].astype(np.float64)
+                s = kh @ qh * SCALE
+                best = int(s.argmax())
+                if len(s) == 1 or s[best] - np.delete(s, best).max() > 276 * U * (np.abs(kh) @ np.abs(qh)).max() * SCALE + 128:
+                    assert (np.abs(got[r, h] - vh[best]) <= 2.0 ** -19 * np.abs(vh[best]) + len(s) * np.abs(vh).max() * 2.0 ** -33).all(), (r, h)
+                    seen.add("far")
+        assert len(seen) == 2
     finally:
         p.sc.kv.destroy()
 
